@@ -74,6 +74,18 @@ SIGNATURES = {
     "brk_flash_attn_bwd_workspace_bytes": (sz, [i32, i32, i32]),
     "brk_flash_attn_bwd": (i32, [p, p, p, i64, p, p, i64, p, p, p, p, i64, p, p, i32, i32, i32, i32, p, sz, p]),
     "brk_flash_attn_status": (i32, []),
+    "brk_doc_plan": (i32, [p, p, p, i32, i32, p, p, p, p]),
+    "brk_doc_attn_fwd": (i32, [p, p, p, i64, i64, p, i64, p, p, p, f32, i32, i32, i32, i32, i32, p]),
+    "brk_doc_attn_bwd_workspace_bytes": (sz, [i32, i32, i32]),
+    "brk_doc_attn_bwd": (i32, [p, p, p, i64, i64, p, p, i64, p, p, i64, p, p, i64, p, p, f32, i32, i32, i32, i32, i32, p, sz, p]),
+    "brk_doc_attn_status": (i32, []),
+    "brk_act8_pack": (i32, [p, p, p, i64, i64, i32, p]),
+    "brk_act8_unpack": (i32, [p, p, p, i64, i64, i32, p]),
+    "brk_gelu_fwd_act8": (i32, [p, p, p, p, i64, i64, i32, p]),
+    "brk_gelu_bwd_act8": (i32, [p, p, p, p, p, i64, i64, i32, p]),
+    "brk_layernorm_fwd_act8": (i32, [p, p, p, p, p, p, p, i64, i64, f32, i32, p]),
+    "brk_layernorm_bwd_act8_workspace_bytes": (sz, [i64, i64]),
+    "brk_layernorm_bwd_act8": (i32, [p, p, p, p, p, p, p, p, p, p, p, i64, i64, p, sz, i32, i32, p]),
 }
 
 _lib = None

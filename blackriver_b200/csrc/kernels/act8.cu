@@ -1,0 +1,771 @@
+// Activations kept in 8 bits between the forward and the backward pass.
+//
+// A row is cut into blocks of 128 columns (the last one may be shorter).  With top = the largest magnitude of a block
+//     q = rint(x * 127 / top)   (int8),     scale = top / 127   (fp32),     the kept value is q * scale,
+// so a kept value is off by at most half a step, top / 254, of its own block: an outlier column coarsens its 127
+// neighbours in that row and nothing else.  int8 and not an 8-bit float: inside a block of normalised activations the
+// magnitudes span two or three powers of two, and there the uniform step of 1/127 of the largest is finer than the
+// 2^-4 of the value itself that a float with three mantissa bits leaves.  A block that holds an infinity or a NaN gets
+// the scale NaN, so every value of it reads NaN: an overflow stays visible.  A block whose largest magnitude is below
+// 2^-119 (where 127 / top would overflow) is kept as zeros.
+//
+// LayerNorm keeps the normalised row xhat and not y = xhat * gamma + beta: xhat = (y - beta) / gamma would divide the
+// rounding error by gamma.
+//
+// All of it is bound by HBM: one pass, 16-byte accesses, everything that a block shares travels by warp shuffles.
+#include <mutex>
+
+#include "brk_common.cuh"
+
+namespace brk {
+
+constexpr int A8_BLOCK = 128;                 // columns that share a scale
+constexpr int A8_THREADS = 256;
+constexpr float A8_TINY = 1.5046328e-36f;     // 2^-119
+
+// ---- 8-bit arithmetic ----------------------------------------------------------------------------------------------
+
+// largest magnitude as a bit pattern: NaN and infinity order above every number
+__device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+struct A8Scale {
+    float inv, scale;
+};
+__device__ __forceinline__ A8Scale a8_scale(uint32_t top_bits) {
+    A8Scale s;
+    const float top = __uint_as_float(top_bits);
+    if (top_bits >= 0x7f800000u) {
+        s.inv = 0.0f;
+        s.scale = __uint_as_float(0x7fffffffu);
+    } else if (top < A8_TINY) {
+        s.inv = 0.0f;
+        s.scale = 0.0f;
+    } else {
+        s.inv = __fdiv_rn(127.0f, top);
+        s.scale = __fdiv_rn(top, 127.0f);
+    }
+    return s;
+}
+// Four values to four bytes.  Adding 1.5 * 2^23 leaves the nearest integer (ties to even) in the low mantissa bits, and
+// a byte permute gathers them: no conversion instruction, which would run at an eighth of the rate.  With inv == 0 the
+// product is 0, or NaN for a value that is not finite; its low byte is whatever it is, the block's scale is NaN then.
+__device__ __forceinline__ uint32_t a8_pack4(float a, float b, float c, float d, float inv) {
+    const uint32_t ia = __float_as_uint(fmaf(a, inv, 12582912.0f)), ib = __float_as_uint(fmaf(b, inv, 12582912.0f));
+    const uint32_t ic = __float_as_uint(fmaf(c, inv, 12582912.0f)), id = __float_as_uint(fmaf(d, inv, 12582912.0f));
+    return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+}
+// Byte b of a word as the number it stands for: 2^23 + (b + 128) assembled from its bits, exactly.
+template <int B>
+__device__ __forceinline__ float a8_byte(uint32_t flipped) {
+    return __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7440 + B)) - 8388736.0f;
+}
+__device__ __forceinline__ void a8_unpack4(uint32_t w, float scale, float* o) {
+    w ^= 0x80808080u;
+    o[0] = a8_byte<0>(w) * scale;
+    o[1] = a8_byte<1>(w) * scale;
+    o[2] = a8_byte<2>(w) * scale;
+    o[3] = a8_byte<3>(w) * scale;
+}
+
+// ---- N consecutive elements of storage type T ------------------------------------------------------------------------
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T* p, float* o) {
+    constexpr int VN = Vec<T>::N;
+    uint4 raw[N / VN];
+#pragma unroll
+    for (int i = 0; i < N / VN; i++) raw[i] = ld_raw_stream(p + i * VN);
+#pragma unroll
+    for (int i = 0; i < N / VN; i++) {
+        Vec<T> v;
+        v.unpack(raw[i]);
+#pragma unroll
+        for (int e = 0; e < VN; e++) o[i * VN + e] = v.v[e];
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_n(T* p, const float* x) {
+    constexpr int VN = Vec<T>::N;
+#pragma unroll
+    for (int i = 0; i < N / VN; i++) {
+        Vec<T> v;
+#pragma unroll
+        for (int e = 0; e < VN; e++) v.v[e] = x[i * VN + e];
+        v.store_stream(p + i * VN);
+    }
+}
+
+// ---- bloom GELU in fp32: tanh(u) = 1 - 2 / (1 + exp(2u)), absolute error about 1e-7 -----------------------------------
+struct GeluTerms {
+    float y, dy;      // gelu(x) and its derivative
+};
+__device__ __forceinline__ GeluTerms gelu_terms(float x) {
+    const float x2 = x * x;
+    const float t = 1.0f - __fdividef(2.0f, __expf(x * fmaf(2.0f * 0.79788456f * 0.044715f, x2, 2.0f * 0.79788456f)) + 1.0f);
+    const float hx = 0.5f * x;
+    GeluTerms r;
+    r.y = fmaf(hx, t, hx);
+    r.dy = fmaf(hx * fmaf(-t, t, 1.0f), fmaf(3.0f * 0.79788456f * 0.044715f, x2, 0.79788456f), fmaf(0.5f, t, 0.5f));
+    return r;
+}
+
+// ---- pack, and GELU that keeps its input: a thread owns 16 columns, 8 neighbouring lanes a block ----------------------
+// units_per_row counts 16-column units with the last block filled up to 8 of them, so that a block never leaves its lanes.
+template <typename T, bool GELU>
+__global__ void __launch_bounds__(A8_THREADS)
+a8_pack_kernel(const T* x, T* y, int8_t* __restrict__ q, float* __restrict__ scale, int64_t units, int units_per_row, int cols) {
+    pdl_wait();
+    const bool whole = (cols & (A8_BLOCK - 1)) == 0;
+    for (int64_t u = (int64_t)blockIdx.x * A8_THREADS + threadIdx.x; u - threadIdx.x % 32 < units; u += (int64_t)gridDim.x * A8_THREADS) {
+        int64_t at = u * 16;
+        bool live = u < units;
+        if (!whole) {
+            const int64_t row = u / units_per_row;
+            const int c = (int)(u - row * units_per_row) * 16;
+            live = live && c < cols;
+            at = row * cols + c;
+        }
+        float v[16];
+        uint32_t top = 0;
+        if (live) {
+            load_n<T, 16>(x + at, v);
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = max(top, mag_bits(v[e]));
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (live) {
+            const A8Scale s = a8_scale(top);
+            uint4 w;
+            w.x = a8_pack4(v[0], v[1], v[2], v[3], s.inv);
+            w.y = a8_pack4(v[4], v[5], v[6], v[7], s.inv);
+            w.z = a8_pack4(v[8], v[9], v[10], v[11], s.inv);
+            w.w = a8_pack4(v[12], v[13], v[14], v[15], s.inv);
+            __stcs(reinterpret_cast<uint4*>(q + at), w);
+            if ((threadIdx.x & 7) == 0) scale[u >> 3] = s.scale;
+            if (GELU) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) v[e] = gelu_terms(v[e]).y;
+                store_n<T, 16>(y + at, v);
+            }
+        }
+    }
+    pdl_launch_dependents();
+}
+
+// any column count and alignment: a warp owns a block, scalar accesses
+template <typename T, bool GELU>
+__global__ void __launch_bounds__(A8_THREADS)
+a8_pack_generic_kernel(const T* x, T* y, int8_t* q, float* scale, int64_t rows, int blocks, int cols) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t w = ((int64_t)blockIdx.x * A8_THREADS + threadIdx.x) >> 5; w < rows * blocks; w += ((int64_t)gridDim.x * A8_THREADS) >> 5) {
+        const int64_t row = w / blocks;
+        const int c0 = (int)(w - row * blocks) * A8_BLOCK;
+        const int64_t at = row * cols + c0;
+        float v[4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int c = i * 32 + lane;
+            v[i] = c0 + c < cols ? to_f32(x[at + c]) : 0.0f;
+            top = max(top, mag_bits(v[i]));
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        const A8Scale s = a8_scale(top);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int c = i * 32 + lane;
+            if (c0 + c < cols) {
+                q[at + c] = (int8_t)(a8_pack4(v[i], 0.0f, 0.0f, 0.0f, s.inv) & 0xff);
+                if (GELU) y[at + c] = from_f32<T>(gelu_terms(v[i]).y);
+            }
+        }
+        if (lane == 0) scale[w] = s.scale;
+    }
+}
+
+// ---- unpack (DY = false): out = q * scale.  GELU backward: dx = dy * gelu'(q * scale), and gelu(q * scale) again when y --
+template <typename T, bool DY>
+__global__ void __launch_bounds__(A8_THREADS)
+a8_unpack_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, const T* dy, T* out, T* y, int64_t units, int units_per_row, int cols) {
+    pdl_wait();
+    const bool whole = (cols & (A8_BLOCK - 1)) == 0;
+    for (int64_t u = (int64_t)blockIdx.x * A8_THREADS + threadIdx.x; u < units; u += (int64_t)gridDim.x * A8_THREADS) {
+        int64_t at = u * 16;
+        if (!whole) {
+            const int64_t row = u / units_per_row;
+            const int c = (int)(u - row * units_per_row) * 16;
+            if (c >= cols) continue;
+            at = row * cols + c;
+        }
+        const uint4 w = __ldcs(reinterpret_cast<const uint4*>(q + at));
+        const float s = scale[u >> 3];
+        float g[16], v[16];
+        if (DY) load_n<T, 16>(dy + at, g);
+        a8_unpack4(w.x, s, v);
+        a8_unpack4(w.y, s, v + 4);
+        a8_unpack4(w.z, s, v + 8);
+        a8_unpack4(w.w, s, v + 12);
+        if (DY) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const GeluTerms t = gelu_terms(v[e]);
+                g[e] *= t.dy;
+                v[e] = t.y;
+            }
+            store_n<T, 16>(out + at, g);
+            if (y) store_n<T, 16>(y + at, v);
+        } else {
+            store_n<T, 16>(out + at, v);
+        }
+    }
+    pdl_launch_dependents();
+}
+
+template <typename T, bool DY>
+__global__ void __launch_bounds__(A8_THREADS)
+a8_unpack_generic_kernel(const int8_t* q, const float* scale, const T* dy, T* out, T* y, int64_t rows, int blocks, int cols) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t w = ((int64_t)blockIdx.x * A8_THREADS + threadIdx.x) >> 5; w < rows * blocks; w += ((int64_t)gridDim.x * A8_THREADS) >> 5) {
+        const int64_t row = w / blocks;
+        const int c0 = (int)(w - row * blocks) * A8_BLOCK;
+        const int64_t at = row * cols + c0;
+        const float s = scale[w];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int c = i * 32 + lane;
+            if (c0 + c < cols) {
+                const float v = (float)q[at + c] * s;
+                if (DY) {
+                    const GeluTerms t = gelu_terms(v);
+                    out[at + c] = from_f32<T>(to_f32(dy[at + c]) * t.dy);
+                    if (y) y[at + c] = from_f32<T>(t.y);
+                } else {
+                    out[at + c] = from_f32<T>(v);
+                }
+            }
+        }
+    }
+}
+
+static int a8_grid(int64_t threads) {
+    const int64_t want = (threads + A8_THREADS - 1) / A8_THREADS, cap = (int64_t)sm_count() * 16;
+    return (int)(want < cap ? want : cap);
+}
+
+template <typename T, bool GELU>
+static int a8_pack(const void* x, void* y, int8_t* q, float* scale, int64_t rows, int64_t cols, cudaStream_t st) {
+    const int blocks = (int)((cols + A8_BLOCK - 1) / A8_BLOCK);
+    if (cols % 16 == 0 && aligned16(x) && aligned16(q) && (!GELU || aligned16(y))) {
+        const int64_t units = rows * blocks * 8;
+        const cudaError_t e = launch_pdl(a8_pack_kernel<T, GELU>, a8_grid(units), A8_THREADS, 0, st, (const T*)x, (T*)y, q, scale, units, blocks * 8, (int)cols);
+        if (e != cudaSuccess) {
+            set_cuda_error(e, "a8_pack_kernel");
+            return BRK_CUDA_ERROR;
+        }
+        return launch_status("a8_pack_kernel");
+    }
+    a8_pack_generic_kernel<T, GELU><<<a8_grid(rows * blocks * 32), A8_THREADS, 0, st>>>((const T*)x, (T*)y, q, scale, rows, blocks, (int)cols);
+    return launch_status("a8_pack_generic_kernel");
+}
+
+template <typename T, bool DY>
+static int a8_unpack(const int8_t* q, const float* scale, const void* dy, void* out, void* y, int64_t rows, int64_t cols, cudaStream_t st) {
+    const int blocks = (int)((cols + A8_BLOCK - 1) / A8_BLOCK);
+    if (cols % 16 == 0 && aligned16(q) && aligned16(out) && (!DY || aligned16(dy)) && (!y || aligned16(y))) {
+        const int64_t units = rows * blocks * 8;
+        const cudaError_t e = launch_pdl(a8_unpack_kernel<T, DY>, a8_grid(units), A8_THREADS, 0, st, q, scale, (const T*)dy, (T*)out, (T*)y, units, blocks * 8, (int)cols);
+        if (e != cudaSuccess) {
+            set_cuda_error(e, "a8_unpack_kernel");
+            return BRK_CUDA_ERROR;
+        }
+        return launch_status("a8_unpack_kernel");
+    }
+    a8_unpack_generic_kernel<T, DY><<<a8_grid(rows * blocks * 32), A8_THREADS, 0, st>>>(q, scale, (const T*)dy, (T*)out, (T*)y, rows, blocks, (int)cols);
+    return launch_status("a8_unpack_generic_kernel");
+}
+
+// ---- LayerNorm ---------------------------------------------------------------------------------------------------------
+// A thread owns 8 columns, so 16 neighbouring lanes are a block of 128; a row is owned by a team of `team` threads (a
+// multiple of 32, at most 1024: rows of up to 8192 columns), and a CTA holds blockDim.x / team teams that meet at named
+// barriers of their own and never wait for one another.
+constexpr int A8_LN_MAX_COLS = 8192;
+
+__device__ __forceinline__ void team_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// Sum of a and b over the team; red: 64 floats of this team, used alternately by the caller (two buffers) so that one
+// barrier per reduction is enough.
+__device__ __forceinline__ float2 team_sum2(float a, float b, float2* red, int id, int team) {
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if (team == 32) return make_float2(a, b);
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x % team) >> 5, warps = team >> 5;
+    if (lane == 0) red[warp] = make_float2(a, b);
+    team_barrier(id, team);
+    const float2 t = lane < warps ? red[lane] : make_float2(0.0f, 0.0f);
+    return make_float2(warp_sum(t.x), warp_sum(t.y));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024)
+a8_ln_fwd_kernel(const T* x, const T* __restrict__ gamma, const T* __restrict__ beta, T* y, int8_t* __restrict__ q,
+                 float* __restrict__ scale, float* __restrict__ var, int64_t rows, int cols, float eps, int team) {
+    __shared__ float2 red[32][2];            // [warp of the CTA][buffer]: a team uses its own warps' cells
+    const int tid = threadIdx.x % team, group = threadIdx.x / team, groups = blockDim.x / team;
+    const int c = tid * 8, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
+    const bool live = c < cols;
+    const float inv_n = 1.0f / (float)cols;
+    float2* r0 = &red[0][0] + group * (team >> 5);
+    float2* r1 = r0 + 32;
+    float ga[8], be[8];
+    if (live) {
+        load_n<T, 8>(gamma + c, ga);
+        load_n<T, 8>(beta + c, be);
+    }
+    pdl_wait();
+    for (int64_t row = (int64_t)blockIdx.x * groups + group; row < rows; row += (int64_t)gridDim.x * groups) {
+        float v[8];
+        if (live) {
+            load_n<T, 8>(x + row * cols + c, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = 0.0f;
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) s += v[e];
+        const float mu = team_sum2(s, 0.0f, r0, group + 1, team).x * inv_n;
+        float d2 = 0.0f;
+        if (live) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[e] -= mu;
+                d2 = fmaf(v[e], v[e], d2);
+            }
+        }
+        const float va = fmaf(team_sum2(d2, 0.0f, r1, group + 1, team).x, inv_n, eps);
+        const float rstd = rsqrtf(va);
+        uint32_t top = 0;
+        if (live) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[e] *= rstd;
+                top = max(top, mag_bits(v[e]));
+            }
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (live) {
+            const A8Scale sc = a8_scale(top);
+            uint2 w;
+            w.x = a8_pack4(v[0], v[1], v[2], v[3], sc.inv);
+            w.y = a8_pack4(v[4], v[5], v[6], v[7], sc.inv);
+            __stcs(reinterpret_cast<uint2*>(q + row * cols + c), w);
+            if ((threadIdx.x & 15) == 0) scale[row * blocks + (c >> 7)] = sc.scale;
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = fmaf(v[e], ga[e], be[e]);
+            store_n<T, 8>(y + row * cols + c, v);
+        }
+        if (tid == 0) var[row] = va;
+    }
+    pdl_launch_dependents();
+}
+
+// any column count and alignment: one CTA per row, the row read three times
+template <typename T>
+__global__ void __launch_bounds__(A8_THREADS)
+a8_ln_fwd_generic_kernel(const T* x, const T* gamma, const T* beta, T* y, int8_t* q, float* scale, float* var, int cols, float eps) {
+    __shared__ float red[64];
+    const int64_t row = blockIdx.x;
+    const T* xr = x + row * cols;
+    const int blocks = (cols + A8_BLOCK - 1) / A8_BLOCK, lane = threadIdx.x & 31;
+    float s = 0.0f, z = 0.0f;
+    for (int i = threadIdx.x; i < cols; i += A8_THREADS) s += to_f32(xr[i]);
+    block_sum2(s, z, red);
+    const float mu = s / (float)cols;
+    float d2 = 0.0f;
+    z = 0.0f;
+    for (int i = threadIdx.x; i < cols; i += A8_THREADS) {
+        const float d = to_f32(xr[i]) - mu;
+        d2 = fmaf(d, d, d2);
+    }
+    block_sum2(d2, z, red);
+    const float va = d2 / (float)cols + eps, rstd = rsqrtf(va);
+    for (int b = threadIdx.x >> 5; b < blocks; b += A8_THREADS / 32) {
+        float v[4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int c = b * A8_BLOCK + i * 32 + lane;
+            v[i] = c < cols ? (to_f32(xr[c]) - mu) * rstd : 0.0f;
+            top = max(top, mag_bits(v[i]));
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        const A8Scale sc = a8_scale(top);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int c = b * A8_BLOCK + i * 32 + lane;
+            if (c < cols) {
+                q[row * cols + c] = (int8_t)(a8_pack4(v[i], 0.0f, 0.0f, 0.0f, sc.inv) & 0xff);
+                y[row * cols + c] = from_f32<T>(fmaf(v[i], to_f32(gamma[c]), to_f32(beta[c])));
+            }
+        }
+        if (lane == 0) scale[row * blocks + b] = sc.scale;
+    }
+    if (threadIdx.x == 0) var[row] = va;
+}
+
+// Backward.  g = dy * gamma;  dx = rstd * (g - mean(g) - xhat * mean(g * xhat)) (+ residual);  the column sums of
+// dy * xhat and dy stay in the registers of the column's owner over all rows of the CTA, are added over the CTA's teams
+// through shared memory and leave as one row of `part` [gridDim.x][2][cols], which a second kernel adds in order.
+// The next row's packets are fetched before this row's barrier, so a row's latency passes behind the row before it.
+template <typename T, bool RES, bool AGAIN>
+__global__ void __launch_bounds__(1024, 1)
+a8_ln_bwd_kernel(const T* dy, const T* __restrict__ gamma, const T* __restrict__ beta, const float* __restrict__ var,
+                 const int8_t* __restrict__ q, const float* __restrict__ scale, const T* residual, T* dx, T* __restrict__ y,
+                 float* __restrict__ part, int64_t rows, int cols, int team) {
+    constexpr int VN = Vec<T>::N, NP = 8 / VN;
+    extern __shared__ float fold[];          // [teams - 1][2][cols]
+    __shared__ float2 red[2][32];
+    const int tid = threadIdx.x % team, group = threadIdx.x / team, groups = blockDim.x / team;
+    const int c = tid * 8, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
+    const bool live = c < cols;
+    const float inv_n = 1.0f / (float)cols;
+    float2* r0 = red[0] + group * (team >> 5);
+    float2* r1 = red[1] + group * (team >> 5);
+    float dg[8], db[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) dg[e] = db[e] = 0.0f;
+    uint4 gam[NP], bet[NP];                  // kept packed: eight floats each would not fit the registers
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            gam[i] = ld_raw(gamma + c + i * VN);
+            if (AGAIN) bet[i] = ld_raw(beta + c + i * VN);
+        }
+    }
+    pdl_wait();
+
+    uint4 n_dy[NP], n_res[NP];
+    uint2 n_q = make_uint2(0x80808080u, 0x80808080u);
+    float n_scale = 0.0f, n_var = 1.0f;
+    auto fetch = [&](int64_t row) {
+        if (live) {
+            const int64_t at = row * cols + c;
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                n_dy[i] = ld_raw_stream(dy + at + i * VN);
+                if (RES) n_res[i] = ld_raw_stream(residual + at + i * VN);
+            }
+            n_q = __ldcs(reinterpret_cast<const uint2*>(q + at));
+            n_scale = scale[row * blocks + (c >> 7)];
+        }
+        n_var = var[row];
+    };
+    const int64_t step = (int64_t)gridDim.x * groups;
+    int64_t row = (int64_t)blockIdx.x * groups + group;
+    if (row < rows) fetch(row);
+    for (int turn = 0; row < rows; row += step, turn ^= 1) {
+        float xh[8], g[8];
+        uint4 res[NP];
+        const float rstd = rsqrtf(n_var);
+        float a = 0.0f, b = 0.0f;
+        if (live) {
+            a8_unpack4(n_q.x, n_scale, xh);
+            a8_unpack4(n_q.y, n_scale, xh + 4);
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                Vec<T> d, w;
+                d.unpack(n_dy[i]);
+                w.unpack(gam[i]);
+                if (RES) res[i] = n_res[i];
+#pragma unroll
+                for (int e = 0; e < VN; e++) {
+                    const int j = i * VN + e;
+                    dg[j] = fmaf(d.v[e], xh[j], dg[j]);
+                    db[j] += d.v[e];
+                    g[j] = d.v[e] * w.v[e];
+                    a += g[j];
+                    b = fmaf(g[j], xh[j], b);
+                }
+            }
+        }
+        if (row + step < rows) fetch(row + step);
+        const float2 m = team_sum2(a, b, turn ? r1 : r0, group + 1, team);
+        if (live) {
+            const float mg = m.x * inv_n, mgx = m.y * inv_n;
+            const int64_t at = row * cols + c;
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                Vec<T> o, r;
+                if (RES) r.unpack(res[i]);
+#pragma unroll
+                for (int e = 0; e < VN; e++) {
+                    const int j = i * VN + e;
+                    o.v[e] = rstd * (g[j] - mg - xh[j] * mgx);
+                    if (RES) o.v[e] += r.v[e];
+                }
+                o.store_stream(dx + at + i * VN);
+                if (AGAIN) {
+                    Vec<T> w, s;
+                    w.unpack(gam[i]);
+                    s.unpack(bet[i]);
+#pragma unroll
+                    for (int e = 0; e < VN; e++) o.v[e] = fmaf(xh[i * VN + e], w.v[e], s.v[e]);
+                    o.store_stream(y + at + i * VN);
+                }
+            }
+        }
+    }
+    if (groups > 1) {
+        if (group > 0 && live) {
+            float* f = fold + (int64_t)(group - 1) * 2 * cols + c;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f[e] = dg[e];
+                f[cols + e] = db[e];
+            }
+        }
+        __syncthreads();
+        if (group == 0 && live) {
+            for (int k = 0; k < groups - 1; k++) {
+                const float* f = fold + (int64_t)k * 2 * cols + c;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    dg[e] += f[e];
+                    db[e] += f[cols + e];
+                }
+            }
+        }
+    }
+    if (group == 0 && live) {
+        float* p = part + (int64_t)blockIdx.x * 2 * cols + c;
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            *reinterpret_cast<float4*>(p + e) = make_float4(dg[e], dg[e + 1], dg[e + 2], dg[e + 3]);
+            *reinterpret_cast<float4*>(p + cols + e) = make_float4(db[e], db[e + 1], db[e + 2], db[e + 3]);
+        }
+    }
+    pdl_launch_dependents();
+}
+
+// any column count and alignment: a CTA walks rows one at a time, scalar accesses, column sums in its row of `part`
+template <typename T>
+__global__ void __launch_bounds__(A8_THREADS)
+a8_ln_bwd_generic_kernel(const T* dy, const T* gamma, const T* beta, const float* var, const int8_t* q, const float* scale, const T* residual,
+                         T* dx, T* y, float* part, int64_t rows, int cols) {
+    __shared__ float red[64];
+    const int blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
+    float* p = part + (int64_t)blockIdx.x * 2 * cols;
+    for (int i = threadIdx.x; i < 2 * cols; i += A8_THREADS) p[i] = 0.0f;
+    __syncthreads();
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int64_t at = row * cols;
+        float a = 0.0f, b = 0.0f;
+        for (int i = threadIdx.x; i < cols; i += A8_THREADS) {
+            const float xh = (float)q[at + i] * scale[row * blocks + i / A8_BLOCK], d = to_f32(dy[at + i]), g = d * to_f32(gamma[i]);
+            a += g;
+            b = fmaf(g, xh, b);
+            p[i] = fmaf(d, xh, p[i]);              // column i of this CTA's sums belongs to this thread in every row
+            p[cols + i] += d;
+        }
+        block_sum2(a, b, red);
+        const float mg = a / (float)cols, mgx = b / (float)cols, rstd = rsqrtf(var[row]);
+        for (int i = threadIdx.x; i < cols; i += A8_THREADS) {
+            const float xh = (float)q[at + i] * scale[row * blocks + i / A8_BLOCK], w = to_f32(gamma[i]);
+            float o = rstd * (to_f32(dy[at + i]) * w - mg - xh * mgx);
+            if (residual) o += to_f32(residual[at + i]);
+            dx[at + i] = from_f32<T>(o);
+            if (y) y[at + i] = from_f32<T>(fmaf(xh, w, to_f32(beta[i])));
+        }
+    }
+}
+
+// out[j] (+)= sum of part[k][j] in a fixed order: 32 columns per CTA, 8 warps take every 8th partial row each
+template <typename T>
+__global__ void __launch_bounds__(256)
+a8_ln_reduce_kernel(const float* part, T* dgamma, T* dbeta, int parts, int cols, int accumulate) {
+    __shared__ float s[8][33];
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+    float a = 0.0f;
+    if (j < 2 * (int64_t)cols)
+        for (int k = warp; k < parts; k += 8) a += part[(int64_t)k * 2 * cols + j];
+    s[warp][lane] = a;
+    __syncthreads();
+    if (warp == 0 && j < 2 * (int64_t)cols) {
+        for (int k = 1; k < 8; k++) a += s[k][lane];
+        T* o = j < cols ? dgamma + j : dbeta + (j - cols);
+        *o = from_f32<T>(accumulate ? to_f32(*o) + a : a);
+    }
+}
+
+// threads that own a row of `cols` columns, 8 each
+static int a8_team(int64_t cols) { return (int)((cols + 255) / 256) * 32; }
+
+constexpr int A8_MAX_PARTS = 256;             // partial rows of the LayerNorm backward: one per CTA
+
+template <typename T>
+static int a8_ln_fwd(const void* x, const void* gamma, const void* beta, void* y, int8_t* q, float* scale, float* var, int64_t rows, int64_t cols,
+                     float eps, cudaStream_t st) {
+    if (cols % 8 == 0 && cols <= A8_LN_MAX_COLS && aligned16(x) && aligned16(gamma) && aligned16(beta) && aligned16(y) && (reinterpret_cast<uintptr_t>(q) & 7) == 0) {
+        const int team = a8_team(cols), groups = team >= 256 ? 1 : 256 / team;
+        const int64_t want = (rows + groups - 1) / groups, cap = (int64_t)sm_count() * (2048 / (team * groups));
+        const cudaError_t e = launch_pdl(a8_ln_fwd_kernel<T>, (int)(want < cap ? want : cap), team * groups, 0, st, (const T*)x, (const T*)gamma, (const T*)beta,
+                                         (T*)y, q, scale, var, rows, (int)cols, eps, team);
+        if (e != cudaSuccess) {
+            set_cuda_error(e, "a8_ln_fwd_kernel");
+            return BRK_CUDA_ERROR;
+        }
+        return launch_status("a8_ln_fwd_kernel");
+    }
+    a8_ln_fwd_generic_kernel<T><<<(unsigned)rows, A8_THREADS, 0, st>>>((const T*)x, (const T*)gamma, (const T*)beta, (T*)y, q, scale, var, (int)cols, eps);
+    return launch_status("a8_ln_fwd_generic_kernel");
+}
+
+template <typename T, bool RES, bool AGAIN>
+static cudaError_t a8_launch_ln_bwd(int grid, int block, size_t smem, cudaStream_t st, const T* dy, const T* gamma, const T* beta, const float* var,
+                                    const int8_t* q, const float* scale, const T* residual, T* dx, T* y, float* part, int64_t rows, int cols, int team) {
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(a8_ln_bwd_kernel<T, RES, AGAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pdl(a8_ln_bwd_kernel<T, RES, AGAIN>, grid, block, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, cols, team);
+}
+
+template <typename T>
+static int a8_ln_bwd(const void* dy_, const void* gamma_, const void* beta_, const float* var, const int8_t* q, const float* scale, const void* residual_,
+                     void* dgamma, void* dbeta, void* dx_, void* y_, int64_t rows, int64_t cols, float* part, int accumulate, cudaStream_t st) {
+    const T *dy = (const T*)dy_, *gamma = (const T*)gamma_, *beta = (const T*)beta_, *residual = (const T*)residual_;
+    T *dx = (T*)dx_, *y = (T*)y_;
+    int parts;
+    if (cols % 8 == 0 && cols <= A8_LN_MAX_COLS && aligned16(dy) && aligned16(gamma) && aligned16(dx) && aligned16(part) && (!residual || aligned16(residual)) &&
+        (!y || (aligned16(y) && aligned16(beta))) && (reinterpret_cast<uintptr_t>(q) & 7) == 0) {
+        const int team = a8_team(cols);
+        int groups = 1024 / team;
+        if ((int64_t)groups * sm_count() > rows) groups = (int)((rows + sm_count() - 1) / sm_count());      // few rows: spread them over the SMs
+        if (groups > 15) groups = 15;                                                                      // named barriers 1..15
+        const int64_t want = (rows + groups - 1) / groups;
+        int grid = sm_count() < A8_MAX_PARTS ? sm_count() : A8_MAX_PARTS;
+        if (want < grid) grid = (int)want;
+        const size_t smem = (size_t)(groups - 1) * 2 * cols * sizeof(float);
+        cudaError_t e;
+        if (residual)
+            e = y ? a8_launch_ln_bwd<T, true, true>(grid, team * groups, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team)
+                  : a8_launch_ln_bwd<T, true, false>(grid, team * groups, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team);
+        else
+            e = y ? a8_launch_ln_bwd<T, false, true>(grid, team * groups, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team)
+                  : a8_launch_ln_bwd<T, false, false>(grid, team * groups, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team);
+        if (e != cudaSuccess) {
+            set_cuda_error(e, "a8_ln_bwd_kernel");
+            return BRK_CUDA_ERROR;
+        }
+        const int rc = launch_status("a8_ln_bwd_kernel");
+        if (rc) return rc;
+        parts = grid;
+    } else {
+        parts = (int)(rows < A8_MAX_PARTS ? rows : A8_MAX_PARTS);
+        a8_ln_bwd_generic_kernel<T><<<parts, A8_THREADS, 0, st>>>(dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols);
+        const int rc = launch_status("a8_ln_bwd_generic_kernel");
+        if (rc) return rc;
+    }
+    const cudaError_t e = launch_pdl(a8_ln_reduce_kernel<T>, (int)((2 * cols + 31) / 32), 256, 0, st, (const float*)part, (T*)dgamma, (T*)dbeta, parts, (int)cols, accumulate);
+    if (e != cudaSuccess) {
+        set_cuda_error(e, "a8_ln_reduce_kernel");
+        return BRK_CUDA_ERROR;
+    }
+    return launch_status("a8_ln_reduce_kernel");
+}
+
+static bool a8_sizes_ok(int64_t rows, int64_t cols) { return rows >= 0 && cols > 0 && rows <= 0x7fffffff && cols <= (1 << 24); }
+
+}  // namespace brk
+
+using namespace brk;
+
+extern "C" int brk_act8_pack(const void* x, int8_t* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream) {
+    if (!a8_sizes_ok(rows, cols)) return BRK_ATTR_ERROR;
+    if (dtype != BRK_F32 && dtype != BRK_F16) return BRK_ATTR_ERROR;
+    if (rows == 0) return BRK_OK;
+    if (!x) return BRK_INPUT_ERROR;
+    if (!q || !scale) return BRK_OUTPUT_ERROR;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == BRK_F32) return a8_pack<float, false>(x, nullptr, q, scale, rows, cols, st);
+    return a8_pack<__half, false>(x, nullptr, q, scale, rows, cols, st);
+}
+
+extern "C" int brk_act8_unpack(const int8_t* q, const float* scale, void* out, int64_t rows, int64_t cols, int dtype, void* stream) {
+    if (!a8_sizes_ok(rows, cols)) return BRK_ATTR_ERROR;
+    if (dtype != BRK_F32 && dtype != BRK_F16) return BRK_ATTR_ERROR;
+    if (rows == 0) return BRK_OK;
+    if (!q || !scale) return BRK_INPUT_ERROR;
+    if (!out) return BRK_OUTPUT_ERROR;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == BRK_F32) return a8_unpack<float, false>(q, scale, nullptr, out, nullptr, rows, cols, st);
+    return a8_unpack<__half, false>(q, scale, nullptr, out, nullptr, rows, cols, st);
+}
+
+extern "C" int brk_gelu_fwd_act8(const void* x, void* y, int8_t* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream) {
+    if (!a8_sizes_ok(rows, cols)) return BRK_ATTR_ERROR;
+    if (dtype != BRK_F32 && dtype != BRK_F16) return BRK_ATTR_ERROR;
+    if (rows == 0) return BRK_OK;
+    if (!x) return BRK_INPUT_ERROR;
+    if (!y || !q || !scale) return BRK_OUTPUT_ERROR;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == BRK_F32) return a8_pack<float, true>(x, y, q, scale, rows, cols, st);
+    return a8_pack<__half, true>(x, y, q, scale, rows, cols, st);
+}
+
+extern "C" int brk_gelu_bwd_act8(const void* dy, const int8_t* q, const float* scale, void* dx, void* y, int64_t rows, int64_t cols, int dtype, void* stream) {
+    if (!a8_sizes_ok(rows, cols)) return BRK_ATTR_ERROR;
+    if (dtype != BRK_F32 && dtype != BRK_F16) return BRK_ATTR_ERROR;
+    if (rows == 0) return BRK_OK;
+    if (!dy || !q || !scale) return BRK_INPUT_ERROR;
+    if (!dx) return BRK_OUTPUT_ERROR;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == BRK_F32) return a8_unpack<float, true>(q, scale, dy, dx, y, rows, cols, st);
+    return a8_unpack<__half, true>(q, scale, dy, dx, y, rows, cols, st);
+}
+
+extern "C" int brk_layernorm_fwd_act8(const void* x, const void* gamma, const void* beta, void* y, int8_t* q, float* scale, float* var, int64_t rows,
+                                      int64_t hidden, float eps, int dtype, void* stream) {
+    if (!a8_sizes_ok(rows, hidden) || !(eps >= 0.0f)) return BRK_ATTR_ERROR;
+    if (dtype != BRK_F32 && dtype != BRK_F16) return BRK_ATTR_ERROR;
+    if (rows == 0) return BRK_OK;
+    if (!x || !gamma || !beta) return BRK_INPUT_ERROR;
+    if (!y || !q || !scale || !var) return BRK_OUTPUT_ERROR;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == BRK_F32) return a8_ln_fwd<float>(x, gamma, beta, y, q, scale, var, rows, hidden, eps, st);
+    return a8_ln_fwd<__half>(x, gamma, beta, y, q, scale, var, rows, hidden, eps, st);
+}
+
+extern "C" size_t brk_layernorm_bwd_act8_workspace_bytes(int64_t rows, int64_t hidden) {
+    if (rows <= 0 || hidden <= 0) return 0;
+    return (size_t)(rows < A8_MAX_PARTS ? rows : A8_MAX_PARTS) * 2 * (size_t)hidden * sizeof(float);
+}
+
+extern "C" int brk_layernorm_bwd_act8(const void* dy, const void* gamma, const void* beta, const float* var, const int8_t* q, const float* scale,
+                                      const void* residual, void* dgamma, void* dbeta, void* dx, void* y, int64_t rows, int64_t hidden, void* workspace,
+                                      size_t workspace_bytes, int accumulate, int dtype, void* stream) {
+    if (!a8_sizes_ok(rows, hidden)) return BRK_ATTR_ERROR;
+    if (dtype != BRK_F32 && dtype != BRK_F16) return BRK_ATTR_ERROR;
+    if (!gamma || (y && !beta)) return BRK_INPUT_ERROR;
+    if (!dgamma || !dbeta) return BRK_OUTPUT_ERROR;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (rows == 0) {                          // no rows: the sums are zero
+        if (accumulate) return BRK_OK;
+        const size_t bytes = (size_t)hidden * (dtype == BRK_F32 ? 4 : 2);
+        cudaError_t e = cudaMemsetAsync(dgamma, 0, bytes, st);
+        if (e == cudaSuccess) e = cudaMemsetAsync(dbeta, 0, bytes, st);
+        if (e != cudaSuccess) {
+            set_cuda_error(e, "layernorm_bwd_act8 clear");
+            return BRK_CUDA_ERROR;
+        }
+        return BRK_OK;
+    }
+    if (!dy || !var || !q || !scale) return BRK_INPUT_ERROR;
+    if (!dx) return BRK_OUTPUT_ERROR;
+    if (!workspace || workspace_bytes < brk_layernorm_bwd_act8_workspace_bytes(rows, hidden) || (reinterpret_cast<uintptr_t>(workspace) & 3)) return BRK_ATTR_ERROR;
+    if (dtype == BRK_F32) return a8_ln_bwd<float>(dy, gamma, beta, var, q, scale, residual, dgamma, dbeta, dx, y, rows, hidden, (float*)workspace, accumulate, st);
+    return a8_ln_bwd<__half>(dy, gamma, beta, var, q, scale, residual, dgamma, dbeta, dx, y, rows, hidden, (float*)workspace, accumulate, st);
+}

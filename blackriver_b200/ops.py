@@ -212,6 +212,211 @@ def gemm_f16(a, b, c, m, n, k, trans_a, trans_b, lda, ldb, ldc, bias=None, resid
     return c
 
 
+# --- packed documents ---
+def _chk_all(expect, **named):
+    """Each tensor (None passes): contiguous, on the current device, of its dtype and shape in `expect`."""
+    for name, t in named.items():
+        if t is None:
+            continue
+        _chk(t)
+        _chk_device(t)
+        dtype, shape = expect[name]
+        if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _chk_device(t):
+    if t.device.index != torch.cuda.current_device():
+        raise RuntimeError("tensors must live on the current device, whose stream the kernels are queued on")
+
+
+def doc_plan(mask, prompt=None, ids=None):
+    """Spans of packed documents: mask [batch, tokens] int32 numbers the documents (0 or less = padding), prompt marks
+    the tokens of prompts.  Returns int32 spans [batch, tokens, 4] for doc_attn; with ids also the loss targets and their
+    count: (spans, target, count)."""
+    if mask.dim() != 2:
+        raise ValueError("mask must be [batch, tokens]")
+    like = (torch.int32, mask.shape)
+    _chk_all({"mask": like, "prompt": like, "ids": like}, mask=mask, prompt=prompt, ids=ids)
+    b, t = mask.shape
+    spans = torch.empty((b, t, 4), dtype=torch.int32, device=mask.device)
+    target = count = None
+    if ids is not None:
+        target = torch.empty_like(ids)
+        count = torch.empty(1, dtype=torch.int32, device=ids.device)
+    brk.call("brk_doc_plan", _ptr(mask), _ptr(prompt), _ptr(ids), b, t, _ptr(spans), _ptr(target), _ptr(count), stream())
+    return spans if ids is None else (spans, target, count)
+
+
+def _heads_view(name, t, batch, tokens, heads, dim):
+    """Row stride of a [batch, tokens, heads, head_dim] fp16 tensor whose heads lie side by side in a token's row."""
+    if not t.is_cuda:
+        raise RuntimeError("blackriver_b200 operators run on CUDA tensors only (no CPU path)")
+    _chk_device(t)
+    if t.dtype != torch.float16:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    if t.dim() != 4 or t.shape[0] != batch or t.shape[1] != tokens or t.shape[3] != dim or (heads is not None and t.shape[2] != heads):
+        raise ValueError(f"{name} must be [{batch}, {tokens}, {heads or 'heads'}, {dim}], got {tuple(t.shape)}")
+    ld = t.stride(1) if tokens > 1 else t.stride(0) if batch > 1 else t.shape[2] * dim
+    if t.numel() and ((dim > 1 and t.stride(3) != 1) or (t.shape[2] > 1 and t.stride(2) != dim) or (batch > 1 and t.stride(0) != tokens * ld)):
+        raise ValueError(f"{name}: heads must lie side by side and tokens at one stride")
+    return ld
+
+
+def _doc_args(q, k, v, spans, slopes):
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q, k and v must be [batch, tokens, heads, head_dim]")
+    b, t, h, d = q.shape
+    hk = k.shape[2]
+    ld_q, ld_kv = _heads_view("q", q, b, t, h, d), _heads_view("k", k, b, t, hk, d)
+    if _heads_view("v", v, b, t, hk, d) != ld_kv:
+        raise ValueError("k and v must have the same row stride")
+    _chk_all({"spans": (torch.int32, (b, t, 4)), "slopes": (torch.float32, (h,))}, spans=spans, slopes=slopes)
+    return b, t, h, hk, d, ld_q, ld_kv
+
+
+def doc_attn(q, k, v, spans, slopes=None, cap=0.0, out=None, lse=None):
+    """Attention over packed documents: q [batch, tokens, heads, head_dim], k and v [batch, tokens, kv_heads, head_dim]
+    fp16 (views of a fused projection are read in place), spans from doc_plan.  slopes [heads]: bias -slope * distance;
+    cap: scores capped by cap * tanh(score / cap).  Returns (out, lse [batch, heads, tokens])."""
+    b, t, h, hk, d, ld_q, ld_kv = _doc_args(q, k, v, spans, slopes)
+    out = torch.empty((b, t, h, d), dtype=q.dtype, device=q.device) if out is None else out
+    lse = torch.empty((b, h, t), dtype=torch.float32, device=q.device) if lse is None else lse
+    ld_out = _heads_view("out", out, b, t, h, d)
+    _chk_all({"lse": (torch.float32, (b, h, t))}, lse=lse)
+    brk.call("brk_doc_attn_fwd", _ptr(q), _ptr(k), _ptr(v), ld_q, ld_kv, _ptr(out), ld_out, _ptr(lse), _ptr(spans), _ptr(slopes), float(cap),
+             b, t, h, hk, d, stream())
+    return out, lse
+
+
+def doc_attn_backward(d_out, q, k, v, out, lse, spans, slopes=None, cap=0.0, dq=None, dk=None, dv=None, workspace=None):
+    """Gradients (dq, dk, dv) of doc_attn; without dq, dk and dv they are views of one fused [batch, tokens, heads + 2 kv_heads,
+    head_dim] buffer, as the projection's backward wants them."""
+    b, t, h, hk, d, ld_q, ld_kv = _doc_args(q, k, v, spans, slopes)
+    ld_out = _heads_view("out", out, b, t, h, d)
+    if _heads_view("d_out", d_out, b, t, h, d) != ld_out:
+        raise ValueError("out and d_out must have the same row stride")
+    _chk_all({"lse": (torch.float32, (b, h, t))}, lse=lse)
+    if dq is None and dk is None and dv is None:
+        fused = torch.empty((b, t, h + 2 * hk, d), dtype=q.dtype, device=q.device)
+        dq, dk, dv = fused[:, :, :h], fused[:, :, h:h + hk], fused[:, :, h + hk:]
+    elif dq is None or dk is None or dv is None:
+        raise ValueError("give all of dq, dk and dv, or none")
+    ld_dq, ld_dkv = _heads_view("dq", dq, b, t, h, d), _heads_view("dk", dk, b, t, hk, d)
+    if _heads_view("dv", dv, b, t, hk, d) != ld_dkv:
+        raise ValueError("dk and dv must have the same row stride")
+    if workspace is None:
+        workspace = torch.empty(max(brk.lib().brk_doc_attn_bwd_workspace_bytes(b, t, h), 16), dtype=torch.uint8, device=q.device)
+    _chk(workspace)
+    _chk_device(workspace)
+    brk.call("brk_doc_attn_bwd", _ptr(q), _ptr(k), _ptr(v), ld_q, ld_kv, _ptr(out), _ptr(d_out), ld_out, _ptr(lse), _ptr(dq), ld_dq, _ptr(dk),
+             _ptr(dv), ld_dkv, _ptr(spans), _ptr(slopes), float(cap), b, t, h, hk, d, _ptr(workspace), workspace.numel() * workspace.element_size(), stream())
+    return dq, dk, dv
+
+
+# --- activations kept in 8 bits ---
+ACT8_BLOCK = 128        # columns that share a scale
+
+
+def _act8_shapes(rows, cols):
+    return {"q": (torch.int8, (rows, cols)), "scale": (torch.float32, (rows, -(-cols // ACT8_BLOCK)))}
+
+
+def _act8_new(rows, cols, device):
+    return (torch.empty((rows, cols), dtype=torch.int8, device=device),
+            torch.empty((rows, -(-cols // ACT8_BLOCK)), dtype=torch.float32, device=device))
+
+
+def _rows_cols(t):
+    if t.dim() < 1 or t.shape[-1] == 0:
+        raise ValueError("activations need at least one column")
+    return t.numel() // t.shape[-1], t.shape[-1]
+
+
+def act8_pack(x):
+    """x [..., cols] -> (q int8 [rows, cols], scale fp32 [rows, ceil(cols / 128)])."""
+    _chk(x)
+    _chk_device(x)
+    rows, cols = _rows_cols(x)
+    q, scale = _act8_new(rows, cols, x.device)
+    brk.call("brk_act8_pack", _ptr(x), _ptr(q), _ptr(scale), rows, cols, _dt(x), stream())
+    return q, scale
+
+
+def act8_unpack(q, scale, dtype=torch.float16, out=None):
+    """The kept values, [rows, cols] of `dtype` (or into out)."""
+    rows, cols = _rows_cols(q)
+    _chk_all(_act8_shapes(rows, cols), q=q, scale=scale)
+    out = torch.empty((rows, cols), dtype=dtype, device=q.device) if out is None else out
+    _chk_all({"out": (out.dtype, q.shape)}, out=out)
+    brk.call("brk_act8_unpack", _ptr(q), _ptr(scale), _ptr(out), rows, cols, _dt(out), stream())
+    return out
+
+
+def gelu_act8(x, out=None):
+    """gelu(x) and x kept in 8 bits: (y, q, scale)."""
+    _chk(x, out)
+    _chk_device(x)
+    rows, cols = _rows_cols(x)
+    y = torch.empty_like(x) if out is None else out
+    _chk_all({"out": (x.dtype, x.shape)}, out=y)
+    q, scale = _act8_new(rows, cols, x.device)
+    brk.call("brk_gelu_fwd_act8", _ptr(x), _ptr(y), _ptr(q), _ptr(scale), rows, cols, _dt(x), stream())
+    return y, q, scale
+
+
+def gelu_backward_act8(dy, q, scale, out=None, recompute=False):
+    """dy * gelu'(kept x); with recompute also gelu(kept x) again: dx, or (dx, y)."""
+    _chk(dy, out)
+    _chk_device(dy)
+    rows, cols = _rows_cols(dy)
+    _chk_all(_act8_shapes(rows, cols), q=q, scale=scale)
+    dx = torch.empty_like(dy) if out is None else out
+    _chk_all({"out": (dy.dtype, dy.shape)}, out=dx)
+    y = torch.empty_like(dy) if recompute else None
+    brk.call("brk_gelu_bwd_act8", _ptr(dy), _ptr(q), _ptr(scale), _ptr(dx), _ptr(y), rows, cols, _dt(dy), stream())
+    return (dx, y) if recompute else dx
+
+
+def layernorm_act8(x, gamma, beta, eps=1e-5, out=None):
+    """LayerNorm that keeps the normalised rows in 8 bits: (y, q, scale, var)."""
+    _chk(x, out)
+    _chk_device(x)
+    rows, cols = _rows_cols(x)
+    vec = (x.dtype, (cols,))
+    _chk_all({"gamma": vec, "beta": vec}, gamma=gamma, beta=beta)
+    y = torch.empty_like(x) if out is None else out
+    _chk_all({"out": (x.dtype, x.shape)}, out=y)
+    q, scale = _act8_new(rows, cols, x.device)
+    var = torch.empty(rows, dtype=torch.float32, device=x.device)
+    brk.call("brk_layernorm_fwd_act8", _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(q), _ptr(scale), _ptr(var), rows, cols, eps, _dt(x), stream())
+    return y, q, scale, var
+
+
+def layernorm_backward_act8(dy, gamma, var, q, scale, beta=None, residual=None, dgamma=None, dbeta=None, dx=None, accumulate=False, workspace=None):
+    """LayerNorm backward from the kept rows: (dgamma, dbeta, dx), and with beta the forward's output again as a fourth."""
+    _chk(dy)
+    _chk_device(dy)
+    rows, cols = _rows_cols(dy)
+    if accumulate and (dgamma is None or dbeta is None):
+        raise ValueError("accumulate needs dgamma and dbeta")
+    vec, full = (dy.dtype, (cols,)), (dy.dtype, dy.shape)
+    dgamma = torch.empty(cols, dtype=dy.dtype, device=dy.device) if dgamma is None else dgamma
+    dbeta = torch.empty(cols, dtype=dy.dtype, device=dy.device) if dbeta is None else dbeta
+    dx = torch.empty_like(dy) if dx is None else dx
+    y = torch.empty_like(dy) if beta is not None else None
+    _chk_all({"gamma": vec, "beta": vec, "dgamma": vec, "dbeta": vec, "var": (torch.float32, (rows,)), "residual": full, "dx": full, **_act8_shapes(rows, cols)},
+             gamma=gamma, beta=beta, dgamma=dgamma, dbeta=dbeta, var=var, residual=residual, dx=dx, q=q, scale=scale)
+    need = brk.lib().brk_layernorm_bwd_act8_workspace_bytes(rows, cols)
+    if workspace is None:
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dy.device)
+    _chk(workspace)
+    _chk_device(workspace)
+    brk.call("brk_layernorm_bwd_act8", _ptr(dy), _ptr(gamma), _ptr(beta), _ptr(var), _ptr(q), _ptr(scale), _ptr(residual), _ptr(dgamma), _ptr(dbeta), _ptr(dx),
+             _ptr(y), rows, cols, _ptr(workspace), workspace.numel() * workspace.element_size(), int(accumulate), _dt(dy), stream())
+    return (dgamma, dbeta, dx) if y is None else (dgamma, dbeta, dx, y)
+
+
 # --- operator-level compositions with the reference's semantics (blackriver/cuda_tensor.cpp) ---
 def linear(x, w, bias, out=None):
     """op_linear (:147-193): y[n,o] = sum_i x[n,i] w[o,i] + b[o]."""

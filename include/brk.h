@@ -266,6 +266,73 @@ BRK_API int brk_flash_attn_bwd(const void* q, const void* k, const void* v, int6
                        void* workspace, size_t workspace_bytes, void* stream);
 BRK_API int brk_flash_attn_status(void);
 
+/* ---- packed documents ---------------------------------------------------------------------------
+ * Several documents in one row of the batch, for fine-tuning on prompts and answers without padding.  Nothing of the kind
+ * exists in the reference, whose rows hold one right-padded sequence (blackriver/train_bloom.cpp:58-90).
+ *
+ * brk_doc_plan: mask [batch, tokens] numbers the documents (0 or less = padding; with the 0/1 mask of the other calls a
+ * row is one document); a run of equal numbers is one document, so neighbouring documents carry different numbers.
+ * prompt (or NULL) is non-zero on tokens of a prompt; the leading ones of a document see each other in both directions.
+ * spans [batch, tokens, 4] receives, as positions in the row: keys [lo, hi) the token sees as a query, queries [qlo, qhi)
+ * that see it as a key; a token of padding gets the empty span at the start of its run.
+ * target (or NULL; needs ids [batch, tokens]) receives ids[b, t+1] where t+1 belongs to the same document and is not
+ * marked in `prompt`, else -100: what brk_loss_targets does for a 0/1 mask.  count (or NULL; needs target) receives the
+ * number of targets.  batch * tokens <= 2^30; spans 16-byte aligned. */
+BRK_API int brk_doc_plan(const int32_t* mask, const int32_t* prompt, const int32_t* ids, int batch, int tokens, int32_t* spans,
+                 int32_t* target, int32_t* count, void* stream);
+
+/* Attention over packed documents (fp16, tcgen05):
+ *     x = Q K^T / sqrt(d);   s = cap * tanh(x / cap) when cap > 0, else x;   s -= slopes[h] * |query - key| when slopes
+ *     P = softmax(s) over the keys lo <= key < hi of the query's span,   out = P V
+ * q, out, d_out, dq: token-major fp16, head h at columns h*head_dim of a row, row strides ld_q, ld_out, ld_out, ld_dq; k, v and
+ * dk, dv: kv_heads heads, row strides ld_kv and ld_dkv (thirds of one fused buffer, or tensors of their own).  heads is a
+ * multiple of kv_heads; query head h reads key head h / (heads / kv_heads), whose gradient is the sum over its query heads.
+ * spans [batch, tokens, 4] as brk_doc_plan makes them: inside a row none of the four falls from a token to the next (other
+ * values give wrong sums, never an access outside the tensors).  slopes [heads] fp32 or NULL; 0 <= cap <= 10000, 0 = none.
+ * A query that sees nothing (padding) has out = 0, lse = 0 and no gradient, a key that nobody sees has gradient 0; all rows of
+ * the outputs are written.  What a query does not see does not reach it, NaN and infinity included.
+ * lse [batch, heads, tokens] fp32, natural log (NULL when no backward follows).  The gradients are the same from run to run.
+ * head_dim 64 or 128, tokens <= 2^22, batch * tokens <= 2^30, strides multiples of 8, pointers 16-byte aligned.
+ * The backward's workspace is brk_doc_attn_bwd_workspace_bytes() of device scratch; calls that may run at the same time
+ * need one each.  brk_doc_attn_status() (synchronous) returns non-zero if a kernel gave up on a bounded wait. */
+BRK_API int brk_doc_attn_fwd(const void* q, const void* k, const void* v, int64_t ld_q, int64_t ld_kv, void* out, int64_t ld_out,
+                     float* lse, const int32_t* spans, const float* slopes, float cap, int batch, int tokens, int heads,
+                     int kv_heads, int head_dim, void* stream);
+BRK_API size_t brk_doc_attn_bwd_workspace_bytes(int batch, int tokens, int heads);
+BRK_API int brk_doc_attn_bwd(const void* q, const void* k, const void* v, int64_t ld_q, int64_t ld_kv, const void* out,
+                     const void* d_out, int64_t ld_out, const float* lse, void* dq, int64_t ld_dq, void* dk, void* dv,
+                     int64_t ld_dkv, const int32_t* spans, const float* slopes, float cap, int batch, int tokens, int heads,
+                     int kv_heads, int head_dim, void* workspace, size_t workspace_bytes, void* stream);
+BRK_API int brk_doc_attn_status(void);
+
+/* ---- activations kept in 8 bits --------------------------------------------------------------------
+ * What the backward pass reads of the forward's activations, at half the bytes (the reference keeps them in fp32,
+ * bloomz-7b/train.words:10-135).  Each block of 128 columns of a row (the last may be shorter) has one scale:
+ *     top = largest magnitude of the block,  q = rint(x * 127 / top),  scale = top / 127,  kept value = q * scale
+ * q [rows, cols] int8, scale [rows, ceil(cols / 128)] fp32.  A block with an infinity or a NaN gets the scale NaN (all of
+ * it reads NaN); one whose largest magnitude is below 2^-119 is kept as zeros.  Any cols; cols a multiple of 16 (LayerNorm: 8
+ * and at most 8192) with 16-byte aligned pointers takes the wide paths.  `dtype` is the storage type of all other tensors. */
+BRK_API int brk_act8_pack(const void* x, int8_t* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream);
+BRK_API int brk_act8_unpack(const int8_t* q, const float* scale, void* out, int64_t rows, int64_t cols, int dtype, void* stream);
+/* y = bloom_gelu(x) and x kept, in one pass; y may alias x. */
+BRK_API int brk_gelu_fwd_act8(const void* x, void* y, int8_t* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream);
+/* dx = dy * bloom_gelu'(kept x), and (y not NULL) y = bloom_gelu(kept x) again, the operand of the next layer's weight gradient;
+ * dx may alias dy. */
+BRK_API int brk_gelu_bwd_act8(const void* dy, const int8_t* q, const float* scale, void* dx, void* y, int64_t rows, int64_t cols, int dtype,
+                      void* stream);
+/* brk_layernorm_fwd that also keeps the normalised row xhat = (x - mean) / sqrt(var) (not y: recovering xhat from y would
+ * divide the rounding by gamma).  var [rows] = biased variance + eps.  y may alias x. */
+BRK_API int brk_layernorm_fwd_act8(const void* x, const void* gamma, const void* beta, void* y, int8_t* q, float* scale, float* var, int64_t rows,
+                           int64_t hidden, float eps, int dtype, void* stream);
+/* Backward from the kept xhat: dx = (g - mean(g) - xhat * mean(g * xhat)) / sqrt(var) (+ residual), g = dy * gamma; dgamma, dbeta
+ * [hidden] overwritten, or added to when `accumulate` != 0 (sums in a fixed order); y (not NULL; needs beta) = xhat * gamma + beta
+ * again, the operand of the next layer's weight gradient.  residual may be NULL; dx may alias dy or residual.  Workspace of
+ * brk_layernorm_bwd_act8_workspace_bytes(), one for each call that may run at the same time. */
+BRK_API size_t brk_layernorm_bwd_act8_workspace_bytes(int64_t rows, int64_t hidden);
+BRK_API int brk_layernorm_bwd_act8(const void* dy, const void* gamma, const void* beta, const float* var, const int8_t* q, const float* scale,
+                           const void* residual, void* dgamma, void* dbeta, void* dx, void* y, int64_t rows, int64_t hidden,
+                           void* workspace, size_t workspace_bytes, int accumulate, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,324 @@
+"""Attention over packed documents and the plan that feeds it, against plain 64-bit forms."""
+import random
+
+import pytest
+import torch
+
+from tests import doc_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def ops():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need a CUDA device")
+    from blackriver_b200 import ops
+    return ops
+
+
+def status():
+    from blackriver_b200 import brk
+    torch.cuda.synchronize()
+    return brk.lib().brk_doc_attn_status()
+
+
+def rows(batch, tokens, docs, seed, prompts=True):
+    """mask and prompt lists: per row the document lengths in docs (negative: padding), cut or padded to tokens."""
+    rng = random.Random(seed)
+    mask, prompt = [], []
+    for b in range(batch):
+        m, p, number = [], [], 1
+        for n in docs[b % len(docs)]:
+            if n < 0:
+                m += [0] * -n
+                p += [rng.randint(0, 1) for _ in range(-n)]
+            else:
+                lead = rng.randint(0, n)
+                m += [number] * n
+                p += [1] * lead + [0 if rng.random() < 0.8 else 1 for _ in range(n - lead)]
+                number += rng.randint(1, 3)
+        m, p = (m + [0] * tokens)[:tokens], (p + [0] * tokens)[:tokens]
+        mask.append(m)
+        prompt.append(p)
+    return mask, prompt if prompts else None
+
+
+@pytest.mark.parametrize("batch,tokens,docs", [
+    (1, 1, [[1]]), (1, 1, [[-1]]), (3, 2, [[1, 1], [2], [-1, 1]]), (2, 31, [[31], [5, -3, 7]]), (5, 33, [[33], [1] * 33]),
+    (2, 255, [[100, 100], [-255]]), (3, 1024, [[300, 1, 500], [1024], [10, -100, 900]]), (1, 9001, [[4000, 2, 5000]]), (7, 8193, [[8000], [1, -8000, 192]]),
+])
+def test_plan(batch, tokens, docs):
+    o = ops()
+    mask, prompt = rows(batch, tokens, docs, tokens)
+    ids = [[random.Random(b).randint(0, 250879) for _ in range(tokens)] for b in range(batch)]
+    cu = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for p in (prompt, None):
+        want = ref.plan(mask, p, ids)
+        spans, target, count = o.doc_plan(cu(mask), None if p is None else cu(p), cu(ids))
+        assert spans.tolist() == [[list(s) for s in r] for r in want[0]]
+        assert target.tolist() == want[1] and count.tolist() == [want[2]]
+        assert torch.equal(o.doc_plan(cu(mask), None if p is None else cu(p)), spans)
+    # a 0/1 mask without prompts is the padded sequence of the other calls
+    one = [[1] * (tokens - b) + [0] * b for b in range(batch)] if tokens > batch else [[1] * tokens] * batch
+    t1, c1 = o.loss_targets(cu(ids), cu(one))
+    _, t2, c2 = o.doc_plan(cu(one), None, cu(ids))
+    assert torch.equal(t1, t2) and torch.equal(c1, c2)
+
+
+def inputs(batch, tokens, heads, kv, d, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    qkv = torch.randn(batch, tokens, heads + 2 * kv, d, generator=g).half()
+    qkv[:, :, :heads] *= scale
+    do = torch.randn(batch, tokens, heads, d, generator=g).half()
+    return qkv, do
+
+
+def split(qkv, heads, kv):
+    return qkv[:, :, :heads], qkv[:, :, heads:heads + kv], qkv[:, :, heads + kv:]
+
+
+CASES = [
+    # batch, tokens, heads, kv heads, head_dim, documents, prompts, slopes, cap, scale of q
+    (1, 1, 1, 1, 64, [[1]], False, False, 0.0, 1),
+    (3, 1, 2, 1, 128, [[1], [-1], [1]], True, True, 5.0, 1),
+    (1, 2, 1, 1, 128, [[1, 1]], False, True, 0.0, 1),
+    (2, 127, 2, 2, 64, [[127], [60, 67]], False, False, 0.0, 1),
+    (2, 128, 2, 1, 128, [[128], [1, 126, 1]], True, False, 0.0, 1),
+    (2, 129, 2, 2, 64, [[129], [128, 1]], True, True, 0.0, 1),
+    (2, 256, 4, 2, 128, [[256], [64, 64, 64, 64]], False, True, 30.0, 4),
+    (1, 257, 3, 1, 64, [[257]], True, False, 10.0, 4),
+    (3, 300, 4, 4, 128, [[300], [100, -50, 150], [-300]], True, True, 0.0, 1),
+    (2, 385, 4, 1, 64, [[-200, 185], [7] * 55], True, True, 20.0, 3),
+    (1, 700, 2, 2, 128, [[650, -20, 30]], False, True, 0.0, 1),
+    (1, 1100, 2, 1, 128, [[500, 1, 599]], True, False, 0.0, 1),
+    (2, 1030, 2, 2, 64, [[1030], [3, 1000]], True, True, 0.0, 3),
+]
+
+
+@pytest.mark.parametrize("batch,tokens,heads,kv,d,docs,prompts,bias,cap,scale", CASES)
+def test_forward_and_backward(batch, tokens, heads, kv, d, docs, prompts, bias, cap, scale):
+    o = ops()
+    mask, prompt = rows(batch, tokens, docs, tokens + d, prompts)
+    spans = torch.tensor(ref.plan(mask, prompt)[0], dtype=torch.int32)
+    slopes = torch.tensor([2.0 ** -(1 + i) for i in range(heads)]) if bias else None
+    qkv, do = inputs(batch, tokens, heads, kv, d, tokens * 7 + d, scale)
+    want = ref.attention(*split(qkv, heads, kv), spans, slopes, cap, do)
+    cq = qkv.cuda()
+    args = dict(slopes=None if slopes is None else slopes.cuda(), cap=cap)
+    out = torch.full((batch, tokens, heads, d), 7.0, dtype=torch.float16, device="cuda")
+    out, lse = o.doc_attn(*split(cq, heads, kv), spans.cuda(), out=out, **args)
+    assert status() == 0
+    ref.assert_close(out, *want["out"], "out")
+    ref.assert_close(lse, *want["lse"], "lse")
+    grads = torch.full((batch, tokens, heads + 2 * kv, d), 7.0, dtype=torch.float16, device="cuda")
+    dq, dk, dv = split(grads, heads, kv)
+    o.doc_attn_backward(do.cuda(), *split(cq, heads, kv), out, lse, spans.cuda(), dq=dq, dk=dk, dv=dv, **args)
+    assert status() == 0
+    for name, got in (("dv", dv), ("dk", dk), ("dq", dq)):
+        ref.assert_close(got, *want[name], name)
+    # the same again: no result depends on the order in which blocks happen to run
+    again = o.doc_attn_backward(do.cuda(), *split(cq, heads, kv), out, lse, spans.cuda(), **args)
+    for a, b in zip(again, (dq, dk, dv)):
+        assert torch.equal(a, b)
+    # a tensor of its own for each of q, k, v
+    q2, k2, v2 = (x.contiguous() for x in split(cq, heads, kv))
+    out2, lse2 = o.doc_attn(q2, k2, v2, spans.cuda(), **args)
+    assert torch.equal(out2, out) and torch.equal(lse2, lse)
+
+
+def test_gradients_against_differences():
+    """(f(x + h) - f(x - h)) / 2h in 64 bits of the loss sum(out * d_out), at a few elements of q, k and v, against the kernel."""
+    o = ops()
+    batch, tokens, heads, kv, d, cap = 1, 40, 2, 1, 64, 3.0
+    mask, prompt = rows(batch, tokens, [[25, -2, 13]], 3)
+    spans = torch.tensor(ref.plan(mask, prompt)[0], dtype=torch.int32)
+    slopes = torch.tensor([0.5, 0.1])
+    qkv, do = inputs(batch, tokens, heads, kv, d, 5, 2.0)
+    cq = qkv.cuda()
+    out, lse = o.doc_attn(*split(cq, heads, kv), spans.cuda(), slopes=slopes.cuda(), cap=cap)
+    got = o.doc_attn_backward(do.cuda(), *split(cq, heads, kv), out, lse, spans.cuda(), slopes=slopes.cuda(), cap=cap)
+    bounds = ref.attention(*split(qkv, heads, kv), spans, slopes, cap, do)
+
+    def loss(x):
+        return (ref.attention(*split(x, heads, kv), spans, slopes, cap)["out"][0] * do.double()).sum().item()
+
+    h = 1e-5
+    x = qkv.double()
+    for which, (t, i, e) in enumerate([(5, 0, 3), (20, 1, 63), (30, 0, 10)] * 3):
+        part = which // 3
+        col = (i if part == 0 else heads if part == 1 else heads + kv)
+        hi, lo = x.clone(), x.clone()
+        hi[0, t, col, e] += h
+        lo[0, t, col, e] -= h
+        slope = (loss(hi) - loss(lo)) / (2 * h)
+        name = ("dq", "dk", "dv")[part]
+        at = (0, t, i if part == 0 else 0, e)
+        assert abs(got[part][at].item() - slope) <= bounds[name][1][at].item() + 1e-6 * (1 + abs(slope)), name
+
+
+def test_what_is_masked_does_not_reach_a_query():
+    """NaN and infinity in padding, in another document and in later tokens: rows that do not see them keep every bit."""
+    o = ops()
+    batch, tokens, heads, kv, d = 2, 400, 4, 2, 128
+    mask, prompt = rows(batch, tokens, [[150, 130, -40, 60], [390]], 11)
+    spans = torch.tensor(ref.plan(mask, None)[0], dtype=torch.int32).cuda()
+    slopes = torch.tensor([0.5, 0.25, 0.125, 0.0625]).cuda()
+    qkv, do = inputs(batch, tokens, heads, kv, d, 9)
+    clean, do = qkv.cuda(), do.cuda()
+    bad = clean.clone()
+    bad_do = do.clone()
+    value = [float("nan"), float("inf"), float("-inf"), 65504.0]
+    poisoned = {0: [200, 290, 300, 385], 1: [250, 395]}        # a later document's token, padding, padding behind, the last tokens
+    for b, places in poisoned.items():
+        for n, t in enumerate(places):
+            bad[b, t] = value[n % 3]
+            bad_do[b, t] = value[(n + 1) % 3]
+    for cap in (0.0, 20.0):
+        args = dict(slopes=slopes, cap=cap)
+        out, lse = o.doc_attn(*split(clean, heads, kv), spans, **args)
+        out2, lse2 = o.doc_attn(*split(bad, heads, kv), spans, **args)
+        grads = o.doc_attn_backward(do, *split(clean, heads, kv), out, lse, spans, **args)
+        grads2 = o.doc_attn_backward(bad_do, *split(bad, heads, kv), out2, lse2, spans, **args)
+        assert status() == 0
+        vis = ref.visible(spans.cpu())
+        hit = torch.zeros(batch, tokens, dtype=torch.bool)
+        for b, places in poisoned.items():
+            hit[b, places] = True
+        q_hit = (vis & hit[:, None]).any(2) | hit                       # queries that see a poisoned token
+        k_hit = (vis & q_hit[:, :, None]).any(1) | hit                  # keys seen by such a query (its gradient is not finite)
+        ok_q, ok_k = ~q_hit.cuda(), ~k_hit.cuda()
+        assert ok_q.sum() > 300 and ok_k.sum() > 100
+        near = dict(rtol=2.0 ** -8, atol=2.0 ** -8)                     # a row evaluated again skips the fp16 operand rounding
+        torch.testing.assert_close(out2[ok_q], out[ok_q], **near)
+        torch.testing.assert_close(lse2.transpose(1, 2)[ok_q], lse.transpose(1, 2)[ok_q], rtol=1e-6, atol=1e-6)
+        torch.testing.assert_close(grads2[0][ok_q], grads[0][ok_q], rtol=2.0 ** -6, atol=2.0 ** -6)
+        for a, b in zip(grads2[1:], grads[1:]):
+            torch.testing.assert_close(a[ok_k], b[ok_k], rtol=2.0 ** -6, atol=2.0 ** -5)
+        padding = (spans[..., 0] == spans[..., 1]).cuda()
+        for x in (out2,) + grads2:
+            assert (x[padding] == 0).all()
+        assert (lse2.transpose(1, 2)[padding] == 0).all()
+        assert torch.isnan(out2[1, 250:390]).any(-1).all()              # and who sees it, gets it
+    # values at the end of fp16's range are ordinary
+    big = clean.clone()
+    big[:, :, heads + kv:] = 60000.0
+    out3, _ = o.doc_attn(*split(big, heads, kv), spans, slopes=slopes)
+    seen = (spans[..., 1] > spans[..., 0])
+    assert (out3[seen] == 60000.0).all() or ((out3[seen].float() - 60000).abs() <= 64).all()
+
+
+def test_many_tiles_and_heads():
+    """More tiles than a CTA sorts, and an item list far longer than the grid, against the same rows one at a time."""
+    o = ops()
+    batch, tokens, heads, kv, d = 600, 140, 2, 1, 64
+    mask, prompt = rows(batch, tokens, [[140], [50, 90], [-20, 100]], 5)
+    cu = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    spans = o.doc_plan(cu(mask), cu(prompt))
+    qkv, do = inputs(batch, tokens, heads, kv, d, 2)
+    qkv, do = qkv.cuda(), do.cuda()
+    out, lse = o.doc_attn(*split(qkv, heads, kv), spans)
+    grads = o.doc_attn_backward(do, *split(qkv, heads, kv), out, lse, spans)
+    assert status() == 0
+    for b in (0, 1, 2, 299, 598, 599):
+        one = qkv[b:b + 1].contiguous()
+        o1, l1 = o.doc_attn(*split(one, heads, kv), spans[b:b + 1].contiguous())
+        g1 = o.doc_attn_backward(do[b:b + 1].contiguous(), *split(one, heads, kv), o1, l1, spans[b:b + 1].contiguous())
+        assert torch.equal(o1[0], out[b]) and torch.equal(l1[0], lse[b])
+        assert all(torch.equal(x[0], y[b]) for x, y in zip(g1, grads))
+
+
+def test_captured_replayed_and_on_another_stream():
+    o = ops()
+    batch, tokens, heads, kv, d = 2, 300, 4, 2, 64
+    mask, prompt = rows(batch, tokens, [[200, 90], [300]], 1)
+    cu = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    m, p = cu(mask), cu(prompt)
+    qkv, do = (x.cuda() for x in inputs(batch, tokens, heads, kv, d, 1))
+
+    def step():
+        spans = o.doc_plan(m, p)
+        out, lse = o.doc_attn(*split(qkv, heads, kv), spans, cap=10.0)
+        return (out, lse) + o.doc_attn_backward(do, *split(qkv, heads, kv), out, lse, spans, cap=10.0)
+
+    want = [x.clone() for x in step()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for x in got:
+        x.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # new inputs in the same buffers, another mask among them
+    other = inputs(batch, tokens, heads, kv, d, 8)
+    qkv.copy_(other[0])
+    do.copy_(other[1])
+    m.copy_(cu(rows(batch, tokens, [[50, 250], [-30, 200]], 2)[0]))
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [x.clone() for x in got]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = step()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    assert status() == 0
+
+
+def test_large_sizes_against_the_existing_attention():
+    """2048 tokens, 32 heads of 128, one document per row: the causal attention with the bias of the padded path."""
+    o = ops()
+    from blackriver_b200 import brk
+    B, T, H, D = 1, 2048, 32, 128
+    g = torch.Generator(device="cuda").manual_seed(0)
+    qkv = torch.randn(B, T, 3 * H, D, generator=g, device="cuda").half()
+    do = torch.randn(B, T, H, D, generator=g, device="cuda").half()
+    slopes = torch.tensor([2.0 ** (-8 * (i + 1) / H) for i in range(H)], device="cuda")
+    spans = o.doc_plan(torch.ones(B, T, dtype=torch.int32, device="cuda"))
+    out, lse = o.doc_attn(*split(qkv, H, H), spans, slopes=slopes)
+    grads = o.doc_attn_backward(do, *split(qkv, H, H), out, lse, spans, slopes=slopes)
+    out2 = torch.empty_like(out)
+    lse2 = torch.empty_like(lse)
+    g2 = torch.empty_like(qkv)
+    ws = torch.empty(brk.lib().brk_flash_attn_bwd_workspace_bytes(B, T, H), dtype=torch.uint8, device="cuda")
+    at, ga, n = qkv.data_ptr(), g2.data_ptr(), 2 * H * D
+    brk.call("brk_flash_attn_fwd", at, at + n, at + 2 * n, 3 * H * D, out2.data_ptr(), H * D, lse2.data_ptr(), 0, slopes.data_ptr(), B, T, H, D, o.stream())
+    brk.call("brk_flash_attn_bwd", at, at + n, at + 2 * n, 3 * H * D, out2.data_ptr(), do.data_ptr(), H * D, lse2.data_ptr(), ga, ga + n, ga + 2 * n, 3 * H * D, 0,
+             slopes.data_ptr(), B, T, H, D, ws.data_ptr(), ws.numel(), o.stream())
+    assert status() == 0 and brk.lib().brk_flash_attn_status() == 0
+    # two fp16 evaluations of the same sums: 2 * 2^-11 of the sum of magnitudes each, which norms of whole tensors bound
+    for a, b in zip((out,) + grads, (out2,) + split(g2, H, H)):
+        assert (a.double() - b.double()).norm() <= 4 * 2.0 ** -11 * b.double().norm()
+    at = torch.arange(T, device="cuda")
+    assert (lse - (lse2 - slopes[None, :, None] * at)).abs().max() < 2e-3       # the padded path's bias is slope * key: up to 1450 in fp32, twice
+
+
+@pytest.mark.parametrize("batch,tokens", [(0, 5), (2, 0)])
+def test_no_tokens(batch, tokens):
+    o = ops()
+    m = torch.empty(batch, tokens, dtype=torch.int32, device="cuda")
+    spans, target, count = o.doc_plan(m, m, m)
+    assert count.item() == 0 and spans.shape == (batch, tokens, 4) and target.shape == m.shape
+    x = torch.empty(batch, tokens, 4, 64, dtype=torch.float16, device="cuda")
+    out, lse = o.doc_attn(x, x[:, :, :2], x[:, :, 2:], spans)
+    grads = o.doc_attn_backward(x, x, x[:, :, :2], x[:, :, 2:], out, lse, spans)
+    assert out.shape == x.shape and grads[1].shape == (batch, tokens, 2, 64)
+
+
+def test_front_end_refuses_layouts_it_would_misread():
+    o = ops()
+    x = torch.zeros(2, 8, 4, 64, dtype=torch.float16, device="cuda")
+    spans = o.doc_plan(torch.ones(2, 8, dtype=torch.int32, device="cuda"))
+    for bad in (x.transpose(1, 2).contiguous().transpose(1, 2), x[:, ::2], x.float(), x[:, :, :, :32], torch.zeros(8, 2, 4, 64, dtype=torch.float16, device="cuda").transpose(0, 1)):
+        with pytest.raises((ValueError, TypeError)):
+            o.doc_attn(bad, x, x, spans)
+    with pytest.raises(ValueError):
+        o.doc_attn(x, x, x, spans[:1].contiguous())
+    with pytest.raises(ValueError):
+        o.doc_attn(x, x, x, spans, slopes=torch.zeros(3, device="cuda"))
+    with pytest.raises(ValueError):
+        o.doc_plan(torch.ones(2, 8, dtype=torch.int64, device="cuda"))
+    from blackriver_b200 import brk
+    with pytest.raises(brk.BrkError):
+        o.doc_attn(x[:, :, :3], x[:, :, :2], x[:, :, 2:], spans)
