@@ -49,9 +49,11 @@ __device__ __forceinline__ A8Scale a8_scale(uint32_t top_bits) {
 // Four values to four bytes.  Adding 1.5 * 2^23 leaves the nearest integer (ties to even) in the low mantissa bits, and
 // a byte permute gathers them: no conversion instruction, which would run at an eighth of the rate.  With inv == 0 the
 // product is 0, or NaN for a value that is not finite; its low byte is whatever it is, the block's scale is NaN then.
+// The product is rounded before the sum, not fused with it: a value in the middle between two steps (half of the block's
+// largest, say) then stays there, and ties go to even as they do in exact arithmetic.
+__device__ __forceinline__ uint32_t a8_round(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f)); }
 __device__ __forceinline__ uint32_t a8_pack4(float a, float b, float c, float d, float inv) {
-    const uint32_t ia = __float_as_uint(fmaf(a, inv, 12582912.0f)), ib = __float_as_uint(fmaf(b, inv, 12582912.0f));
-    const uint32_t ic = __float_as_uint(fmaf(c, inv, 12582912.0f)), id = __float_as_uint(fmaf(d, inv, 12582912.0f));
+    const uint32_t ia = a8_round(a, inv), ib = a8_round(b, inv), ic = a8_round(c, inv), id = a8_round(d, inv);
     return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
 }
 // Byte b of a word as the number it stands for: 2^23 + (b + 128) assembled from its bits, exactly.

@@ -11,11 +11,12 @@
 //
 // What is masked may hold anything.  A masked score or gradient is replaced, never multiplied.  A masked value row still
 // meets a probability of zero inside the tensor core, and 0 * NaN is NaN; the epilogues notice an accumulator that is not
-// finite and evaluate that row again in fp32 over its visible pairs alone, so a NaN or an infinity reaches exactly the
-// rows that see it and costs nothing where there is none.
+// finite, and a row that sees nothing of the kind itself is evaluated again in fp32 over its visible pairs alone.  So a NaN
+// or an infinity reaches exactly the rows that see it, and costs nothing where there is none.
 //
 // Every mbarrier wait is bounded (see brk_ptx.cuh); a give-up raises g_doc_error.
 #include <atomic>
+#include <type_traits>
 
 #include "brk_attn.cuh"
 #include "brk_common.cuh"
@@ -29,7 +30,10 @@ __device__ int g_doc_error = 0;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr int DA_THREADS = 64 + 256;        // producer warp, MMA warp, eight row-owner warps
+// Three warpgroups: a producer warp and an MMA warp in the first (its other two warps only make it whole), eight row-owner
+// warps in the other two, which take most of the first one's registers: 128 * (56 + 2 * 224) of the launch's 384 * 168.
+constexpr int DA_THREADS = 384;
+constexpr int DA_REGS_FEW = 56, DA_REGS_MANY = 224;
 constexpr int DA_SORT = 512;                // tiles whose order a CTA sorts; more are taken as they come
 
 struct DocAttn {
@@ -39,7 +43,7 @@ struct DocAttn {
     int64_t ld_q, ld_kv, ld_out;
     int batch, tokens, heads, kv_heads;
     float scale, scale_log2;                // 1/sqrt(d), times log2(e)
-    float cap_log2, cap_in;                 // cap log2(e); 2 log2(e) / (sqrt(d) cap), so that exp2(cap_in q.k) = e^(2x/cap)
+    float cap_log2, cap_in;                 // cap log2(e); 1 / (sqrt(d) cap)
     // forward
     __half* out;
     float* lse;                             // [batch, heads, tokens], natural log
@@ -53,14 +57,29 @@ struct DocAttn {
 
 // ---- scores --------------------------------------------------------------------------------------------------------------
 
-// Score of a raw product in log2 units without the bias, and with a cap the tanh's derivative.  tanh(u) = 1 - 2r with
-// r = 1 / (1 + e^2u): absolute error about 1e-7 over the whole range, which at a cap of 50 is 1e-5 of the exponent (the
-// hardware tanh's 2^-11 would be 0.02 of it).
-template <bool CAP>
-__device__ __forceinline__ float da_score(float raw, const DocAttn& p) {
-    if (!CAP) return raw * p.scale_log2;
-    const float r = __fdividef(1.0f, 1.0f + fast_exp2(raw * p.cap_in));
-    return fmaf(-2.0f * p.cap_log2, r, p.cap_log2);
+// The cap.  tanh(u) for |u| <= 0.75 is an odd polynomial (least maximum error over the interval, 3e-7 in fp32) on the
+// FMA units, two scores at a time.  Wider arguments take 1 - 2 / (1 + e^2u), two operations on the special function unit,
+// of which the softmax already needs one per score: at 16 a clock and SM that unit, not the tensor core, would set the
+// pace.  Both are within 1e-6 of tanh, 5e-5 of the exponent at a cap of 50; the hardware tanh's 2^-11 would be 0.02 of it.
+constexpr float TANH_REACH = 0.75f;
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 da_tanh_near(float2 u) {
+    const float2 s = __fmul2_rn(u, u);
+    float2 t = __ffma2_rn(both(0.01231877f), s, both(-0.04928038f));
+    t = __ffma2_rn(t, s, both(0.13226089f));
+    t = __ffma2_rn(t, s, both(-0.33323076f));
+    t = __ffma2_rn(t, s, both(0.99999723f));
+    return __fmul2_rn(t, u);
+}
+__device__ __forceinline__ float da_tanh(float u) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + fast_exp2(2.0f * LOG2E * u)));
+    return fmaf(-2.0f, r, 1.0f);
+}
+// tanh of raw * scale / cap; `near`: all of the warp's arguments are within reach of the polynomial
+__device__ __forceinline__ float2 da_capped(float2 raw, const DocAttn& p, bool near) {
+    const float2 u = __fmul2_rn(raw, both(p.cap_in));
+    return near ? da_tanh_near(u) : make_float2(da_tanh(u.x), da_tanh(u.y));
 }
 template <bool CAP>
 __device__ __forceinline__ float da_score(float raw, const DocAttn& p, float& slope_of_tanh) {
@@ -68,16 +87,31 @@ __device__ __forceinline__ float da_score(float raw, const DocAttn& p, float& sl
         slope_of_tanh = 1.0f;
         return raw * p.scale_log2;
     }
-    const float r = __fdividef(1.0f, 1.0f + fast_exp2(raw * p.cap_in));
-    slope_of_tanh = 4.0f * r * (1.0f - r);
-    return fmaf(-2.0f * p.cap_log2, r, p.cap_log2);
+    const float t = da_tanh(raw * p.cap_in);
+    slope_of_tanh = fmaf(-t, t, 1.0f);
+    return t * p.cap_log2;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
+// bits [from, to) of 32, whatever lies outside of them
+__device__ __forceinline__ uint32_t span_bits(int from, int to) {
+    from = min(max(from, 0), 32);
+    to = min(max(to, from), 32);
+    return (uint32_t)((1ull << to) - (1ull << from));
+}
+template <bool B>
+using Flag = std::integral_constant<bool, B>;
+// key (or query) numbers 2i and 2i + 1 of a chunk
+__device__ __forceinline__ float2 pair_of(int i) { return make_float2((float)(2 * i), (float)(2 * i + 1)); }
 
 // ---- tiles ---------------------------------------------------------------------------------------------------------------
 
 struct Range {
     int begin, end;
 };
+// a value that is the same in the whole warp, known to be
+template <typename T>
+__device__ __forceinline__ T uniform(T x) { return __shfl_sync(0xffffffffu, x, 0); }
 // keys (KEYS) that 128 queries from t0 on see, or queries that see 128 keys, as a range of `unit`-sized blocks
 template <bool KEYS>
 __device__ __forceinline__ Range da_blocks(const DocAttn& p, int b, int t0, int unit) {
@@ -123,7 +157,22 @@ __device__ __forceinline__ void da_sort(DaTable* table, int n_tiles, W weight) {
 }
 
 // ---- rows evaluated again without the tensor core (see the top) ------------------------------------------------------------
+// Called by whole warps with one row per lane, `bad` where the row's accumulator is not finite.  A row that sees an operand
+// that is not finite keeps what it has (32 partners are looked at at a time, one per lane, until every bad row has found
+// one); the others are evaluated one after another by the warp: a lane forms the pair terms of one partner in 32, then the
+// lanes share the sum over them, D / 32 columns each.
 
+template <int D>
+__device__ __forceinline__ bool da_not_finite(const __half* row) {
+    bool found = false;
+    for (int c = 0; c < D; c += 8) {
+        const uint4 w = *reinterpret_cast<const uint4*>(row + c);
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) found |= (x[e] & 0x7c00u) == 0x7c00u || (x[e] & 0x7c000000u) == 0x7c000000u;
+    }
+    return found;
+}
 template <int D>
 __device__ __forceinline__ float da_dot(const __half* a, const __half* b) {
     float s = 0.0f;
@@ -136,80 +185,134 @@ __device__ __forceinline__ float da_dot(const __half* a, const __half* b) {
     }
     return s;
 }
-template <int D, bool CAP>
-__device__ float da_log2_score(const DocAttn& p, int b, int h, int i, int j, float& dt) {
-    const int kh = h / (p.heads / p.kv_heads);
-    const __half* q = p.q + ((int64_t)b * p.tokens + i) * p.ld_q + h * D;
-    const __half* k = p.k + ((int64_t)b * p.tokens + j) * p.ld_kv + kh * D;
-    float s = da_score<CAP>(da_dot<D>(q, k), p, dt);
-    if (p.slopes) s -= p.slopes[h] * LOG2E * fabsf((float)(i - j));
-    return s;
+// which of the bad rows see no partner for which found(partner) holds
+template <typename F>
+__device__ __forceinline__ uint32_t da_to_mend(bool bad, int lo, int hi, F found) {
+    const int lane = threadIdx.x & 31;
+    const int from = __reduce_min_sync(0xffffffffu, bad ? lo : 0x7fffffff), to = __reduce_max_sync(0xffffffffu, bad ? hi : 0);
+    uint32_t left = __ballot_sync(0xffffffffu, bad);
+    for (int k0 = from; k0 < to && left; k0 += 32) {
+        const uint32_t hits = __ballot_sync(0xffffffffu, k0 + lane < to && found(k0 + lane));
+        if (hits & span_bits(lo - k0, hi - k0)) bad = false;
+        left = __ballot_sync(0xffffffffu, bad);
+    }
+    return left;
 }
-template <int D, bool CAP>
-__device__ __noinline__ void da_out_row(const DocAttn& p, int b, int h, int i, int lo, int hi, float lse2) {
-    const int kh = h / (p.heads / p.kv_heads);
-    __half* o = p.out + ((int64_t)b * p.tokens + i) * p.ld_out + h * D;
-    for (int c = 0; c < D; c += 32) {
-        float acc[32] = {};
-        for (int j = lo; j < hi; j++) {
-            float dt;
-            const float w = fast_exp2(da_log2_score<D, CAP>(p, b, h, i, j, dt) - lse2);
-            const __half* v = p.v + ((int64_t)b * p.tokens + j) * p.ld_kv + kh * D + c;
+// acc[e] += w * row[lane * D / 32 + e] for each partner of a block of 32, whose weight is in the lane of its number
+template <int D>
+__device__ __forceinline__ void da_add_rows(float (&acc)[D / 32], float w, const __half* rows, int64_t ld, int n) {
+    const int lane = threadIdx.x & 31;
+    for (int i = 0; i < n; i++) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        const __half2* x = reinterpret_cast<const __half2*>(rows + i * ld + lane * (D / 32));
 #pragma unroll
-            for (int e = 0; e < 32; e++) acc[e] = fmaf(w, __half2float(v[e]), acc[e]);
+        for (int e = 0; e < D / 64; e++) {
+            const float2 f = __half22float2(x[e]);
+            acc[2 * e] = fmaf(wi, f.x, acc[2 * e]);
+            acc[2 * e + 1] = fmaf(wi, f.y, acc[2 * e + 1]);
         }
-        for (int e = 0; e < 32; e++) o[c + e] = __float2half_rn(acc[e]);
     }
 }
-// P and dS of one visible pair
-template <int D, bool CAP>
-__device__ float da_pair(const DocAttn& p, int b, int h, int i, int j, float& ds) {
-    const int kh = h / (p.heads / p.kv_heads);
-    const int64_t at = ((int64_t)b * p.heads + h) * p.tokens + i;
-    float dt;
-    const float w = fast_exp2(da_log2_score<D, CAP>(p, b, h, i, j, dt) - p.lse_in[at] * LOG2E);
-    const float dp = da_dot<D>(p.d_out + ((int64_t)b * p.tokens + i) * p.ld_out + h * D, p.v + ((int64_t)b * p.tokens + j) * p.ld_kv + kh * D);
-    ds = w * (dp - p.delta[at]) * dt;
-    return w;
-}
-template <int D, bool CAP>
-__device__ __noinline__ void da_dq_row(const DocAttn& p, int b, int h, int i, int lo, int hi) {
-    const int kh = h / (p.heads / p.kv_heads);
-    __half* o = p.dq + ((int64_t)b * p.tokens + i) * p.ld_dq + h * D;
-    for (int c = 0; c < D; c += 32) {
-        float acc[32] = {};
-        for (int j = lo; j < hi; j++) {
-            float ds;
-            da_pair<D, CAP>(p, b, h, i, j, ds);
-            const __half* k = p.k + ((int64_t)b * p.tokens + j) * p.ld_kv + kh * D + c;
+template <int D>
+__device__ __forceinline__ void da_store_row(__half* row, const float (&acc)[D / 32], float scale) {
+    __half2* o = reinterpret_cast<__half2*>(row + (threadIdx.x & 31) * (D / 32));
 #pragma unroll
-            for (int e = 0; e < 32; e++) acc[e] = fmaf(ds, __half2float(k[e]), acc[e]);
+    for (int e = 0; e < D / 64; e++) o[e] = __floats2half2_rn(acc[2 * e] * scale, acc[2 * e + 1] * scale);
+}
+// the tensors of one row of the batch and one head
+template <int D>
+struct DaHead {
+    const __half *q, *k, *v, *g;
+    const float *lse, *delta;
+    float slope2;
+    __device__ DaHead(const DocAttn& p, int b, int h) {
+        const int64_t row = (int64_t)b * p.tokens, at = ((int64_t)b * p.heads + h) * p.tokens;
+        const int kh = h / (p.heads / p.kv_heads);
+        q = p.q + row * p.ld_q + h * D;
+        k = p.k + row * p.ld_kv + kh * D;
+        v = p.v + row * p.ld_kv + kh * D;
+        g = p.d_out ? p.d_out + row * p.ld_out + h * D : nullptr;
+        lse = p.lse_in ? p.lse_in + at : nullptr;
+        delta = p.delta ? p.delta + at : nullptr;
+        slope2 = p.slopes ? p.slopes[h] * LOG2E : 0.0f;
+    }
+    // score in log2 units of a visible pair
+    template <bool CAP>
+    __device__ float score(const DocAttn& p, int i, int j, float& dt) const {
+        return da_score<CAP>(da_dot<D>(q + i * p.ld_q, k + j * p.ld_kv), p, dt) - slope2 * fabsf((float)(i - j));
+    }
+    // P and dS of a visible pair
+    template <bool CAP>
+    __device__ float pair(const DocAttn& p, int i, int j, float& ds) const {
+        float dt;
+        const float w = fast_exp2(score<CAP>(p, i, j, dt) - lse[i] * LOG2E);
+        ds = w * (da_dot<D>(g + i * p.ld_out, v + j * p.ld_kv) - delta[i]) * dt;
+        return w;
+    }
+};
+template <int D, bool CAP>
+__device__ __noinline__ void da_mend_out(const DocAttn& p, int b, int h, int i, int lo, int hi, float lse2, bool bad) {
+    const DaHead<D> t(p, b, h);
+    const int lane = threadIdx.x & 31;
+    uint32_t left = da_to_mend(bad, lo, hi, [&](int j) { return da_not_finite<D>(t.v + j * p.ld_kv); });
+    for (; left; left &= left - 1) {
+        const int r = __ffs(left) - 1, ri = __shfl_sync(0xffffffffu, i, r), from = __shfl_sync(0xffffffffu, lo, r), to = __shfl_sync(0xffffffffu, hi, r);
+        const float rl = __shfl_sync(0xffffffffu, lse2, r);
+        float acc[D / 32] = {};
+        for (int j = from; j < to; j += 32) {
+            float dt, w = 0.0f;
+            if (j + lane < to) w = fast_exp2(t.template score<CAP>(p, ri, j + lane, dt) - rl);
+            da_add_rows<D>(acc, w, t.v + j * p.ld_kv, p.ld_kv, min(32, to - j));
         }
-        for (int e = 0; e < 32; e++) o[c + e] = __float2half_rn(acc[e] * p.scale);
+        da_store_row<D>(p.out + ((int64_t)b * p.tokens + ri) * p.ld_out + h * D, acc, 1.0f);
     }
 }
 template <int D, bool CAP>
-__device__ __noinline__ void da_dkv_row(const DocAttn& p, int b, int kh, int j, int qlo, int qhi) {
-    const int group = p.heads / p.kv_heads;
-    const int64_t at = ((int64_t)b * p.tokens + j) * p.ld_dkv + kh * D;
-    for (int c = 0; c < D; c += 32) {
-        float ak[32] = {}, av[32] = {};
-        for (int h = kh * group; h < (kh + 1) * group; h++)
-            for (int i = qlo; i < qhi; i++) {
-                float ds;
-                const float w = da_pair<D, CAP>(p, b, h, i, j, ds);
-                const __half* q = p.q + ((int64_t)b * p.tokens + i) * p.ld_q + h * D + c;
-                const __half* g = p.d_out + ((int64_t)b * p.tokens + i) * p.ld_out + h * D + c;
-#pragma unroll
-                for (int e = 0; e < 32; e++) {
-                    ak[e] = fmaf(ds, __half2float(q[e]), ak[e]);
-                    av[e] = fmaf(w, __half2float(g[e]), av[e]);
-                }
+__device__ __noinline__ void da_mend_dq(const DocAttn& p, int b, int h, int i, int lo, int hi, bool bad) {
+    const DaHead<D> t(p, b, h);
+    const int lane = threadIdx.x & 31;
+    if (bad && (!(fabsf(t.lse[i]) < INFINITY) || !(fabsf(t.delta[i]) < INFINITY) || da_not_finite<D>(t.q + i * p.ld_q) || da_not_finite<D>(t.g + i * p.ld_out))) bad = false;
+    uint32_t left = da_to_mend(bad, lo, hi, [&](int j) { return da_not_finite<D>(t.k + j * p.ld_kv) || da_not_finite<D>(t.v + j * p.ld_kv); });
+    for (; left; left &= left - 1) {
+        const int r = __ffs(left) - 1, ri = __shfl_sync(0xffffffffu, i, r), from = __shfl_sync(0xffffffffu, lo, r), to = __shfl_sync(0xffffffffu, hi, r);
+        float acc[D / 32] = {};
+        for (int j = from; j < to; j += 32) {
+            float ds = 0.0f;
+            if (j + lane < to) t.template pair<CAP>(p, ri, j + lane, ds);
+            da_add_rows<D>(acc, ds, t.k + j * p.ld_kv, p.ld_kv, min(32, to - j));
+        }
+        da_store_row<D>(p.dq + ((int64_t)b * p.tokens + ri) * p.ld_dq + h * D, acc, p.scale);
+    }
+}
+template <int D, bool CAP>
+__device__ __noinline__ void da_mend_dkv(const DocAttn& p, int b, int kh, int j, int lo, int hi, bool bad) {
+    const int group = p.heads / p.kv_heads, lane = threadIdx.x & 31;
+    {
+        const DaHead<D> t(p, b, kh * group);
+        if (bad && (da_not_finite<D>(t.k + j * p.ld_kv) || da_not_finite<D>(t.v + j * p.ld_kv))) bad = false;
+    }
+    for (int h = kh * group; h < (kh + 1) * group; h++) {
+        const DaHead<D> t(p, b, h);
+        const uint32_t left = da_to_mend(bad, lo, hi, [&](int i) {
+            return !(fabsf(t.lse[i]) < INFINITY) || !(fabsf(t.delta[i]) < INFINITY) || da_not_finite<D>(t.q + i * p.ld_q) || da_not_finite<D>(t.g + i * p.ld_out);
+        });
+        bad = left >> lane & 1;
+    }
+    for (uint32_t left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
+        const int r = __ffs(left) - 1, rj = __shfl_sync(0xffffffffu, j, r), from = __shfl_sync(0xffffffffu, lo, r), to = __shfl_sync(0xffffffffu, hi, r);
+        float ak[D / 32] = {}, av[D / 32] = {};
+        for (int h = kh * group; h < (kh + 1) * group; h++) {
+            const DaHead<D> t(p, b, h);
+            for (int i = from; i < to; i += 32) {
+                float ds = 0.0f, w = 0.0f;
+                if (i + lane < to) w = t.template pair<CAP>(p, i + lane, rj, ds);
+                da_add_rows<D>(ak, ds, t.q + i * p.ld_q, p.ld_q, min(32, to - i));
+                da_add_rows<D>(av, w, t.g + i * p.ld_out, p.ld_out, min(32, to - i));
             }
-        for (int e = 0; e < 32; e++) {
-            p.dk[at + c + e] = __float2half_rn(ak[e] * p.scale);
-            p.dv[at + c + e] = __float2half_rn(av[e]);
         }
+        const int64_t at = ((int64_t)b * p.tokens + rj) * p.ld_dkv + kh * D;
+        da_store_row<D>(p.dk + at, ak, p.scale);
+        da_store_row<D>(p.dv + at, av, 1.0f);
     }
 }
 
@@ -230,8 +333,9 @@ __device__ __forceinline__ uint32_t da_half2(float a, float b) {
 // tensor memory, over the scores they came from, as the A operand of P V: they never pass through shared memory, whose
 // bandwidth the two operands of Q K^T already need.  A tile's next scores may be issued right behind its P V without a
 // wait, since the tensor core works off its instructions in order.
-// The running maximum is lazy: probabilities are taken relative to a reference that moves (and the accumulator is
-// rescaled) only when the true maximum has run ahead of it by 2^8, so that P stays far inside fp16; fp16 and not fp32
+// Keys are walked from the last block to the first: with the distance bias the largest scores come first, and the running
+// maximum settles in the first block or two.  It is lazy besides: probabilities are taken relative to a reference that
+// moves (and the accumulator is rescaled) only when the true maximum has run ahead of it by 2^8, so that P stays far inside fp16; fp16 and not fp32
 // because it is the tensor core's operand type: 2^-11 of each probability, the same as V's own rounding.
 // ==========================================================================================================================
 template <int D>
@@ -270,7 +374,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     uint64_t* o_empty = bars + 18;           // 2: the tile's output has been read
     uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(bars + 20);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int per_row = (p.tokens + 255) / 256, n_pairs = p.batch * per_row;
     const bool sorted = n_pairs <= DA_SORT;
 
@@ -305,45 +409,47 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem_base = *tmem_base_smem;
+    const uint32_t tmem_base = uniform(*tmem_base_smem);
     const int group = p.heads / p.kv_heads;
 
     struct Item {
         int b, t0, head;
-        Range r[2];          // key blocks of the two tiles
-        int first, n;        // the blocks that either needs
+        Range r0, r1;        // key blocks of the two tiles
+        int last, n;         // the n blocks up to `last` that either needs, walked from the last one down
     };
     auto item_of = [&](int round, Item& m) {
         int pair;
         if (!da_item(round, n_pairs, p.heads, table, sorted, pair, m.head)) return false;
         m.b = pair / per_row;
         m.t0 = (pair % per_row) * 256;
-        m.r[0] = da_blocks<true>(p, m.b, m.t0, 128);
-        m.r[1] = da_blocks<true>(p, m.b, m.t0 + 128, 128);
-        const bool has0 = m.r[0].end > m.r[0].begin, has1 = m.r[1].end > m.r[1].begin;
-        m.first = has0 ? (has1 ? min(m.r[0].begin, m.r[1].begin) : m.r[0].begin) : m.r[1].begin;
-        m.n = max(m.r[0].end, m.r[1].end) - m.first;
+        m.r0 = da_blocks<true>(p, m.b, m.t0, 128);
+        m.r1 = da_blocks<true>(p, m.b, m.t0 + 128, 128);
+        const bool has0 = m.r0.end > m.r0.begin, has1 = m.r1.end > m.r1.begin;
+        m.last = max(m.r0.end, m.r1.end) - 1;
+        m.n = m.last + 1 - (has0 ? (has1 ? min(m.r0.begin, m.r1.begin) : m.r0.begin) : m.r1.begin);
         return true;
     };
 
+    if (warp < 4) give_registers<DA_REGS_FEW>();
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         if (lane == 0) {
             bool ok = true;
-            uint32_t it = 0, q_count[2] = {0, 0};
+            uint32_t it = 0, q_count0 = 0, q_count1 = 0;
             Item m;
             for (int round = 0; ok && item_of(round, m); round++) {
                 const int row = m.b * p.tokens, col = m.head * D, kcol = m.head / group * D;
-                for (int t = 0; t < 2 && ok; t++) {
-                    if (m.r[t].end == m.r[t].begin) continue;
-                    ok = mbar_wait(&q_empty[t], (q_count[t]++ & 1) ^ 1);        // the previous item's scores no longer read Q
-                    if (!ok) break;
+                auto load_q = [&](int t, const Range& r, uint32_t& count) {
+                    if (r.end == r.begin) return true;
+                    if (!mbar_wait(&q_empty[t], (count++ & 1) ^ 1)) return false;       // the previous item's scores no longer read Q
                     mbar_arrive_expect_tx(&q_full[t], S::TILE);
 #pragma unroll
                     for (int a = 0; a < D / 64; a++) tma_load_2d(sQ + t * S::TILE + a * 16384, &tmap_q, &q_full[t], col + a * 64, row + m.t0 + t * 128);
-                }
+                    return true;
+                };
+                ok = load_q(0, m.r0, q_count0) && load_q(1, m.r1, q_count1);
                 for (int n = 0; n < m.n && ok; n++, it++) {
-                    const int s = it % S::STAGES, y = row + (m.first + n) * 128;
+                    const int s = it % S::STAGES, y = row + (m.last - n) * 128;
                     const uint32_t par = ((it / S::STAGES) & 1) ^ 1;
                     ok = mbar_wait(&k_empty[s], par);
                     if (!ok) break;
@@ -360,60 +466,72 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             if (!ok) atomicExch(&g_doc_error, 1);
         }
     } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        if (lane == 0) {
+        // ---------------- MMA issuer: the warp walks and waits together, which keeps addresses and descriptors in uniform
+        // registers; one lane issues ----------------
+        {
+            const bool issuer = elect_one();
             bool ok = true;
-            uint32_t it = 0, q_count[2] = {0, 0}, p_count[2] = {0, 0};        // blocks, and per tile: items, blocks
+            uint32_t it = 0, q_count0 = 0, q_count1 = 0, p_count0 = 0, p_count1 = 0;        // blocks, and per tile: items, blocks
+            const uint64_t q_desc = make_smem_desc_sw128(smem_u32(sQ), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(sK), 16, 1024);
+            const uint64_t v_desc = make_smem_desc_sw128(smem_u32(sV), 16384, 1024);
             Item m;
             for (int round = 0; ok && item_of(round, m); round++) {
+                m.last = uniform(m.last), m.n = uniform(m.n);
+                m.r0.begin = uniform(m.r0.begin), m.r0.end = uniform(m.r0.end), m.r1.begin = uniform(m.r1.begin), m.r1.end = uniform(m.r1.end);
                 for (int n = -1; n < m.n && ok; n++) {
                     const int vs = (it + n) % S::STAGES, ks = (it + n + 1) % S::STAGES;        // n == -1 uses no V
                     const bool more = n + 1 < m.n;
+                    const int blk = m.last - n;
                     if (n >= 0) ok = mbar_wait(&v_full[vs], ((it + n) / S::STAGES) & 1);
                     if (ok && more) ok = mbar_wait(&k_full[ks], ((it + n + 1) / S::STAGES) & 1);
-                    for (int t = 0; t < 2 && ok; t++) {
-                        const int blk = m.first + n;
-                        if (n >= 0 && blk >= m.r[t].begin && blk < m.r[t].end) {
-                            ok = mbar_wait(&p_full[t], p_count[t] & 1);
-                            if (ok && blk == m.r[t].begin) ok = mbar_wait(&o_empty[t], (q_count[t] & 1));      // count is one ahead: this item's scores are out
-                            if (!ok) break;
+                    // P V of block n and then the scores of block n + 1; the index is a constant, so that nothing lands in local memory
+                    auto step = [&](auto tile, const Range& r, uint32_t& q_count, uint32_t& p_count) {
+                        constexpr int t = decltype(tile)::value;
+                        if (n >= 0 && blk >= r.begin && blk < r.end) {
+                            const bool first = blk == r.end - 1;
+                            if (!mbar_wait(&p_full[t], p_count & 1)) return false;
+                            if (first && !mbar_wait(&o_empty[t], q_count & 1)) return false;       // the count is one ahead: this item's scores are out
                             tcgen05_fence_after();
-                            const uint32_t v_addr = smem_u32(sV + vs * S::TILE);
+                            const uint64_t vd = v_desc + (uint32_t)(vs * (S::TILE >> 4));
+                            if (issuer) {
 #pragma unroll
-                            for (int kk = 0; kk < 8; kk++)        // A = P [128 q x 128 keys] in tensor memory, B = V [128 keys x D], d contiguous
-                                umma_f16_ts(tmem_base + 256 + t * D, tmem_base + t * 128 + kk * 8, make_smem_desc_sw128(v_addr + kk * 2048, 16384, 1024), IDESC_PV,
-                                            (blk != m.r[t].begin || kk != 0) ? 1u : 0u);
-                            umma_commit(&o_done[t]);
-                            p_count[t]++;
-                        }
-                        if (more && blk + 1 >= m.r[t].begin && blk + 1 < m.r[t].end) {
-                            if (blk + 1 == m.r[t].begin) {
-                                ok = mbar_wait(&q_full[t], q_count[t]++ & 1);
-                                if (!ok) break;
+                                for (int kk = 0; kk < 8; kk++)        // A = P [128 q x 128 keys] in tensor memory, B = V [128 keys x D], d contiguous
+                                    umma_f16_ts(tmem_base + 256 + t * D, tmem_base + t * 128 + kk * 8, vd + kk * 128, IDESC_PV, kk != 0 || !first ? 1u : 0u);
+                                umma_commit(&o_done[t]);
                             }
+                            p_count++;
+                        }
+                        if (more && blk - 1 >= r.begin && blk - 1 < r.end) {
+                            if (blk == r.end && !mbar_wait(&q_full[t], q_count++ & 1)) return false;
                             tcgen05_fence_after();
-                            const uint32_t q_addr = smem_u32(sQ + t * S::TILE), k_addr = smem_u32(sK + ks * S::TILE);
+                            const uint64_t qd = q_desc + t * (S::TILE >> 4), kd = k_desc + (uint32_t)(ks * (S::TILE >> 4));
+                            if (issuer) {
 #pragma unroll
-                            for (int kk = 0; kk < D / 16; kk++) {
-                                const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-                                umma_f16_ss(tmem_base + t * 128, make_smem_desc_sw128(q_addr + off, 16, 1024), make_smem_desc_sw128(k_addr + off, 16, 1024), IDESC_S,
-                                            kk != 0 ? 1u : 0u);
+                                for (int kk = 0; kk < D / 16; kk++) {
+                                    const int off = (kk >> 2) * 1024 + (kk & 3) * 2;
+                                    umma_f16_ss(tmem_base + t * 128, qd + off, kd + off, IDESC_S, kk != 0 ? 1u : 0u);
+                                }
+                                umma_commit(&s_full[t]);
+                                if (blk - 1 == r.begin) umma_commit(&q_empty[t]);
                             }
-                            umma_commit(&s_full[t]);
-                            if (blk + 2 == m.r[t].end) umma_commit(&q_empty[t]);
                         }
-                    }
+                        return true;
+                    };
+                    ok = ok && step(std::integral_constant<int, 0>(), m.r0, q_count0, p_count0) && step(std::integral_constant<int, 1>(), m.r1, q_count1, p_count1);
                     if (!ok) break;
-                    if (n >= 0) umma_commit(&v_empty[vs]);
-                    if (more) umma_commit(&k_empty[ks]);
+                    if (issuer) {
+                        if (n >= 0) umma_commit(&v_empty[vs]);
+                        if (more) umma_commit(&k_empty[ks]);
+                    }
                 }
                 it += m.n;
             }
-            if (!ok) atomicExch(&g_doc_error, 2);
+            if (!ok && issuer) atomicExch(&g_doc_error, 2);
         }
-    } else {
+    } else if (warp >= 4) {
         // ---------------- softmax / epilogue: one thread per query of the tile ----------------
-        const int t = (warp - 2) >> 2;                  // tile: warps 2-5 and 6-9
+        take_registers<DA_REGS_MANY>();
+        const int t = (warp - 4) >> 2;                  // tile: warps 4-7 and 8-11
         const int quarter = warp & 3;                   // a warp reaches tensor-memory lanes 32 * (warp % 4) ..
         const int r = quarter * 32 + lane;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
@@ -422,13 +540,14 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint32_t it = 0;
         Item m;
         for (int round = 0; item_of(round, m); round++) {
+            const Range blocks = t == 0 ? m.r0 : m.r1;
             const int qi = m.t0 + t * 128 + r;
             const bool live = qi < p.tokens;
             const int64_t row = (int64_t)m.b * p.tokens + qi;
             int4 span = make_int4(0, 0x7fffffff, 0, 0);             // rows behind the sequence never force the masked path
             if (live) span = p.spans[row];
             const int lo = max(span.x, 0), hi = live ? min(span.y, p.tokens) : span.y;
-            if (m.r[t].end == m.r[t].begin) {
+            if (blocks.end == blocks.begin) {
                 if (live) {
                     da_zero_row(p.out + row * p.ld_out + m.head * D, D);
                     if (p.lse) p.lse[((int64_t)m.b * p.heads + m.head) * p.tokens + qi] = 0.0f;
@@ -437,46 +556,88 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             }
             const float slope2 = BIAS ? p.slopes[m.head] * LOG2E : 0.0f;
             const bool ahead = BIAS && __any_sync(0xffffffffu, live && hi > qi + 1);      // some row sees keys behind itself: the prompt's
-            float m_ref = -INFINITY, l = 0.0f;
-            for (int blk = m.r[t].begin; blk < m.r[t].end; blk++, it++) {
+            float m_ref = -INFINITY;
+            float2 l = both(0.0f);
+            for (int blk = blocks.end - 1; blk >= blocks.begin; blk--, it++) {
                 if (ok) ok = mbar_wait(&s_full[t], it & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) continue;
                 tcgen05_fence_after();
+                // The scores are read twice, 32 columns at a time: once for the maximum, once for the exponentials.  Keeping all 128
+                // in registers instead made straight-line code of some 1400 instructions a block, which one warp per scheduler and
+                // tile could not run through in less than 5 clocks each.
                 const int kbase = blk * 128;
-                const bool full = __all_sync(0xffffffffu, lo <= kbase && hi >= kbase + 128);
-                const bool past = !ahead || __all_sync(0xffffffffu, kbase + 127 <= qi);
-                const float base = slope2 * (float)(kbase - qi), dist = (float)(kbase - qi);
-                float x[128];
-                float top = -INFINITY;
+                uint32_t part = 0, whole = 0;                         // which chunks some row of the warp sees, and all rows see throughout
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    uint32_t v[32];
-                    tmem_ld_32x32b_x32(tm_s + c * 32, v);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const int k = c * 32 + e;
-                        float s = da_score<CAP>(__uint_as_float(v[e]), p);
-                        if (BIAS) {
-                            if (past)
-                                s += fmaf(slope2, (float)k, base);
-                            else
-                                s = fmaf(-slope2, fabsf(dist + (float)k), s);
-                        }
-                        if (!full) s = (kbase + k >= lo && kbase + k < hi) ? s : -INFINITY;
-                        x[k] = s;
-                        top = fmaxf(top, s);
-                    }
+                    const int k0 = kbase + c * 32;
+                    if (lo < k0 + 32 && hi > k0) part |= 1u << c;
+                    if (lo <= k0 && hi >= k0 + 32 && (!BIAS || !ahead || k0 + 31 <= qi)) whole |= 1u << c;
                 }
+                part = __reduce_or_sync(0xffffffffu, part);
+                whole = __reduce_and_sync(0xffffffffu, whole);
+                const float slant = slope2 * (float)(kbase - qi), dist = (float)(kbase - qi);
+                // chunk c of the scores: in log2 units with a cap or a bias, else as they are; what is masked -inf
+                auto scores = [&](int c, float2(&x)[16], auto capped) {
+                    if (CAP && capped) {
+                        float wide = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) wide = max3(wide, fabsf(x[i].x), fabsf(x[i].y));
+                        if (__all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH)) {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) x[i] = __fmul2_rn(da_capped(x[i], p, true), both(p.cap_log2));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) x[i] = __fmul2_rn(da_capped(x[i], p, false), both(p.cap_log2));
+                        }
+                    }
+                    if (whole >> c & 1) {
+                        if (BIAS) {
+                            const float2 at = both(fmaf(slope2, (float)(c * 32), slant));
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const float2 bias = __ffma2_rn(both(slope2), pair_of(i), at);
+                                x[i] = CAP ? __fadd2_rn(x[i], bias) : __ffma2_rn(x[i], both(p.scale_log2), bias);
+                            }
+                        }
+                    } else {
+                        const float d0 = dist + (float)(c * 32);
+                        const uint32_t seen = span_bits(lo - kbase - c * 32, hi - kbase - c * 32);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            if (BIAS) {
+                                if (!CAP) x[i] = __fmul2_rn(x[i], both(p.scale_log2));
+                                x[i].x = fmaf(-slope2, fabsf(d0 + (float)(2 * i)), x[i].x);
+                                x[i].y = fmaf(-slope2, fabsf(d0 + (float)(2 * i + 1)), x[i].y);
+                            }
+                            x[i].x = seen & 1u << (2 * i) ? x[i].x : -INFINITY;
+                            x[i].y = seen & 2u << (2 * i) ? x[i].y : -INFINITY;
+                        }
+                    }
+                };
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    if (!(part >> c & 1)) continue;
+                    float2 x[16];
+                    tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<float*>(x));
+                    tmem_ld_wait();
+                    scores(c, x, Flag<CAP && BIAS>());                // the cap alone keeps the order: applied to the maximum below
+                    float t4[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 16; i++) t4[i & 3] = max3(t4[i & 3], x[i].x, x[i].y);
+                    top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                }
+                if (CAP && !BIAS) top = top == -INFINITY ? top : da_tanh(top * p.cap_in) * p.cap_log2;
+                if (!CAP && !BIAS) top *= p.scale_log2;
                 const bool move = top > m_ref + RESCALE_STEP;        // also the row's first visible key (m_ref = -inf)
                 float factor = 1.0f;
                 if (move) {
                     factor = m_ref == -INFINITY ? 0.0f : fast_exp2(m_ref - top);
                     m_ref = top;
-                    l *= factor;
+                    l = __fmul2_rn(l, both(factor));
                 }
-                if (blk > m.r[t].begin && __any_sync(0xffffffffu, move)) {
+                if (blk < blocks.end - 1 && __any_sync(0xffffffffu, move)) {
                     // the accumulator may only be touched between two P V products: wait for the previous one
                     ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (it - 1) & 1));
                     if (!ok) continue;
@@ -491,17 +652,27 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         tmem_st_32x32b_x32(tm_o + c, v);
                     }
                 }
-                const float ref = m_ref == -INFINITY ? 0.0f : m_ref;        // nothing visible yet: every exponential is 0
+                const float2 ref = both(m_ref == -INFINITY ? 0.0f : -m_ref);        // nothing visible yet: every exponential is 0
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    uint32_t w[16];
+                    if (part >> c & 1) {
+                        float2 x[16];
+                        tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<float*>(x));
+                        tmem_ld_wait();
+                        scores(c, x, Flag<true>());
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t w[32];
+                        for (int i = 0; i < 16; i++) {
+                            const float2 e = CAP || BIAS ? __fadd2_rn(x[i], ref) : __ffma2_rn(x[i], both(p.scale_log2), ref);
+                            const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                            l = __fadd2_rn(l, pe);
+                            w[i] = da_half2(pe.x, pe.y);
+                        }
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const float p0 = fast_exp2(x[c * 64 + 2 * e] - ref), p1 = fast_exp2(x[c * 64 + 2 * e + 1] - ref);
-                        l += p0 + p1;
-                        w[e] = da_half2(p0, p1);
+                        for (int i = 0; i < 16; i++) w[i] = 0;
                     }
-                    tmem_st_32x32b_x32(tm_s + c * 32, w);
+                    tmem_st_32x32b_x16(tm_s + c * 16, w);             // over scores that have been read: columns below 32 (c + 1)
                 }
                 tmem_st_wait();
                 tcgen05_fence_before();
@@ -512,8 +683,9 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) continue;
             tcgen05_fence_after();
-            const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);        // a NaN stays one
-            const float lse2 = m_ref + __log2f(l);
+            const float sum = l.x + l.y;
+            const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);        // a NaN stays one
+            const float lse2 = m_ref + __log2f(sum);
             __half* o = p.out + row * p.ld_out + m.head * D;
             const bool none = lo >= hi;
             float bad = 0.0f;
@@ -540,8 +712,9 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             mbar_arrive(&o_empty[t]);
             if (live) {
                 if (p.lse) p.lse[((int64_t)m.b * p.heads + m.head) * p.tokens + qi] = none ? 0.0f : lse2 * LN2;
-                if (bad != 0.0f && !none && fabsf(lse2) < INFINITY) da_out_row<D, CAP>(p, m.b, m.head, qi, lo, hi, lse2);
             }
+            const bool again = live && bad != 0.0f && !none && fabsf(lse2) < INFINITY;
+            if (__any_sync(0xffffffffu, again)) da_mend_out<D, CAP>(p, m.b, m.head, qi, lo, hi, lse2, again);
         }
         if (!ok && lane == 0) atomicExch(&g_doc_error, 3);
     }
@@ -629,7 +802,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     uint64_t* acc_empty = bars + 15;
     uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(bars + 16);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int per_row = (p.tokens + 127) / 128, n_tiles = p.batch * per_row;
     const int group = p.heads / p.kv_heads;
     const bool sorted = n_tiles <= DA_SORT;
@@ -661,7 +834,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem_base = *tmem_base_smem;
+    const uint32_t tmem_base = uniform(*tmem_base_smem);
 
     struct Item {
         int b, t0, head;       // head: of the keys
@@ -678,6 +851,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         return true;
     };
 
+    if (warp < 4) give_registers<DA_REGS_FEW>();
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
@@ -714,12 +888,16 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             if (!ok) atomicExch(&g_doc_error, 11);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        {
             bool ok = true;
-            const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV);
+            const bool issuer = elect_one();
+            const uint64_t k_desc = make_smem_desc_sw128(smem_u32(sK), 16, 1024), v_desc = make_smem_desc_sw128(smem_u32(sV), 16, 1024);
+            const uint64_t q_desc = make_smem_desc_sw128(smem_u32(sQ), 16, 1024), do_desc = make_smem_desc_sw128(smem_u32(sDO), 16, 1024);
+            const uint64_t q_col = make_smem_desc_sw128(smem_u32(sQ), DA_SUB_ATOM, 1024), do_col = make_smem_desc_sw128(smem_u32(sDO), DA_SUB_ATOM, 1024);
             uint32_t it0 = 0, items = 0;
             Item m;
             for (int round = 0; ok && item_of(round, m); round++) {
+                m.n = uniform(m.n);
                 if (m.n == 0) continue;
                 ok = mbar_wait(kv_full, items & 1);
                 // step n issues the transposed scores of block n and then the accumulations of block n - 1, whose P^T / dS^T
@@ -731,17 +909,19 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         ok = mbar_wait(&q_full[s], (i / S::STAGES) & 1);
                         if (!ok) break;
                         tcgen05_fence_after();
-                        const uint32_t q_addr = smem_u32(sQ + s * S::SUB), do_addr = smem_u32(sDO + s * S::SUB);
+                        const uint64_t qd = q_desc + (uint32_t)(s * (S::SUB >> 4)), dod = do_desc + (uint32_t)(s * (S::SUB >> 4));
+                        if (issuer) {
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; kk++)      // S^T = K Q^T : [128 keys x 64 queries]
-                            umma_f16_ss(tmem_base + sb * DA_SUB, make_smem_desc_sw128(k_addr + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
-                                        make_smem_desc_sw128(q_addr + (kk >> 2) * DA_SUB_ATOM + (kk & 3) * 32, 16, 1024), IDESC_ST, kk != 0 ? 1u : 0u);
+                            for (int kk = 0; kk < D / 16; kk++)      // S^T = K Q^T : [128 keys x 64 queries]
+                                umma_f16_ss(tmem_base + sb * DA_SUB, k_desc + (kk >> 2) * 1024 + (kk & 3) * 2, qd + (kk >> 2) * (DA_SUB_ATOM >> 4) + (kk & 3) * 2,
+                                            IDESC_ST, kk != 0 ? 1u : 0u);
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; kk++)      // dP^T = V dO^T
-                            umma_f16_ss(tmem_base + 128 + sb * DA_SUB, make_smem_desc_sw128(v_addr + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
-                                        make_smem_desc_sw128(do_addr + (kk >> 2) * DA_SUB_ATOM + (kk & 3) * 32, 16, 1024), IDESC_ST, kk != 0 ? 1u : 0u);
-                        umma_commit(&s_full[sb]);
-                        if (n == m.n - 1) umma_commit(kv_empty);       // last products of the item that read K / V
+                            for (int kk = 0; kk < D / 16; kk++)      // dP^T = V dO^T
+                                umma_f16_ss(tmem_base + 128 + sb * DA_SUB, v_desc + (kk >> 2) * 1024 + (kk & 3) * 2, dod + (kk >> 2) * (DA_SUB_ATOM >> 4) + (kk & 3) * 2,
+                                            IDESC_ST, kk != 0 ? 1u : 0u);
+                            umma_commit(&s_full[sb]);
+                            if (n == m.n - 1) umma_commit(kv_empty);       // last products of the item that read K / V
+                        }
                     }
                     if (n >= 1) {
                         const uint32_t i = it0 + n - 1;
@@ -750,27 +930,30 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         if (ok && n == 1) ok = mbar_wait(acc_empty, (items & 1) ^ 1);      // the previous item's dV / dK have been read
                         if (!ok) break;
                         tcgen05_fence_after();
-                        const uint32_t q_addr = smem_u32(sQ + s * S::SUB), do_addr = smem_u32(sDO + s * S::SUB);
+                        const uint64_t qd = q_col + (uint32_t)(s * (S::SUB >> 4)), dod = do_col + (uint32_t)(s * (S::SUB >> 4));
+                        if (issuer) {
 #pragma unroll
-                        for (int kk = 0; kk < DA_SUB / 16; kk++)      // dV += P^T dO (contraction over the 64 queries)
-                            umma_f16_ts(tmem_base + 256, tmem_base + sb * DA_SUB + (kk >> 1) * 32 + (kk & 1) * 8,
-                                        make_smem_desc_sw128(do_addr + kk * 2048, DA_SUB_ATOM, 1024), IDESC_ACC, (n != 1 || kk != 0) ? 1u : 0u);
+                            for (int kk = 0; kk < DA_SUB / 16; kk++)      // dV += P^T dO (contraction over the 64 queries)
+                                umma_f16_ts(tmem_base + 256, tmem_base + sb * DA_SUB + (kk >> 1) * 32 + (kk & 1) * 8, dod + kk * 128, IDESC_ACC,
+                                            n != 1 || kk != 0 ? 1u : 0u);
 #pragma unroll
-                        for (int kk = 0; kk < DA_SUB / 16; kk++)      // dK += dS^T Q
-                            umma_f16_ts(tmem_base + 256 + D, tmem_base + 128 + sb * DA_SUB + (kk >> 1) * 32 + (kk & 1) * 8,
-                                        make_smem_desc_sw128(q_addr + kk * 2048, DA_SUB_ATOM, 1024), IDESC_ACC, (n != 1 || kk != 0) ? 1u : 0u);
-                        umma_commit(&q_empty[s]);
+                            for (int kk = 0; kk < DA_SUB / 16; kk++)      // dK += dS^T Q
+                                umma_f16_ts(tmem_base + 256 + D, tmem_base + 128 + sb * DA_SUB + (kk >> 1) * 32 + (kk & 1) * 8, qd + kk * 128, IDESC_ACC,
+                                            n != 1 || kk != 0 ? 1u : 0u);
+                            umma_commit(&q_empty[s]);
+                        }
                     }
                 }
-                if (ok) umma_commit(acc_full);
+                if (ok && issuer) umma_commit(acc_full);
                 it0 += m.n;
                 items++;
             }
-            if (!ok) atomicExch(&g_doc_error, 12);
+            if (!ok && issuer) atomicExch(&g_doc_error, 12);
         }
-    } else {
+    } else if (warp >= 4) {
         // ---------------- row owners: two threads per key, 32 of the 64 query columns each ----------------
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        take_registers<DA_REGS_MANY>();
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
         const int r = quarter * 32 + lane, c0 = half * 32;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
         bool ok = true;
@@ -792,63 +975,99 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             int4 span = make_int4(0, 0, 0, 0x7fffffff);              // rows behind the sequence never force the masked path
             if (live) span = p.spans[row];
             const int qlo = max(span.z, 0), qhi = live ? min(span.w, p.tokens) : span.w;
+            // a step's 64 log-sum-exps (log2 units, with the query's share of the bias) and 64 deltas, all negated: one for each of
+            // the first owners, fetched a step ahead so that the load's latency passes behind the step before it
             int blk = m.r.begin, h = m.head * group;
+            auto fetch = [&]() {
+                const int c = r & 63, i = blk * DA_SUB + c;
+                if (half == 1 || i >= p.tokens) return 0.0f;
+                const int64_t at = ((int64_t)m.b * p.heads + h) * p.tokens + i;
+                if (r >= 64) return -p.delta[at];
+                const float lse2 = p.lse_in[at] * -LOG2E;
+                return BIAS ? fmaf(p.slopes[h] * -LOG2E, (float)c, lse2) : lse2;
+            };
+            float mine = fetch();
             for (int n = 0; n < m.n; n++) {
                 const uint32_t i = it0 + n;
                 const int sb = i & 1, q0 = blk * DA_SUB;
                 const float slope2 = BIAS ? p.slopes[h] * LOG2E : 0.0f;
-                if (half == 0) {
-                    // the step's 64 log-sum-exps (log2 units, with the query's share of the bias) and 64 deltas
-                    const int c = r & 63, qi = q0 + c;
-                    const int64_t at = ((int64_t)m.b * p.heads + h) * p.tokens + qi;
-                    float v = 0.0f;
-                    if (qi < p.tokens) v = r < 64 ? fmaf(p.lse_in[at], LOG2E, slope2 * (float)c) : p.delta[at];
-                    stat[sb * 128 + r] = v;
+                if (half == 0) stat[sb * 128 + r] = mine;
+                if (++blk == m.r.end) {
+                    blk = m.r.begin;
+                    h++;
                 }
+                if (n + 1 < m.n) mine = fetch();
                 // orders this step's writes after every thread's reads two steps ago; every owner reaches it in every step,
                 // also one whose bounded wait gave up (it only skips the work)
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (ok) ok = mbar_wait(&s_full[sb], (i >> 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
-                if (ok) {
-                    tcgen05_fence_after();
-                    const float* lse2 = stat + sb * 128 + c0;
-                    const float* dlt = lse2 + 64;
-                    const bool full = __all_sync(0xffffffffu, qlo <= q0 + c0 && qhi >= q0 + c0 + 32);
-                    const bool past = !BIAS || __all_sync(0xffffffffu, kj <= q0 + c0);
-                    const float bias = slope2 * (float)(kj - q0);          // minus slope * (i - q0), which lse2 holds
-                    uint32_t sv[32], dv[32], wp[16], wd[16];
-                    tmem_ld_32x32b_x32(tm + sb * DA_SUB + c0, sv);
-                    tmem_ld_32x32b_x32(tm + 128 + sb * DA_SUB + c0, dv);
-                    tmem_ld_wait();
+                if (!ok) continue;
+                tcgen05_fence_after();
+                const float4* nlse = reinterpret_cast<const float4*>(stat + sb * 128 + c0);
+                const float4* ndelta = nlse + 16;
+                float2 x[16], g[16];
+                tmem_ld_32x32b_x32(tm + sb * DA_SUB + c0, reinterpret_cast<float*>(x));
+                tmem_ld_32x32b_x32(tm + 128 + sb * DA_SUB + c0, reinterpret_cast<float*>(g));
+                tmem_ld_wait();
+                const float2 bias = both(slope2 * (float)(kj - q0));       // minus slope * (query - q0), which nlse holds
+                const bool inner = qlo <= q0 + c0 && qhi >= q0 + c0 + 32 && (!BIAS || kj <= q0 + c0);
+                const bool plain = __all_sync(0xffffffffu, inner);
+                bool near = true;
+                if (CAP) {
+                    float wide = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float pe[2], de[2];
+                    for (int e = 0; e < 16; e++) wide = max3(wide, fabsf(x[e].x), fabsf(x[e].y));
+                    near = __all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH);
+                }
+                auto step = [&](auto edge, auto reach) {
 #pragma unroll
-                        for (int f = 0; f < 2; f++) {
-                            const int qi = q0 + c0 + e + f;
-                            float dt;
-                            float s = da_score<CAP>(__uint_as_float(sv[e + f]), p, dt);
-                            s += bias - lse2[e + f];
-                            if (BIAS && !past) s += fminf(0.0f, 2.0f * slope2 * (float)(qi - kj));        // a key ahead of the query: -slope (j - i)
-                            pe[f] = fast_exp2(s);
-                            de[f] = pe[f] * (__uint_as_float(dv[e + f]) - dlt[e + f]);
-                            if (CAP) de[f] *= dt;
-                            if (!full && !(qlo <= qi && qi < qhi)) pe[f] = de[f] = 0.0f;
+                    for (int e = 0; e < 16; e++) {
+                        const float4 l4 = nlse[e >> 1], d4 = ndelta[e >> 1];
+                        float2 off = e & 1 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+                        const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
+                        if (BIAS) off = __fadd2_rn(off, bias);
+                        const int far = q0 + c0 + 2 * e - kj;              // query - key
+                        if (BIAS && edge) {                                // a key ahead of the query: -slope (key - query)
+                            off.x += fminf(0.0f, 2.0f * slope2 * (float)far);
+                            off.y += fminf(0.0f, 2.0f * slope2 * (float)(far + 1));
                         }
-                        wp[e >> 1] = da_half2(pe[0], pe[1]);
-                        wd[e >> 1] = da_half2(de[0], de[1]);
+                        float2 s, t;
+                        if (CAP) {
+                            t = da_capped(x[e], p, reach);
+                            s = __ffma2_rn(t, both(p.cap_log2), off);
+                        } else {
+                            s = __ffma2_rn(x[e], both(p.scale_log2), off);
+                        }
+                        float2 pe = make_float2(fast_exp2(s.x), fast_exp2(s.y));
+                        float2 de = __fmul2_rn(pe, __fadd2_rn(g[e], nd));
+                        if (CAP) de = __fmul2_rn(de, __ffma2_rn(neg2(t), t, both(1.0f)));
+                        if (edge) {
+                            const int qi = q0 + c0 + 2 * e;
+                            if (!(qlo <= qi && qi < qhi)) pe.x = de.x = 0.0f;
+                            if (!(qlo <= qi + 1 && qi + 1 < qhi)) pe.y = de.y = 0.0f;
+                        }
+                        x[e].x = __uint_as_float(da_half2(pe.x, pe.y));
+                        g[e].x = __uint_as_float(da_half2(de.x, de.y));
                     }
-                    tmem_st_32x32b_x16(tm + sb * DA_SUB + c0, wp);
-                    tmem_st_32x32b_x16(tm + 128 + sb * DA_SUB + c0, wd);
-                    tmem_st_wait();
-                    tcgen05_fence_before();
-                    mbar_arrive(&p_full[sb]);
+                };
+                if (near) {
+                    if (plain) step(Flag<false>(), Flag<true>());
+                    else step(Flag<true>(), Flag<true>());
+                } else {
+                    step(Flag<true>(), Flag<false>());
                 }
-                if (++blk == m.r.end) {
-                    blk = m.r.begin;
-                    h++;
+                uint32_t wp[16], wd[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    wp[e] = __float_as_uint(x[e].x);
+                    wd[e] = __float_as_uint(g[e].x);
                 }
+                tmem_st_32x32b_x16(tm + sb * DA_SUB + c0, wp);
+                tmem_st_32x32b_x16(tm + 128 + sb * DA_SUB + c0, wd);
+                tmem_st_wait();
+                tcgen05_fence_before();
+                mbar_arrive(&p_full[sb]);
             }
             it0 += m.n;
             if (ok) ok = mbar_wait(acc_full, items & 1);
@@ -883,10 +1102,11 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 tcgen05_fence_before();
                 mbar_arrive(acc_empty);            // the accumulators may take the next item's first products
             }
-            // Evaluated again by the row's first owner, after both owners' stores (the barrier orders them).
+            // evaluated again by the warps of the rows' first owners, after both owners' stores (the barrier orders them)
             stat[half * 128 + r] = bad;
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (half == 0 && live && !none && (stat[r] != 0.0f || stat[128 + r] != 0.0f)) da_dkv_row<D, CAP>(p, m.b, m.head, kj, qlo, qhi);
+            const bool redo = live && !none && (stat[r] != 0.0f || stat[128 + r] != 0.0f);
+            if (half == 0 && __any_sync(0xffffffffu, redo)) da_mend_dkv<D, CAP>(p, m.b, m.head, kj, qlo, qhi, redo);
             asm volatile("bar.sync 1, 256;" ::: "memory");
         }
         if (!ok && lane == 0) atomicExch(&g_doc_error, 13);
@@ -940,7 +1160,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     uint64_t* acc_empty = bars + 17;
     uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(bars + 18);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int per_row = (p.tokens + 127) / 128, n_tiles = p.batch * per_row;
     const int group = p.heads / p.kv_heads;
     const bool sorted = n_tiles <= DA_SORT;
@@ -974,7 +1194,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem_base = *tmem_base_smem;
+    const uint32_t tmem_base = uniform(*tmem_base_smem);
 
     struct Item {
         int b, t0, head;
@@ -991,6 +1211,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         return true;
     };
 
+    if (warp < 4) give_registers<DA_REGS_FEW>();
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
@@ -1025,12 +1246,16 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             if (!ok) atomicExch(&g_doc_error, 21);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        {
             bool ok = true;
-            const uint32_t q_addr = smem_u32(sQ), do_addr = smem_u32(sDO);
+            const bool issuer = elect_one();
+            const uint64_t q_desc = make_smem_desc_sw128(smem_u32(sQ), 16, 1024), do_desc = make_smem_desc_sw128(smem_u32(sDO), 16, 1024);
+            const uint64_t k_desc = make_smem_desc_sw128(smem_u32(sK), 16, 1024), v_desc = make_smem_desc_sw128(smem_u32(sV), 16, 1024);
+            const uint64_t k_col = make_smem_desc_sw128(smem_u32(sK), 16384, 1024);
             uint32_t it0 = 0, items = 0;
             Item m;
             for (int round = 0; ok && item_of(round, m); round++) {
+                m.n = uniform(m.n);
                 if (m.n == 0) continue;
                 ok = mbar_wait(q_full, items & 1);
                 for (int n = 0; n <= m.n && ok; n++) {
@@ -1040,26 +1265,26 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                         ok = mbar_wait(&k_full[s], (i / S::STAGES) & 1);
                         if (!ok) break;
                         tcgen05_fence_after();
-                        const uint32_t k_addr = smem_u32(sK + s * S::TILE), v_addr = smem_u32(sV + s * S::TILE);
+                        const uint64_t kd = k_desc + (uint32_t)(s * (S::TILE >> 4)), vd = v_desc + (uint32_t)(s * (S::TILE >> 4));
+                        if (issuer) {
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; kk++) {     // S = Q K^T : [128 queries x 128 keys]
-                            const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-                            umma_f16_ss(tmem_base + sb * 128, make_smem_desc_sw128(q_addr + off, 16, 1024), make_smem_desc_sw128(k_addr + off, 16, 1024), IDESC_S,
-                                        kk != 0 ? 1u : 0u);
+                            for (int kk = 0; kk < D / 16; kk++)      // S = Q K^T : [128 queries x 128 keys]
+                                umma_f16_ss(tmem_base + sb * 128, q_desc + (kk >> 2) * 1024 + (kk & 3) * 2, kd + (kk >> 2) * 1024 + (kk & 3) * 2, IDESC_S,
+                                            kk != 0 ? 1u : 0u);
+                            umma_commit(&s_full[sb]);
                         }
-                        umma_commit(&s_full[sb]);
                         ok = mbar_wait(&v_full[s], (i / S::STAGES) & 1) && mbar_wait(dp_empty, (i & 1) ^ 1);
                         if (!ok) break;
                         tcgen05_fence_after();
+                        if (issuer) {
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; kk++) {     // dP = dO V^T
-                            const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-                            umma_f16_ss(tmem_base + 256, make_smem_desc_sw128(do_addr + off, 16, 1024), make_smem_desc_sw128(v_addr + off, 16, 1024), IDESC_S,
-                                        kk != 0 ? 1u : 0u);
+                            for (int kk = 0; kk < D / 16; kk++)      // dP = dO V^T
+                                umma_f16_ss(tmem_base + 256, do_desc + (kk >> 2) * 1024 + (kk & 3) * 2, vd + (kk >> 2) * 1024 + (kk & 3) * 2, IDESC_S,
+                                            kk != 0 ? 1u : 0u);
+                            umma_commit(dp_full);
+                            umma_commit(&v_empty[s]);
+                            if (n == m.n - 1) umma_commit(q_empty);
                         }
-                        umma_commit(dp_full);
-                        umma_commit(&v_empty[s]);
-                        if (n == m.n - 1) umma_commit(q_empty);
                     }
                     if (n >= 1) {
                         const uint32_t i = it0 + n - 1;
@@ -1068,23 +1293,26 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                         if (ok && n == 1) ok = mbar_wait(acc_empty, (items & 1) ^ 1);
                         if (!ok) break;
                         tcgen05_fence_after();
-                        const uint32_t k_addr = smem_u32(sK + s * S::TILE);
+                        const uint64_t kd = k_col + (uint32_t)(s * (S::TILE >> 4));
+                        if (issuer) {
 #pragma unroll
-                        for (int kk = 0; kk < 8; kk++)            // dQ += dS K : dS [128 q x 128 keys] in tensor memory, K [128 keys x d], d contiguous
-                            umma_f16_ts(tmem_base + 384, tmem_base + sb * 128 + (kk >> 2) * 64 + (kk & 3) * 8, make_smem_desc_sw128(k_addr + kk * 2048, 16384, 1024),
-                                        IDESC_DQ, (n != 1 || kk != 0) ? 1u : 0u);
-                        umma_commit(&k_empty[s]);
+                            for (int kk = 0; kk < 8; kk++)            // dQ += dS K : dS [128 q x 128 keys] in tensor memory, K [128 keys x d], d contiguous
+                                umma_f16_ts(tmem_base + 384, tmem_base + sb * 128 + (kk >> 2) * 64 + (kk & 3) * 8, kd + kk * 128, IDESC_DQ,
+                                            n != 1 || kk != 0 ? 1u : 0u);
+                            umma_commit(&k_empty[s]);
+                        }
                     }
                 }
-                if (ok) umma_commit(acc_full);
+                if (ok && issuer) umma_commit(acc_full);
                 it0 += m.n;
                 items++;
             }
-            if (!ok) atomicExch(&g_doc_error, 22);
+            if (!ok && issuer) atomicExch(&g_doc_error, 22);
         }
-    } else {
+    } else if (warp >= 4) {
         // ---------------- row owners: two threads per query, 64 of the 128 key columns each ----------------
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        take_registers<DA_REGS_MANY>();
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
         const int r = quarter * 32 + lane, c0 = half * 64;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
         bool ok = true;
@@ -1116,37 +1344,60 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sb], (i >> 1) & 1) && mbar_wait(dp_full, i & 1));
                 if (!ok) break;
                 tcgen05_fence_after();
-                const bool full = __all_sync(0xffffffffu, lo <= kbase && hi >= kbase + 64);
-                const bool past = !ahead || __all_sync(0xffffffffu, kbase + 63 <= qi);
-                const float dist = (float)(kbase - qi), base = fmaf(slope2, dist, -lse2);
+                const bool inner = lo <= kbase && hi >= kbase + 64 && (!BIAS || kbase + 63 <= qi || !ahead);
+                const bool plain = __all_sync(0xffffffffu, inner);
+                const float dist = (float)(kbase - qi);
+                const float2 base = both(fmaf(slope2, dist, -lse2));
+                const int from = lo - kbase, to = hi - kbase;
                 uint32_t w[2][16];
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    uint32_t sv[32], dv[32];
-                    tmem_ld_32x32b_x32(tm + sb * 128 + c0 + c * 32, sv);
-                    tmem_ld_32x32b_x32(tm + 256 + c0 + c * 32, dv);
+                    float2 x[16], g[16];
+                    tmem_ld_32x32b_x32(tm + sb * 128 + c0 + c * 32, reinterpret_cast<float*>(x));
+                    tmem_ld_32x32b_x32(tm + 256 + c0 + c * 32, reinterpret_cast<float*>(g));
                     tmem_ld_wait();
                     if (c == 1) {
                         tcgen05_fence_before();
                         mbar_arrive(dp_empty);
                     }
+                    bool near = true;
+                    if (CAP) {
+                        float wide = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float de[2];
+                        for (int e = 0; e < 16; e++) wide = max3(wide, fabsf(x[e].x), fabsf(x[e].y));
+                        near = __all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH);
+                    }
+                    auto step = [&](auto edge, auto reach) {
 #pragma unroll
-                        for (int f = 0; f < 2; f++) {
-                            const int k = c * 32 + e + f;
-                            float dt;
-                            float s = da_score<CAP>(__uint_as_float(sv[e + f]), p, dt);
-                            if (BIAS)
-                                s += past ? fmaf(slope2, (float)k, base) : fmaf(-slope2, fabsf(dist + (float)k), -lse2);
-                            else
-                                s -= lse2;
-                            de[f] = fast_exp2(s) * (__uint_as_float(dv[e + f]) - dlt);
-                            if (CAP) de[f] *= dt;
-                            if (!full && !(kbase + k >= lo && kbase + k < hi)) de[f] = 0.0f;
+                        for (int e = 0; e < 16; e++) {
+                            const int k = c * 32 + 2 * e;
+                            float2 off = base, s, t;
+                            if (BIAS) {
+                                if (edge)
+                                    off = make_float2(fmaf(-slope2, fabsf(dist + (float)k), -lse2), fmaf(-slope2, fabsf(dist + (float)(k + 1)), -lse2));
+                                else
+                                    off = __ffma2_rn(both(slope2), pair_of(c * 16 + e), base);
+                            }
+                            if (CAP) {
+                                t = da_capped(x[e], p, reach);
+                                s = __ffma2_rn(t, both(p.cap_log2), off);
+                            } else {
+                                s = __ffma2_rn(x[e], both(p.scale_log2), off);
+                            }
+                            float2 de = __fmul2_rn(make_float2(fast_exp2(s.x), fast_exp2(s.y)), __fadd2_rn(g[e], both(-dlt)));
+                            if (CAP) de = __fmul2_rn(de, __ffma2_rn(neg2(t), t, both(1.0f)));
+                            if (edge) {
+                                if (!(k >= from && k < to)) de.x = 0.0f;
+                                if (!(k + 1 >= from && k + 1 < to)) de.y = 0.0f;
+                            }
+                            w[c][e] = da_half2(de.x, de.y);
                         }
-                        w[c][e >> 1] = da_half2(de[0], de[1]);
+                    };
+                    if (near) {
+                        if (plain) step(Flag<false>(), Flag<true>());
+                        else step(Flag<true>(), Flag<true>());
+                    } else {
+                        step(Flag<true>(), Flag<false>());
                     }
                 }
                 tmem_st_32x32b_x16(tm + sb * 128 + c0, w[0]);
@@ -1185,10 +1436,11 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 tcgen05_fence_before();
                 mbar_arrive(acc_empty);
             }
-            // evaluated again by the row's first owner, after both owners' stores (the barrier orders them)
+            // evaluated again by the warps of the rows' first owners, after both owners' stores (the barrier orders them)
             again[half * 128 + r] = bad;
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (half == 0 && live && !none && (again[r] != 0.0f || again[128 + r] != 0.0f)) da_dq_row<D, CAP>(p, m.b, m.head, qi, lo, hi);
+            const bool redo = live && !none && (again[r] != 0.0f || again[128 + r] != 0.0f);
+            if (half == 0 && __any_sync(0xffffffffu, redo)) da_mend_dq<D, CAP>(p, m.b, m.head, qi, lo, hi, redo);
             asm volatile("bar.sync 1, 256;" ::: "memory");
         }
         if (!ok && lane == 0) atomicExch(&g_doc_error, 23);
@@ -1288,7 +1540,7 @@ static DocAttn da_params(const void* q, const void* k, const void* v, int64_t ld
     p.scale = (float)scale;
     p.scale_log2 = (float)(scale * log2e);
     p.cap_log2 = (float)(cap * log2e);
-    p.cap_in = cap > 0.0f ? (float)(2.0 * scale * log2e / cap) : 0.0f;
+    p.cap_in = cap > 0.0f ? (float)(scale / cap) : 0.0f;
     return p;
 }
 
