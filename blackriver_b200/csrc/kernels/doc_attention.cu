@@ -45,6 +45,7 @@ struct DocAttn {
     float scale, scale_log2;                // 1/sqrt(d), times log2(e)
     float cap_log2, cap_in;                 // cap log2(e); 1 / (sqrt(d) cap)
     // forward
+    bool wide_out;                          // rows of out start on 32-byte boundaries
     __half* out;
     float* lse;                             // [batch, heads, tokens], natural log
     // backward
@@ -132,7 +133,7 @@ __device__ __forceinline__ Range da_blocks(const DocAttn& p, int b, int t0, int 
 // tile); the table lives in shared memory.
 struct DaTable {
     uint16_t order[DA_SORT];
-    uint16_t weight[DA_SORT];
+    ushort4 blocks[DA_SORT];                // per tile: first and last block it needs, of its first and second half
 };
 __device__ __forceinline__ bool da_item(int round, int n_tiles, int n_heads, const DaTable* table, bool sorted, int& tile, int& head) {
     const int64_t G = gridDim.x, c = blockIdx.x;
@@ -143,15 +144,25 @@ __device__ __forceinline__ bool da_item(int round, int n_tiles, int n_heads, con
     head = (int)(idx % n_heads);
     return true;
 }
-// weight(tile) for all tiles, then the rank of each: heavier first, ties by number.  All threads of the CTA.
-template <typename W>
-__device__ __forceinline__ void da_sort(DaTable* table, int n_tiles, W weight) {
-    for (int i = threadIdx.x; i < n_tiles; i += DA_THREADS) table->weight[i] = (uint16_t)min(weight(i), 65535);
+// ranges(tile, second half) for all tiles, then the rank of each by the blocks it needs: heavier first, ties by number.  All threads of the CTA.
+template <typename R>
+__device__ __forceinline__ void da_sort(DaTable* table, int n_tiles, R ranges) {
+    for (int i = threadIdx.x; i < n_tiles; i += blockDim.x) {
+        const Range a = ranges(i, false), c = ranges(i, true);
+        table->blocks[i] = make_ushort4(a.begin, a.end, c.begin, c.end);
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < n_tiles; i += DA_THREADS) {
-        const int w = table->weight[i];
+    auto weight = [&](int i) {
+        const ushort4 t = table->blocks[i];
+        return t.y - t.x + t.w - t.z;
+    };
+    for (int i = threadIdx.x; i < n_tiles; i += blockDim.x) {
+        const int w = weight(i);
         int rank = 0;
-        for (int j = 0; j < n_tiles; j++) rank += table->weight[j] > w || (table->weight[j] == w && j < i);
+        for (int j = 0; j < n_tiles; j++) {
+            const int v = weight(j);
+            rank += v > w || (v == w && j < i);
+        }
         table->order[rank] = (uint16_t)i;
     }
 }
@@ -319,6 +330,20 @@ __device__ __noinline__ void da_mend_dkv(const DocAttn& p, int b, int kh, int j,
 __device__ __forceinline__ void da_zero_row(__half* row, int d) {
     for (int e = 0; e < d; e += 8) *reinterpret_cast<uint4*>(row + e) = make_uint4(0, 0, 0, 0);
 }
+// 64 bytes of a row.  Neighbouring lanes write rows far apart, so a lane writes whole sectors of 32 bytes where the row is
+// aligned to them.
+__device__ __forceinline__ void da_store64(__half* to, const uint32_t (&w)[16], bool wide) {
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 8)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + i * 2), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]),
+                         "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                         : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(to + i * 2) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
+}
 __device__ __forceinline__ uint32_t da_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -342,11 +367,13 @@ template <int D>
 struct FwdSmem {
     static constexpr uint32_t TILE = 128 * D * 2;
     static constexpr int STAGES = 2;                    // of K and of V each
-    static constexpr size_t BYTES = 1024 + TILE * (2 + 2 * STAGES) + sizeof(DaTable) + 256;
+    static constexpr size_t BYTES = 1024 + TILE * (2 + 2 * STAGES) + sizeof(DaTable) + 256 + 2 * 2 * 2 * 128 * sizeof(float);
 };
 
+constexpr int DA_FWD_THREADS = 64 + 512;
+
 template <int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(DA_THREADS, 1)
+__global__ void __launch_bounds__(DA_FWD_THREADS, 1)
 doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                     const __grid_constant__ DocAttn p) {
     using S = FwdSmem<D>;
@@ -373,6 +400,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     uint64_t* o_done = bars + 16;            // 2: a P V product of the tile is complete
     uint64_t* o_empty = bars + 18;           // 2: the tile's output has been read
     uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(bars + 20);
+    float* exchange = reinterpret_cast<float*>(bars + 32);       // [tile][turn][owner][row]: the two owners' maxima
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int per_row = (p.tokens + 255) / 256, n_pairs = p.batch * per_row;
@@ -387,9 +415,9 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             mbar_init(&v_full[t], 1);
             mbar_init(&v_empty[t], 1);
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[t], 128);
+            mbar_init(&p_full[t], 256);
             mbar_init(&o_done[t], 1);
-            mbar_init(&o_empty[t], 128);
+            mbar_init(&o_empty[t], 256);
         }
         fence_barrier_init();
         prefetch_tensormap(&tmap_q);
@@ -401,11 +429,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         tmem_relinquish();
     }
     if (sorted)
-        da_sort(table, n_pairs, [&](int i) {
-            const int b = i / per_row, t0 = (i % per_row) * 256;
-            const Range r0 = da_blocks<true>(p, b, t0, 128), r1 = da_blocks<true>(p, b, t0 + 128, 128);
-            return r0.end - r0.begin + r1.end - r1.begin;
-        });
+        da_sort(table, n_pairs, [&](int i, bool second) { return da_blocks<true>(p, i / per_row, (i % per_row) * 256 + (second ? 128 : 0), 128); });
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -422,15 +446,20 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         if (!da_item(round, n_pairs, p.heads, table, sorted, pair, m.head)) return false;
         m.b = pair / per_row;
         m.t0 = (pair % per_row) * 256;
-        m.r0 = da_blocks<true>(p, m.b, m.t0, 128);
-        m.r1 = da_blocks<true>(p, m.b, m.t0 + 128, 128);
+        if (sorted) {
+            const ushort4 t = table->blocks[pair];
+            m.r0 = {t.x, t.y};
+            m.r1 = {t.z, t.w};
+        } else {
+            m.r0 = da_blocks<true>(p, m.b, m.t0, 128);
+            m.r1 = da_blocks<true>(p, m.b, m.t0 + 128, 128);
+        }
         const bool has0 = m.r0.end > m.r0.begin, has1 = m.r1.end > m.r1.begin;
         m.last = max(m.r0.end, m.r1.end) - 1;
         m.n = m.last + 1 - (has0 ? (has1 ? min(m.r0.begin, m.r1.begin) : m.r0.begin) : m.r1.begin);
         return true;
     };
 
-    if (warp < 4) give_registers<DA_REGS_FEW>();
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         if (lane == 0) {
@@ -496,7 +525,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                             if (issuer) {
 #pragma unroll
                                 for (int kk = 0; kk < 8; kk++)        // A = P [128 q x 128 keys] in tensor memory, B = V [128 keys x D], d contiguous
-                                    umma_f16_ts(tmem_base + 256 + t * D, tmem_base + t * 128 + kk * 8, vd + kk * 128, IDESC_PV, kk != 0 || !first ? 1u : 0u);
+                                    umma_f16_ts(tmem_base + 256 + t * D, tmem_base + t * 128 + (kk >> 2) * 64 + (kk & 3) * 8, vd + kk * 128, IDESC_PV, kk != 0 || !first ? 1u : 0u);
                                 umma_commit(&o_done[t]);
                             }
                             p_count++;
@@ -528,55 +557,65 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             }
             if (!ok && issuer) atomicExch(&g_doc_error, 2);
         }
-    } else if (warp >= 4) {
-        // ---------------- softmax / epilogue: one thread per query of the tile ----------------
-        take_registers<DA_REGS_MANY>();
-        const int t = (warp - 4) >> 2;                  // tile: warps 4-7 and 8-11
+    } else {
+        // ---------------- softmax / epilogue: two threads per query, 64 of the 128 key columns each ----------------
+        const int t = (warp - 2) >> 3, half = (warp - 2) >> 2 & 1;
         const int quarter = warp & 3;                   // a warp reaches tensor-memory lanes 32 * (warp % 4) ..
         const int r = quarter * 32 + lane;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t tm_s = tm + t * 128, tm_o = tm + 256 + t * D;
+        const uint32_t tm_s = tm + t * 128 + half * 64, tm_o = tm + 256 + t * D + half * (D / 2);
+        float* const cells = exchange + t * 512 + r;
+        // The owners of 32 rows meet once a block.  Every owner reaches it in every block, also one whose bounded wait gave up.
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quarter) : "memory"); };
         bool ok = true;
         uint32_t it = 0;
         Item m;
-        for (int round = 0; item_of(round, m); round++) {
-            const Range blocks = t == 0 ? m.r0 : m.r1;
+        auto span_of = [&]() {
             const int qi = m.t0 + t * 128 + r;
+            // rows behind the sequence never force the masked path
+            return qi < p.tokens ? p.spans[(int64_t)m.b * p.tokens + qi] : make_int4(0, 0x7fffffff, 0, 0);
+        };
+        bool have = item_of(0, m);
+        int4 span = make_int4(0, 0, 0, 0);
+        if (have) span = span_of();
+        for (int round = 1; have; round++) {
+            const Range blocks = t == 0 ? m.r0 : m.r1;
+            const int head = m.head, b = m.b, qi = m.t0 + t * 128 + r;
             const bool live = qi < p.tokens;
-            const int64_t row = (int64_t)m.b * p.tokens + qi;
-            int4 span = make_int4(0, 0x7fffffff, 0, 0);             // rows behind the sequence never force the masked path
-            if (live) span = p.spans[row];
+            const int64_t row = (int64_t)b * p.tokens + qi;
             const int lo = max(span.x, 0), hi = live ? min(span.y, p.tokens) : span.y;
+            have = item_of(round, m);                   // the next item's span travels while this one is worked on
+            if (have) span = span_of();
+            __half* o = p.out + row * p.ld_out + head * D + half * (D / 2);
+            float* lse = p.lse && half == 0 ? p.lse + ((int64_t)b * p.heads + head) * p.tokens + qi : nullptr;
             if (blocks.end == blocks.begin) {
                 if (live) {
-                    da_zero_row(p.out + row * p.ld_out + m.head * D, D);
-                    if (p.lse) p.lse[((int64_t)m.b * p.heads + m.head) * p.tokens + qi] = 0.0f;
+                    da_zero_row(o, D / 2);
+                    if (lse) *lse = 0.0f;
                 }
                 continue;
             }
-            const float slope2 = BIAS ? p.slopes[m.head] * LOG2E : 0.0f;
+            const float slope2 = BIAS ? p.slopes[head] * LOG2E : 0.0f;
             const bool ahead = BIAS && __any_sync(0xffffffffu, live && hi > qi + 1);      // some row sees keys behind itself: the prompt's
             float m_ref = -INFINITY;
             float2 l = both(0.0f);
             for (int blk = blocks.end - 1; blk >= blocks.begin; blk--, it++) {
                 if (ok) ok = mbar_wait(&s_full[t], it & 1);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) continue;
-                tcgen05_fence_after();
-                // The scores are read twice, 32 columns at a time: once for the maximum, once for the exponentials.  Keeping all 128
-                // in registers instead made straight-line code of some 1400 instructions a block, which one warp per scheduler and
-                // tile could not run through in less than 5 clocks each.
-                const int kbase = blk * 128;
+                // The scores are read twice, 32 columns at a time: once for the maximum, once for the exponentials.  Keeping all of
+                // a row's in registers instead made straight-line code of some 1400 instructions a block, which the warps could
+                // not run through in less than 5 clocks each.
+                const int kbase = blk * 128 + half * 64;
                 uint32_t part = 0, whole = 0;                         // which chunks some row of the warp sees, and all rows see throughout
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < 2; c++) {
                     const int k0 = kbase + c * 32;
                     if (lo < k0 + 32 && hi > k0) part |= 1u << c;
                     if (lo <= k0 && hi >= k0 + 32 && (!BIAS || !ahead || k0 + 31 <= qi)) whole |= 1u << c;
                 }
                 part = __reduce_or_sync(0xffffffffu, part);
                 whole = __reduce_and_sync(0xffffffffu, whole);
-                const float slant = slope2 * (float)(kbase - qi), dist = (float)(kbase - qi);
+                const float dist = (float)(kbase - qi), slant = slope2 * dist;
                 // chunk c of the scores: in log2 units with a cap or a bias, else as they are; what is masked -inf
                 auto scores = [&](int c, float2(&x)[16], auto capped) {
                     if (CAP && capped) {
@@ -616,18 +655,26 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     }
                 };
                 float top = -INFINITY;
+                if (ok) {
+                    tcgen05_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    if (!(part >> c & 1)) continue;
-                    float2 x[16];
-                    tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<float*>(x));
-                    tmem_ld_wait();
-                    scores(c, x, Flag<CAP && BIAS>());                // the cap alone keeps the order: applied to the maximum below
-                    float t4[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+                    for (int c = 0; c < 2; c++) {
+                        if (!(part >> c & 1)) continue;
+                        float2 x[16];
+                        tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<float*>(x));
+                        tmem_ld_wait();
+                        scores(c, x, Flag<CAP && BIAS>());            // the cap alone keeps the order: applied to the maximum below
+                        float t4[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 16; i++) t4[i & 3] = max3(t4[i & 3], x[i].x, x[i].y);
-                    top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                        for (int i = 0; i < 16; i++) t4[i & 3] = max3(t4[i & 3], x[i].x, x[i].y);
+                        top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                    }
                 }
+                float* const cell = cells + (it & 1) * 256;           // two turns, so that one meeting a block is enough
+                cell[half * 128] = top;
+                meet();
+                top = fmaxf(top, cell[(half ^ 1) * 128]);
+                if (!ok) continue;
                 if (CAP && !BIAS) top = top == -INFINITY ? top : da_tanh(top * p.cap_in) * p.cap_log2;
                 if (!CAP && !BIAS) top *= p.scale_log2;
                 const bool move = top > m_ref + RESCALE_STEP;        // also the row's first visible key (m_ref = -inf)
@@ -643,7 +690,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     if (!ok) continue;
                     tcgen05_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
+                    for (int c = 0; c < D / 2; c += 32) {
                         uint32_t v[32];
                         tmem_ld_32x32b_x32(tm_o + c, v);
                         tmem_ld_wait();
@@ -654,7 +701,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 }
                 const float2 ref = both(m_ref == -INFINITY ? 0.0f : -m_ref);        // nothing visible yet: every exponential is 0
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < 2; c++) {
                     uint32_t w[16];
                     if (part >> c & 1) {
                         float2 x[16];
@@ -672,49 +719,49 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 #pragma unroll
                         for (int i = 0; i < 16; i++) w[i] = 0;
                     }
-                    tmem_st_32x32b_x16(tm_s + c * 16, w);             // over scores that have been read: columns below 32 (c + 1)
+                    tmem_st_32x32b_x16(tm_s + c * 16, w);             // over this owner's scores that have been read: columns below 32 (c + 1)
                 }
                 tmem_st_wait();
                 tcgen05_fence_before();
                 mbar_arrive(&p_full[t]);
             }
             // epilogue: O / l -> fp16, token-major; log-sum-exp for the backward
+            float* const cell = cells + (it & 1) * 256;
+            cell[half * 128] = l.x + l.y;
+            meet();
+            const float sum = cell[0] + cell[128];
+            meet();                                     // the next item's first block uses the same cells
             if (ok) ok = mbar_wait(&o_done[t], (it - 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) continue;
-            tcgen05_fence_after();
-            const float sum = l.x + l.y;
             const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);        // a NaN stays one
             const float lse2 = m_ref + __log2f(sum);
-            __half* o = p.out + row * p.ld_out + m.head * D;
             const bool none = lo >= hi;
             float bad = 0.0f;
+            if (ok) {
+                tcgen05_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tm_o + c, v);
-                tmem_ld_wait();
-                if (live) {
+                for (int c = 0; c < D / 2; c += 32) {
+                    float2 x[16];
+                    tmem_ld_32x32b_x32(tm_o + c, reinterpret_cast<float*>(x));
+                    tmem_ld_wait();
+                    uint32_t w[16];
 #pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        Vec<__half> w;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const float a = __uint_as_float(v[g * 8 + e]);
-                            bad = fmaf(a, 0.0f, bad);
-                            w.v[e] = none ? 0.0f : a * inv;
-                        }
-                        w.store(o + c + g * 8);
+                    for (int i = 0; i < 16; i++) {
+                        bad = fmaf(x[i].x, 0.0f, fmaf(x[i].y, 0.0f, bad));
+                        w[i] = none ? 0 : da_half2(x[i].x * inv, x[i].y * inv);
                     }
+                    if (live) da_store64(o + c, w, p.wide_out);
                 }
-            }
-            tcgen05_fence_before();
-            mbar_arrive(&o_empty[t]);
-            if (live) {
-                if (p.lse) p.lse[((int64_t)m.b * p.heads + m.head) * p.tokens + qi] = none ? 0.0f : lse2 * LN2;
+                tcgen05_fence_before();
+                mbar_arrive(&o_empty[t]);
+                if (live && lse) *lse = none ? 0.0f : lse2 * LN2;
             }
             const bool again = live && bad != 0.0f && !none && fabsf(lse2) < INFINITY;
-            if (__any_sync(0xffffffffu, again)) da_mend_out<D, CAP>(p, m.b, m.head, qi, lo, hi, lse2, again);
+            cell[half * 128] = again ? 1.0f : 0.0f;
+            meet();                                     // orders both owners' stores before the row is written again
+            const bool redo = cell[0] + cell[128] != 0.0f;
+            if (half == 0 && __any_sync(0xffffffffu, redo)) da_mend_out<D, CAP>(p, b, head, qi, lo, hi, lse2, redo);
+            meet();
         }
         if (!ok && lane == 0) atomicExch(&g_doc_error, 3);
     }
@@ -827,10 +874,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         tmem_relinquish();
     }
     if (sorted)
-        da_sort(table, n_tiles, [&](int i) {
-            const Range r = da_blocks<false>(p, i / per_row, (i % per_row) * 128, DA_SUB);
-            return r.end - r.begin;
-        });
+        da_sort(table, n_tiles, [&](int i, bool second) { return second ? Range{0, 0} : da_blocks<false>(p, i / per_row, (i % per_row) * 128, DA_SUB); });
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -846,7 +890,8 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         if (!da_item(round, n_tiles, p.kv_heads, table, sorted, tile, m.head)) return false;
         m.b = tile / per_row;
         m.t0 = (tile % per_row) * 128;
-        m.r = da_blocks<false>(p, m.b, m.t0, DA_SUB);
+        if (sorted) m.r = {table->blocks[tile].x, table->blocks[tile].y};
+        else m.r = da_blocks<false>(p, m.b, m.t0, DA_SUB);
         m.n = (m.r.end - m.r.begin) * group;
         return true;
     };
@@ -1187,10 +1232,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         tmem_relinquish();
     }
     if (sorted)
-        da_sort(table, n_tiles, [&](int i) {
-            const Range r = da_blocks<true>(p, i / per_row, (i % per_row) * 128, 128);
-            return r.end - r.begin;
-        });
+        da_sort(table, n_tiles, [&](int i, bool second) { return second ? Range{0, 0} : da_blocks<true>(p, i / per_row, (i % per_row) * 128, 128); });
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -1206,7 +1248,8 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (!da_item(round, n_tiles, p.heads, table, sorted, tile, m.head)) return false;
         m.b = tile / per_row;
         m.t0 = (tile % per_row) * 128;
-        m.r = da_blocks<true>(p, m.b, m.t0, 128);
+        if (sorted) m.r = {table->blocks[tile].x, table->blocks[tile].y};
+        else m.r = da_blocks<true>(p, m.b, m.t0, 128);
         m.n = m.r.end - m.r.begin;
         return true;
     };
@@ -1481,7 +1524,7 @@ static int da_fwd(const DocMaps& t, const DocAttn& p, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     const int rc = da_allow_smem(doc_attn_fwd_kernel<D, CAP, BIAS>, smem, done, "doc_attn_fwd smem attribute");
     if (rc) return rc;
-    doc_attn_fwd_kernel<D, CAP, BIAS><<<da_grid((int64_t)p.batch * ((p.tokens + 255) / 256) * p.heads), DA_THREADS, smem, st>>>(t.q, t.k, t.v, p);
+    doc_attn_fwd_kernel<D, CAP, BIAS><<<da_grid((int64_t)p.batch * ((p.tokens + 255) / 256) * p.heads), DA_FWD_THREADS, smem, st>>>(t.q, t.k, t.v, p);
     return launch_status("doc_attn_fwd_kernel");
 }
 template <int D, bool CAP, bool BIAS>
@@ -1558,6 +1601,7 @@ extern "C" int brk_doc_attn_fwd(const void* q, const void* k, const void* v, int
     if (!out) return BRK_OUTPUT_ERROR;
     DocAttn p = da_params(q, k, v, ld_q, ld_kv, ld_out, spans, slopes, cap, batch, tokens, heads, kv_heads, head_dim);
     p.out = (__half*)out;
+    p.wide_out = (reinterpret_cast<uintptr_t>(out) & 31) == 0 && ld_out % 16 == 0;
     p.lse = lse;
     const uint64_t rows = (uint64_t)batch * tokens, qc = (uint64_t)heads * head_dim, kc = (uint64_t)kv_heads * head_dim;
     DocMaps t;

@@ -120,6 +120,11 @@ def test_forward_and_backward(batch, tokens, heads, kv, d, docs, prompts, bias, 
     again = o.doc_attn_backward(do.cuda(), *split(cq, heads, kv), out, lse, spans.cuda(), **args)
     for a, b in zip(again, (dq, dk, dv)):
         assert torch.equal(a, b)
+    # rows of out that start on 16-byte boundaries only
+    wide = heads * d + 8
+    out3 = torch.zeros(batch * tokens + 1, wide, dtype=torch.float16, device="cuda").as_strided((batch, tokens, heads, d), (tokens * wide, wide, d, 1), 8)
+    o.doc_attn(*split(cq, heads, kv), spans.cuda(), out=out3, **args)
+    assert torch.equal(out3, out)
     # a tensor of its own for each of q, k, v
     q2, k2, v2 = (x.contiguous() for x in split(cq, heads, kv))
     out2, lse2 = o.doc_attn(q2, k2, v2, spans.cuda(), **args)
