@@ -44,6 +44,7 @@ struct DocAttn {
     int batch, tokens, heads, kv_heads;
     float scale, scale_log2;                // 1/sqrt(d), times log2(e)
     float cap_log2, cap_in;                 // cap log2(e); 1 / (sqrt(d) cap)
+    float cap_poly[5];                      // coefficients of the capped score, see da_capped_near
     // forward
     bool wide_out;                          // rows of out start on 32-byte boundaries
     __half* out;
@@ -63,19 +64,30 @@ struct DocAttn {
 // of which the softmax already needs one per score: at 16 a clock and SM that unit, not the tensor core, would set the
 // pace.  Both are within 1e-6 of tanh, 5e-5 of the exponent at a cap of 50; the hardware tanh's 2^-11 would be 0.02 of it.
 constexpr float TANH_REACH = 0.75f;
+constexpr float TANH_1 = 0.99999723f, TANH_3 = -0.33323076f, TANH_5 = 0.13226089f, TANH_7 = -0.04928038f, TANH_9 = 0.01231877f;
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 da_tanh_near(float2 u) {
     const float2 s = __fmul2_rn(u, u);
-    float2 t = __ffma2_rn(both(0.01231877f), s, both(-0.04928038f));
-    t = __ffma2_rn(t, s, both(0.13226089f));
-    t = __ffma2_rn(t, s, both(-0.33323076f));
-    t = __ffma2_rn(t, s, both(0.99999723f));
+    float2 t = __ffma2_rn(both(TANH_9), s, both(TANH_7));
+    t = __ffma2_rn(t, s, both(TANH_5));
+    t = __ffma2_rn(t, s, both(TANH_3));
+    t = __ffma2_rn(t, s, both(TANH_1));
     return __fmul2_rn(t, u);
 }
 __device__ __forceinline__ float da_tanh(float u) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + fast_exp2(2.0f * LOG2E * u)));
     return fmaf(-2.0f, r, 1.0f);
+}
+// cap * tanh(raw * scale / cap) in log2 units plus `off`, by the polynomial, whose coefficients hold the cap
+__device__ __forceinline__ float2 da_capped_near(float2 raw, const DocAttn& p, float2 off) {
+    const float2 u = __fmul2_rn(raw, both(p.cap_in)), s = __fmul2_rn(u, u);
+    float2 t = __ffma2_rn(both(p.cap_poly[4]), s, both(p.cap_poly[3]));
+    t = __ffma2_rn(t, s, both(p.cap_poly[2]));
+    t = __ffma2_rn(t, s, both(p.cap_poly[1]));
+    t = __ffma2_rn(t, s, both(p.cap_poly[0]));
+    return __ffma2_rn(t, u, off);
 }
 // tanh of raw * scale / cap; `near`: all of the warp's arguments are within reach of the polynomial
 __device__ __forceinline__ float2 da_capped(float2 raw, const DocAttn& p, bool near) {
@@ -92,7 +104,6 @@ __device__ __forceinline__ float da_score(float raw, const DocAttn& p, float& sl
     slope_of_tanh = fmaf(-t, t, 1.0f);
     return t * p.cap_log2;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 __device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
 // bits [from, to) of 32, whatever lies outside of them
 __device__ __forceinline__ uint32_t span_bits(int from, int to) {
@@ -129,42 +140,77 @@ __device__ __forceinline__ Range da_blocks(const DocAttn& p, int b, int t0, int 
 }
 
 // The CTAs are persistent and walk items (tile, head): tiles in the order of falling work, dealt in rounds of alternating
-// direction, which evens out the totals without a counter in memory.  Every CTA sorts for itself (it needs two loads per
-// tile); the table lives in shared memory.
-struct DaTable {
-    uint16_t order[DA_SORT];
-    ushort4 blocks[DA_SORT];                // per tile: first and last block it needs, of its first and second half
+// direction, which evens out the totals without a counter in memory.  Every CTA sorts for itself (two loads per tile) and
+// lists its items in shared memory before the walk begins: the divisions and loads behind an item cost 2000 clocks where
+// a role does them between two items.  Only the items behind the list's end are worked out on the way.
+constexpr int DA_LIST = 96;
+struct DaItem {
+    int b, t0, head, pad;
+    Range r0, r1;                           // blocks that the tile's first and second half need
 };
-__device__ __forceinline__ bool da_item(int round, int n_tiles, int n_heads, const DaTable* table, bool sorted, int& tile, int& head) {
-    const int64_t G = gridDim.x, c = blockIdx.x;
-    const int64_t idx = round * G + ((round & 1) ? G - 1 - c : c);
-    if (idx >= (int64_t)n_tiles * n_heads) return false;
-    const int place = (int)(idx / n_heads);
-    tile = sorted ? table->order[place] : n_tiles - 1 - place;
-    head = (int)(idx % n_heads);
+struct DaTable {
+    DaItem items[DA_LIST];
+    ushort4 blocks[DA_SORT];                // per tile: r0, r1
+    uint16_t order[DA_SORT];
+};
+template <typename R>
+__device__ __forceinline__ bool da_find_item(int round, int n_tiles, int n_heads, int per_row, int tile_tokens, const DaTable* table, R ranges, DaItem& m) {
+    const uint32_t G = gridDim.x, c = blockIdx.x;
+    const uint64_t idx = (uint64_t)round * G + ((round & 1) ? G - 1 - c : c);
+    if (idx >= (uint64_t)n_tiles * n_heads) return false;
+    const int place = (int)(idx / (uint32_t)n_heads);
+    m.head = (int)(idx - (uint64_t)place * n_heads);
+    const bool sorted = n_tiles <= DA_SORT;
+    const int tile = sorted ? table->order[place] : n_tiles - 1 - place;
+    m.b = tile / per_row;
+    m.t0 = (tile - m.b * per_row) * tile_tokens;
+    if (sorted) {
+        const ushort4 t = table->blocks[tile];
+        m.r0 = {t.x, t.y};
+        m.r1 = {t.z, t.w};
+    } else {
+        m.r0 = ranges(m.b, m.t0, false);
+        m.r1 = ranges(m.b, m.t0, true);
+    }
     return true;
 }
-// ranges(tile, second half) for all tiles, then the rank of each by the blocks it needs: heavier first, ties by number.  All threads of the CTA.
+// Sorts the tiles (heavier first, ties by number) and lists this CTA's items; returns how many are listed (at most DA_LIST,
+// the walk goes on with da_find_item).  All threads of the CTA; ranges(b, t0, second half).
 template <typename R>
-__device__ __forceinline__ void da_sort(DaTable* table, int n_tiles, R ranges) {
-    for (int i = threadIdx.x; i < n_tiles; i += blockDim.x) {
-        const Range a = ranges(i, false), c = ranges(i, true);
-        table->blocks[i] = make_ushort4(a.begin, a.end, c.begin, c.end);
-    }
-    __syncthreads();
-    auto weight = [&](int i) {
-        const ushort4 t = table->blocks[i];
-        return t.y - t.x + t.w - t.z;
-    };
-    for (int i = threadIdx.x; i < n_tiles; i += blockDim.x) {
-        const int w = weight(i);
-        int rank = 0;
-        for (int j = 0; j < n_tiles; j++) {
-            const int v = weight(j);
-            rank += v > w || (v == w && j < i);
+__device__ __forceinline__ int da_plan_items(DaTable* table, int n_tiles, int n_heads, int per_row, int tile_tokens, R ranges) {
+    if (n_tiles <= DA_SORT) {
+        for (int i = threadIdx.x; i < n_tiles; i += blockDim.x) {
+            const int b = i / per_row, t0 = (i - b * per_row) * tile_tokens;
+            const Range x = ranges(b, t0, false), y = ranges(b, t0, true);
+            table->blocks[i] = make_ushort4(x.begin, x.end, y.begin, y.end);
         }
-        table->order[rank] = (uint16_t)i;
+        __syncthreads();
+        auto weight = [&](int i) {
+            const ushort4 t = table->blocks[i];
+            return t.y - t.x + t.w - t.z;
+        };
+        for (int i = threadIdx.x; i < n_tiles; i += blockDim.x) {
+            const int w = weight(i);
+            int rank = 0;
+            for (int j = 0; j < n_tiles; j++) {
+                const int v = weight(j);
+                rank += v > w || (v == w && j < i);
+            }
+            table->order[rank] = (uint16_t)i;
+        }
+        __syncthreads();
     }
+    const uint64_t items = (uint64_t)n_tiles * n_heads;
+    const uint64_t full = items / gridDim.x, rest = items - full * gridDim.x;
+    // rounds this CTA has an item in: all full ones, and the last one if it is dealt that far
+    const uint64_t mine = full + ((full & 1) ? (blockIdx.x >= gridDim.x - rest) : (blockIdx.x < rest));
+    const int listed = (int)(mine < (uint64_t)DA_LIST ? mine : (uint64_t)DA_LIST);
+    for (int i = threadIdx.x; i < listed; i += blockDim.x) {
+        DaItem m = {};
+        da_find_item(i, n_tiles, n_heads, per_row, tile_tokens, table, ranges, m);
+        table->items[i] = m;
+    }
+    return listed;
 }
 
 // ---- rows evaluated again without the tensor core (see the top) ------------------------------------------------------------
@@ -327,6 +373,11 @@ __device__ __noinline__ void da_mend_dkv(const DocAttn& p, int b, int kh, int j,
     }
 }
 
+// one arrival for the whole warp
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 __device__ __forceinline__ void da_zero_row(__half* row, int d) {
     for (int e = 0; e < d; e += 8) *reinterpret_cast<uint4*>(row + e) = make_uint4(0, 0, 0, 0);
 }
@@ -367,10 +418,10 @@ template <int D>
 struct FwdSmem {
     static constexpr uint32_t TILE = 128 * D * 2;
     static constexpr int STAGES = 2;                    // of K and of V each
-    static constexpr size_t BYTES = 1024 + TILE * (2 + 2 * STAGES) + sizeof(DaTable) + 256 + 2 * 2 * 2 * 128 * sizeof(float);
+    static constexpr size_t BYTES = 1024 + TILE * (2 + 2 * STAGES) + sizeof(DaTable) + 256 + 2 * 4 * 2 * 128 * sizeof(float);
 };
 
-constexpr int DA_FWD_THREADS = 64 + 512;
+constexpr int DA_FWD_THREADS = 64 + 512;        // producer warp, MMA warp, sixteen row-owner warps
 
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(DA_FWD_THREADS, 1)
@@ -400,11 +451,10 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     uint64_t* o_done = bars + 16;            // 2: a P V product of the tile is complete
     uint64_t* o_empty = bars + 18;           // 2: the tile's output has been read
     uint32_t* tmem_base_smem = reinterpret_cast<uint32_t*>(bars + 20);
-    float* exchange = reinterpret_cast<float*>(bars + 32);       // [tile][turn][owner][row]: the two owners' maxima
+    float* exchange = reinterpret_cast<float*>(bars + 32);       // [tile][maxima of even, of odd blocks, sums, flags][owner][row]
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int per_row = (p.tokens + 255) / 256, n_pairs = p.batch * per_row;
-    const bool sorted = n_pairs <= DA_SORT;
+    const int per_row = (p.tokens + 255) / 256, n_tiles = p.batch * per_row;
 
     if (threadIdx.x == 0) {
         for (int t = 0; t < 2; t++) {
@@ -415,9 +465,9 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             mbar_init(&v_full[t], 1);
             mbar_init(&v_empty[t], 1);
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[t], 256);
+            mbar_init(&p_full[t], 8);
             mbar_init(&o_done[t], 1);
-            mbar_init(&o_empty[t], 256);
+            mbar_init(&o_empty[t], 8);
         }
         fence_barrier_init();
         prefetch_tensormap(&tmap_q);
@@ -428,32 +478,20 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         tmem_alloc(tmem_base_smem, TMEM_COLS);
         tmem_relinquish();
     }
-    if (sorted)
-        da_sort(table, n_pairs, [&](int i, bool second) { return da_blocks<true>(p, i / per_row, (i % per_row) * 256 + (second ? 128 : 0), 128); });
+    auto ranges = [&](int b, int t0, bool second) { return da_blocks<true>(p, b, second ? t0 + 128 : t0, 128); };
+    const int listed = da_plan_items(table, n_tiles, p.heads, per_row, 256, ranges);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem_base = uniform(*tmem_base_smem);
     const int group = p.heads / p.kv_heads;
 
-    struct Item {
-        int b, t0, head;
-        Range r0, r1;        // key blocks of the two tiles
-        int last, n;         // the n blocks up to `last` that either needs, walked from the last one down
+    struct Item : DaItem {
+        int last, n;         // the n blocks up to `last` that either tile needs, walked from the last one down
     };
     auto item_of = [&](int round, Item& m) {
-        int pair;
-        if (!da_item(round, n_pairs, p.heads, table, sorted, pair, m.head)) return false;
-        m.b = pair / per_row;
-        m.t0 = (pair % per_row) * 256;
-        if (sorted) {
-            const ushort4 t = table->blocks[pair];
-            m.r0 = {t.x, t.y};
-            m.r1 = {t.z, t.w};
-        } else {
-            m.r0 = da_blocks<true>(p, m.b, m.t0, 128);
-            m.r1 = da_blocks<true>(p, m.b, m.t0 + 128, 128);
-        }
+        if (round < listed) static_cast<DaItem&>(m) = table->items[round];
+        else if (listed < DA_LIST || !da_find_item(round, n_tiles, p.heads, per_row, 256, table, ranges, m)) return false;
         const bool has0 = m.r0.end > m.r0.begin, has1 = m.r1.end > m.r1.begin;
         m.last = max(m.r0.end, m.r1.end) - 1;
         m.n = m.last + 1 - (has0 ? (has1 ? min(m.r0.begin, m.r1.begin) : m.r0.begin) : m.r1.begin);
@@ -564,12 +602,12 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         const int r = quarter * 32 + lane;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
         const uint32_t tm_s = tm + t * 128 + half * 64, tm_o = tm + 256 + t * D + half * (D / 2);
-        float* const cells = exchange + t * 512 + r;
+        float* const cells = exchange + t * 1024 + r;
         // The owners of 32 rows meet once a block.  Every owner reaches it in every block, also one whose bounded wait gave up.
         auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quarter) : "memory"); };
         bool ok = true;
         uint32_t it = 0;
-        Item m;
+        Item m = {};
         auto span_of = [&]() {
             const int qi = m.t0 + t * 128 + r;
             // rows behind the sequence never force the masked path
@@ -616,36 +654,43 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 part = __reduce_or_sync(0xffffffffu, part);
                 whole = __reduce_and_sync(0xffffffffu, whole);
                 const float dist = (float)(kbase - qi), slant = slope2 * dist;
-                // chunk c of the scores: in log2 units with a cap or a bias, else as they are; what is masked -inf
-                auto scores = [&](int c, float2(&x)[16], auto capped) {
-                    if (CAP && capped) {
+                bool near = true;                       // the polynomial reaches every argument of the cap's tanh in this warp's part of the block
+                // Chunk c of the scores plus `shift`, in log2 units; what is masked is -inf.  RAW: as the products are, which is enough for
+                // the maximum where there is no bias (the scale and the cap keep the order).
+                auto scores = [&](int c, float2(&x)[16], float shift, auto raw) {
+                    constexpr bool RAW = decltype(raw)::value;
+                    tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<float*>(x));
+                    tmem_ld_wait();
+                    if (CAP && (RAW || BIAS)) {
                         float wide = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 16; i++) wide = max3(wide, fabsf(x[i].x), fabsf(x[i].y));
-                        if (__all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH)) {
+                        near = __all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH) && near;
+                    }
+                    auto fill = [&](auto line) {        // line: the bias as a straight line in the key's number
+                        constexpr bool LINE = BIAS && decltype(line)::value;
+                        const float2 at = both(LINE ? fmaf(slope2, (float)(c * 32), slant) + shift : shift);
+                        auto off = [&](int i) { return LINE ? __ffma2_rn(both(slope2), pair_of(i), at) : at; };
+                        if (CAP && near) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = __fmul2_rn(da_capped(x[i], p, true), both(p.cap_log2));
+                            for (int i = 0; i < 16; i++) x[i] = da_capped_near(x[i], p, off(i));
+                        } else if (CAP) {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) x[i] = __ffma2_rn(da_capped(x[i], p, false), both(p.cap_log2), off(i));
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = __fmul2_rn(da_capped(x[i], p, false), both(p.cap_log2));
+                            for (int i = 0; i < 16; i++) x[i] = __ffma2_rn(x[i], both(p.scale_log2), off(i));
                         }
-                    }
+                    };
                     if (whole >> c & 1) {
-                        if (BIAS) {
-                            const float2 at = both(fmaf(slope2, (float)(c * 32), slant));
-#pragma unroll
-                            for (int i = 0; i < 16; i++) {
-                                const float2 bias = __ffma2_rn(both(slope2), pair_of(i), at);
-                                x[i] = CAP ? __fadd2_rn(x[i], bias) : __ffma2_rn(x[i], both(p.scale_log2), bias);
-                            }
-                        }
+                        if (!RAW) fill(Flag<true>());
                     } else {
+                        if (!RAW) fill(Flag<false>());
                         const float d0 = dist + (float)(c * 32);
                         const uint32_t seen = span_bits(lo - kbase - c * 32, hi - kbase - c * 32);
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            if (BIAS) {
-                                if (!CAP) x[i] = __fmul2_rn(x[i], both(p.scale_log2));
+                            if (BIAS && !RAW) {
                                 x[i].x = fmaf(-slope2, fabsf(d0 + (float)(2 * i)), x[i].x);
                                 x[i].y = fmaf(-slope2, fabsf(d0 + (float)(2 * i + 1)), x[i].y);
                             }
@@ -661,9 +706,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     for (int c = 0; c < 2; c++) {
                         if (!(part >> c & 1)) continue;
                         float2 x[16];
-                        tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<float*>(x));
-                        tmem_ld_wait();
-                        scores(c, x, Flag<CAP && BIAS>());            // the cap alone keeps the order: applied to the maximum below
+                        scores(c, x, 0.0f, Flag<!BIAS>());
                         float t4[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int i = 0; i < 16; i++) t4[i & 3] = max3(t4[i & 3], x[i].x, x[i].y);
@@ -699,19 +742,16 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         tmem_st_32x32b_x32(tm_o + c, v);
                     }
                 }
-                const float2 ref = both(m_ref == -INFINITY ? 0.0f : -m_ref);        // nothing visible yet: every exponential is 0
+                const float shift = m_ref == -INFINITY ? 0.0f : -m_ref;        // nothing visible yet: every exponential is 0
 #pragma unroll 1
                 for (int c = 0; c < 2; c++) {
                     uint32_t w[16];
                     if (part >> c & 1) {
                         float2 x[16];
-                        tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<float*>(x));
-                        tmem_ld_wait();
-                        scores(c, x, Flag<true>());
+                        scores(c, x, shift, Flag<false>());
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const float2 e = CAP || BIAS ? __fadd2_rn(x[i], ref) : __ffma2_rn(x[i], both(p.scale_log2), ref);
-                            const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                            const float2 pe = make_float2(fast_exp2(x[i].x), fast_exp2(x[i].y));
                             l = __fadd2_rn(l, pe);
                             w[i] = da_half2(pe.x, pe.y);
                         }
@@ -723,23 +763,22 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 }
                 tmem_st_wait();
                 tcgen05_fence_before();
-                mbar_arrive(&p_full[t]);
+                warp_arrive(&p_full[t]);
             }
             // epilogue: O / l -> fp16, token-major; log-sum-exp for the backward
-            float* const cell = cells + (it & 1) * 256;
-            cell[half * 128] = l.x + l.y;
+            float* const sums = cells + 512;
+            sums[half * 128] = l.x + l.y;
             meet();
-            const float sum = cell[0] + cell[128];
-            meet();                                     // the next item's first block uses the same cells
+            const float sum = sums[0] + sums[128];
             if (ok) ok = mbar_wait(&o_done[t], (it - 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);        // a NaN stays one
             const float lse2 = m_ref + __log2f(sum);
             const bool none = lo >= hi;
-            float bad = 0.0f;
+            __half2 bad[2] = {__float2half2_rn(0.0f), __float2half2_rn(0.0f)};
             if (ok) {
                 tcgen05_fence_after();
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < D / 2; c += 32) {
                     float2 x[16];
                     tmem_ld_32x32b_x32(tm_o + c, reinterpret_cast<float*>(x));
@@ -747,21 +786,24 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        bad = fmaf(x[i].x, 0.0f, fmaf(x[i].y, 0.0f, bad));
-                        w[i] = none ? 0 : da_half2(x[i].x * inv, x[i].y * inv);
+                        const float2 y = __fmul2_rn(x[i], both(inv));
+                        w[i] = da_half2(y.x, y.y);
+                        bad[i & 1] = __hfma2(*reinterpret_cast<const __half2*>(&w[i]), __float2half2_rn(0.0f), bad[i & 1]);      // a NaN, once something is not finite
+                        if (none) w[i] = 0;
                     }
                     if (live) da_store64(o + c, w, p.wide_out);
                 }
                 tcgen05_fence_before();
-                mbar_arrive(&o_empty[t]);
+                warp_arrive(&o_empty[t]);
                 if (live && lse) *lse = none ? 0.0f : lse2 * LN2;
             }
-            const bool again = live && bad != 0.0f && !none && fabsf(lse2) < INFINITY;
-            cell[half * 128] = again ? 1.0f : 0.0f;
-            meet();                                     // orders both owners' stores before the row is written again
-            const bool redo = cell[0] + cell[128] != 0.0f;
+            const __half2 any = __hadd2(bad[0], bad[1]);
+            const bool again = live && !none && fabsf(lse2) < INFINITY && (__hisnan(__low2half(any)) || __hisnan(__high2half(any)));
+            float* const flags = cells + 768;
+            flags[half * 128] = again ? 1.0f : 0.0f;
+            meet();                                     // orders both owners' stores before a row is written again
+            const bool redo = flags[0] + flags[128] != 0.0f;
             if (half == 0 && __any_sync(0xffffffffu, redo)) da_mend_out<D, CAP>(p, b, head, qi, lo, hi, lse2, redo);
-            meet();
         }
         if (!ok && lane == 0) atomicExch(&g_doc_error, 3);
     }
@@ -852,7 +894,6 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int per_row = (p.tokens + 127) / 128, n_tiles = p.batch * per_row;
     const int group = p.heads / p.kv_heads;
-    const bool sorted = n_tiles <= DA_SORT;
 
     if (threadIdx.x == 0) {
         mbar_init(kv_full, 1);
@@ -863,36 +904,30 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 256);
+            mbar_init(&p_full[i], 8);
         }
         mbar_init(acc_full, 1);
-        mbar_init(acc_empty, 256);
+        mbar_init(acc_empty, 8);
         fence_barrier_init();
     }
     if (warp == 1) {
         tmem_alloc(tmem_base_smem, TMEM_COLS);
         tmem_relinquish();
     }
-    if (sorted)
-        da_sort(table, n_tiles, [&](int i, bool second) { return second ? Range{0, 0} : da_blocks<false>(p, i / per_row, (i % per_row) * 128, DA_SUB); });
+    auto ranges = [&](int b, int t0, bool second) { return second ? Range{0, 0} : da_blocks<false>(p, b, t0, DA_SUB); };
+    const int listed = da_plan_items(table, n_tiles, p.kv_heads, per_row, 128, ranges);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem_base = uniform(*tmem_base_smem);
 
-    struct Item {
-        int b, t0, head;       // head: of the keys
-        Range r;               // 64-query blocks
-        int n;                 // steps: blocks times query heads of the group
+    struct Item : DaItem {
+        int n;                 // steps: 64-query blocks r0, times query heads of the group
     };
     auto item_of = [&](int round, Item& m) {
-        int tile;
-        if (!da_item(round, n_tiles, p.kv_heads, table, sorted, tile, m.head)) return false;
-        m.b = tile / per_row;
-        m.t0 = (tile % per_row) * 128;
-        if (sorted) m.r = {table->blocks[tile].x, table->blocks[tile].y};
-        else m.r = da_blocks<false>(p, m.b, m.t0, DA_SUB);
-        m.n = (m.r.end - m.r.begin) * group;
+        if (round < listed) static_cast<DaItem&>(m) = table->items[round];
+        else if (listed < DA_LIST || !da_find_item(round, n_tiles, p.kv_heads, per_row, 128, table, ranges, m)) return false;
+        m.n = (m.r0.end - m.r0.begin) * group;
         return true;
     };
 
@@ -913,7 +948,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     tma_load_2d(sK + a * 16384, &tmap_k, kv_full, kcol + a * 64, row + m.t0);
                     tma_load_2d(sV + a * 16384, &tmap_v, kv_full, kcol + a * 64, row + m.t0);
                 }
-                int blk = m.r.begin, col = m.head * group * D;
+                int blk = m.r0.begin, col = m.head * group * D;
                 for (int n = 0; n < m.n && ok; n++, it++) {
                     const int s = it % S::STAGES;
                     ok = mbar_wait(&q_empty[s], ((it / S::STAGES) & 1) ^ 1);
@@ -924,8 +959,8 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         tma_load_2d(sQ + s * S::SUB + a * DA_SUB_ATOM, &tmap_q, &q_full[s], col + a * 64, row + blk * DA_SUB);
                         tma_load_2d(sDO + s * S::SUB + a * DA_SUB_ATOM, &tmap_do, &q_full[s], col + a * 64, row + blk * DA_SUB);
                     }
-                    if (++blk == m.r.end) {
-                        blk = m.r.begin;
+                    if (++blk == m.r0.end) {
+                        blk = m.r0.begin;
                         col += D;
                     }
                 }
@@ -1022,7 +1057,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             const int qlo = max(span.z, 0), qhi = live ? min(span.w, p.tokens) : span.w;
             // a step's 64 log-sum-exps (log2 units, with the query's share of the bias) and 64 deltas, all negated: one for each of
             // the first owners, fetched a step ahead so that the load's latency passes behind the step before it
-            int blk = m.r.begin, h = m.head * group;
+            int blk = m.r0.begin, h = m.head * group;
             auto fetch = [&]() {
                 const int c = r & 63, i = blk * DA_SUB + c;
                 if (half == 1 || i >= p.tokens) return 0.0f;
@@ -1037,8 +1072,8 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 const int sb = i & 1, q0 = blk * DA_SUB;
                 const float slope2 = BIAS ? p.slopes[h] * LOG2E : 0.0f;
                 if (half == 0) stat[sb * 128 + r] = mine;
-                if (++blk == m.r.end) {
-                    blk = m.r.begin;
+                if (++blk == m.r0.end) {
+                    blk = m.r0.begin;
                     h++;
                 }
                 if (n + 1 < m.n) mine = fetch();
@@ -1112,7 +1147,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 tmem_st_32x32b_x16(tm + 128 + sb * DA_SUB + c0, wd);
                 tmem_st_wait();
                 tcgen05_fence_before();
-                mbar_arrive(&p_full[sb]);
+                warp_arrive(&p_full[sb]);
             }
             it0 += m.n;
             if (ok) ok = mbar_wait(acc_full, items & 1);
@@ -1145,7 +1180,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     }
                 }
                 tcgen05_fence_before();
-                mbar_arrive(acc_empty);            // the accumulators may take the next item's first products
+                warp_arrive(acc_empty);            // the accumulators may take the next item's first products
             }
             // evaluated again by the warps of the rows' first owners, after both owners' stores (the barrier orders them)
             stat[half * 128 + r] = bad;
@@ -1208,7 +1243,6 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int per_row = (p.tokens + 127) / 128, n_tiles = p.batch * per_row;
     const int group = p.heads / p.kv_heads;
-    const bool sorted = n_tiles <= DA_SORT;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -1219,38 +1253,32 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&ds_full[i], 256);
+            mbar_init(&ds_full[i], 8);
         }
         mbar_init(dp_full, 1);
-        mbar_init(dp_empty, 256);
+        mbar_init(dp_empty, 8);
         mbar_init(acc_full, 1);
-        mbar_init(acc_empty, 256);
+        mbar_init(acc_empty, 8);
         fence_barrier_init();
     }
     if (warp == 1) {
         tmem_alloc(tmem_base_smem, TMEM_COLS);
         tmem_relinquish();
     }
-    if (sorted)
-        da_sort(table, n_tiles, [&](int i, bool second) { return second ? Range{0, 0} : da_blocks<true>(p, i / per_row, (i % per_row) * 128, 128); });
+    auto ranges = [&](int b, int t0, bool second) { return second ? Range{0, 0} : da_blocks<true>(p, b, t0, 128); };
+    const int listed = da_plan_items(table, n_tiles, p.heads, per_row, 128, ranges);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem_base = uniform(*tmem_base_smem);
 
-    struct Item {
-        int b, t0, head;
-        Range r;
+    struct Item : DaItem {
         int n;
     };
     auto item_of = [&](int round, Item& m) {
-        int tile;
-        if (!da_item(round, n_tiles, p.heads, table, sorted, tile, m.head)) return false;
-        m.b = tile / per_row;
-        m.t0 = (tile % per_row) * 128;
-        if (sorted) m.r = {table->blocks[tile].x, table->blocks[tile].y};
-        else m.r = da_blocks<true>(p, m.b, m.t0, 128);
-        m.n = m.r.end - m.r.begin;
+        if (round < listed) static_cast<DaItem&>(m) = table->items[round];
+        else if (listed < DA_LIST || !da_find_item(round, n_tiles, p.heads, per_row, 128, table, ranges, m)) return false;
+        m.n = m.r0.end - m.r0.begin;
         return true;
     };
 
@@ -1272,7 +1300,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                     tma_load_2d(sDO + a * 16384, &tmap_do, q_full, col + a * 64, row + m.t0);
                 }
                 for (int n = 0; n < m.n && ok; n++, it++) {
-                    const int s = it % S::STAGES, y = row + (m.r.begin + n) * 128;
+                    const int s = it % S::STAGES, y = row + (m.r0.begin + n) * 128;
                     const uint32_t par = ((it / S::STAGES) & 1) ^ 1;
                     ok = mbar_wait(&k_empty[s], par);
                     if (!ok) break;
@@ -1383,7 +1411,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const bool ahead = BIAS && __any_sync(0xffffffffu, live && hi > qi + 1);
             for (int n = 0; n < m.n && ok; n++) {
                 const uint32_t i = it0 + n;
-                const int sb = i & 1, kbase = (m.r.begin + n) * 128 + c0;
+                const int sb = i & 1, kbase = (m.r0.begin + n) * 128 + c0;
                 ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sb], (i >> 1) & 1) && mbar_wait(dp_full, i & 1));
                 if (!ok) break;
                 tcgen05_fence_after();
@@ -1401,7 +1429,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                     tmem_ld_wait();
                     if (c == 1) {
                         tcgen05_fence_before();
-                        mbar_arrive(dp_empty);
+                        warp_arrive(dp_empty);
                     }
                     bool near = true;
                     if (CAP) {
@@ -1447,7 +1475,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 tmem_st_32x32b_x16(tm + sb * 128 + c0 + 16, w[1]);
                 tmem_st_wait();
                 tcgen05_fence_before();
-                mbar_arrive(&ds_full[sb]);
+                warp_arrive(&ds_full[sb]);
             }
             it0 += m.n;
             if (ok) ok = mbar_wait(acc_full, items & 1);
@@ -1477,7 +1505,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                     }
                 }
                 tcgen05_fence_before();
-                mbar_arrive(acc_empty);
+                warp_arrive(acc_empty);
             }
             // evaluated again by the warps of the rows' first owners, after both owners' stores (the barrier orders them)
             again[half * 128 + r] = bad;
@@ -1584,6 +1612,8 @@ static DocAttn da_params(const void* q, const void* k, const void* v, int64_t ld
     p.scale_log2 = (float)(scale * log2e);
     p.cap_log2 = (float)(cap * log2e);
     p.cap_in = cap > 0.0f ? (float)(scale / cap) : 0.0f;
+    const double tanh_poly[5] = {TANH_1, TANH_3, TANH_5, TANH_7, TANH_9};
+    for (int i = 0; i < 5; i++) p.cap_poly[i] = (float)(tanh_poly[i] * cap * log2e);
     return p;
 }
 
