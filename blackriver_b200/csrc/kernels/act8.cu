@@ -42,56 +42,74 @@ __device__ __forceinline__ A8Scale a8_scale(uint32_t top_bits) {
         s.scale = 0.0f;
     } else {
         s.inv = __fdiv_rn(127.0f, top);
-        s.scale = __fdiv_rn(top, 127.0f);
+        s.scale = top * (1.0f / 127.0f);
     }
     return s;
 }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 // Four values to four bytes.  Adding 1.5 * 2^23 leaves the nearest integer (ties to even) in the low mantissa bits, and
-// a byte permute gathers them: no conversion instruction, which would run at an eighth of the rate.  With inv == 0 the
-// product is 0, or NaN for a value that is not finite; its low byte is whatever it is, the block's scale is NaN then.
-// The product is rounded before the sum, not fused with it: a value in the middle between two steps (half of the block's
-// largest, say) then stays there, and ties go to even as they do in exact arithmetic.
-__device__ __forceinline__ uint32_t a8_round(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f)); }
-__device__ __forceinline__ uint32_t a8_pack4(float a, float b, float c, float d, float inv) {
-    const uint32_t ia = a8_round(a, inv), ib = a8_round(b, inv), ic = a8_round(c, inv), id = a8_round(d, inv);
-    return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+// a byte permute gathers them: no conversion instruction, which would run at an eighth of the rate.  The product is rounded
+// before the sum, not fused with it: a value in the middle between two steps (half of the block's largest, say) then stays
+// there, and ties go to even as they do in exact arithmetic.  With inv == 0 the product is 0, or NaN for a value that is
+// not finite; its low byte is whatever it is, the block's scale is NaN then.
+__device__ __forceinline__ uint32_t a8_pack4(float2 a, float2 b, float inv) {
+    const float2 x = __fadd2_rn(__fmul2_rn(a, both(inv)), both(12582912.0f)), y = __fadd2_rn(__fmul2_rn(b, both(inv)), both(12582912.0f));
+    return __byte_perm(__byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040), __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040), 0x5410);
 }
-// Byte b of a word as the number it stands for: 2^23 + (b + 128) assembled from its bits, exactly.
+__device__ __forceinline__ int8_t a8_pack1(float x, float inv) { return (int8_t)(__float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f)) & 0xff); }
+__device__ __forceinline__ uint4 a8_pack16(const float2 (&v)[8], float inv) {
+    return make_uint4(a8_pack4(v[0], v[1], inv), a8_pack4(v[2], v[3], inv), a8_pack4(v[4], v[5], inv), a8_pack4(v[6], v[7], inv));
+}
+// Two bytes of a word as the numbers they stand for: 2^23 + (b + 128) assembled from its bits, exactly.
 template <int B>
-__device__ __forceinline__ float a8_byte(uint32_t flipped) {
-    return __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7440 + B)) - 8388736.0f;
+__device__ __forceinline__ float2 a8_bytes(uint32_t flipped) {
+    const float2 f = make_float2(__uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7440 + B)), __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7441 + B)));
+    return __fadd2_rn(f, both(-8388736.0f));
 }
-__device__ __forceinline__ void a8_unpack4(uint32_t w, float scale, float* o) {
-    w ^= 0x80808080u;
-    o[0] = a8_byte<0>(w) * scale;
-    o[1] = a8_byte<1>(w) * scale;
-    o[2] = a8_byte<2>(w) * scale;
-    o[3] = a8_byte<3>(w) * scale;
-}
-
-// ---- N consecutive elements of storage type T ------------------------------------------------------------------------
-template <typename T, int N>
-__device__ __forceinline__ void load_n(const T* p, float* o) {
-    constexpr int VN = Vec<T>::N;
-    uint4 raw[N / VN];
+__device__ __forceinline__ void a8_unpack16(const uint4& w, float scale, float2 (&o)[8]) {
+    const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
 #pragma unroll
-    for (int i = 0; i < N / VN; i++) raw[i] = ld_raw_stream(p + i * VN);
-#pragma unroll
-    for (int i = 0; i < N / VN; i++) {
-        Vec<T> v;
-        v.unpack(raw[i]);
-#pragma unroll
-        for (int e = 0; e < VN; e++) o[i * VN + e] = v.v[e];
+    for (int i = 0; i < 4; i++) {
+        o[2 * i] = __fmul2_rn(a8_bytes<0>(x[i]), both(scale));
+        o[2 * i + 1] = __fmul2_rn(a8_bytes<2>(x[i]), both(scale));
     }
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_n(T* p, const float* x) {
+
+// ---- 16 consecutive columns of storage type T, packed until used ------------------------------------------------------
+template <typename T>
+struct Pack16 {
+    static constexpr int VN = Vec<T>::N, N = 16 / VN;
+    uint4 v[N];
+    __device__ __forceinline__ void stream(const T* p) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = ld_raw_stream(p + i * VN);
+    }
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = ld_raw(p + i * VN);
+    }
+    __device__ __forceinline__ void to(float2 (&o)[8]) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            Vec<T> x;
+            x.unpack(v[i]);
+#pragma unroll
+            for (int e = 0; e < VN; e += 2) o[(i * VN + e) / 2] = make_float2(x.v[e], x.v[e + 1]);
+        }
+    }
+};
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const float2 (&x)[8]) {
     constexpr int VN = Vec<T>::N;
 #pragma unroll
-    for (int i = 0; i < N / VN; i++) {
+    for (int i = 0; i < 16 / VN; i++) {
         Vec<T> v;
 #pragma unroll
-        for (int e = 0; e < VN; e++) v.v[e] = x[i * VN + e];
+        for (int e = 0; e < VN; e += 2) {
+            v.v[e] = x[(i * VN + e) / 2].x;
+            v.v[e + 1] = x[(i * VN + e) / 2].y;
+        }
         v.store_stream(p + i * VN);
     }
 }
@@ -112,42 +130,54 @@ __device__ __forceinline__ GeluTerms gelu_terms(float x) {
 
 // ---- pack, and GELU that keeps its input: a thread owns 16 columns, 8 neighbouring lanes a block ----------------------
 // units_per_row counts 16-column units with the last block filled up to 8 of them, so that a block never leaves its lanes.
+// Two units of a thread are in flight at once.
+constexpr int A8_UNITS = 2;
+struct A8Unit {
+    int64_t at;          // first element
+    bool live;
+};
+__device__ __forceinline__ A8Unit a8_unit(int64_t u, int64_t units, int units_per_row, int cols, bool whole) {
+    A8Unit r = {u * 16, u < units};
+    if (!whole) {
+        const int64_t row = u / units_per_row;
+        const int c = (int)(u - row * units_per_row) * 16;
+        r.live = r.live && c < cols;
+        r.at = row * cols + c;
+    }
+    return r;
+}
 template <typename T, bool GELU>
 __global__ void __launch_bounds__(A8_THREADS)
 a8_pack_kernel(const T* x, T* y, int8_t* __restrict__ q, float* __restrict__ scale, int64_t units, int units_per_row, int cols) {
     pdl_wait();
     const bool whole = (cols & (A8_BLOCK - 1)) == 0;
-    for (int64_t u = (int64_t)blockIdx.x * A8_THREADS + threadIdx.x; u - threadIdx.x % 32 < units; u += (int64_t)gridDim.x * A8_THREADS) {
-        int64_t at = u * 16;
-        bool live = u < units;
-        if (!whole) {
-            const int64_t row = u / units_per_row;
-            const int c = (int)(u - row * units_per_row) * 16;
-            live = live && c < cols;
-            at = row * cols + c;
-        }
-        float v[16];
-        uint32_t top = 0;
-        if (live) {
-            load_n<T, 16>(x + at, v);
+    const int64_t stride = (int64_t)gridDim.x * A8_THREADS;
+    for (int64_t u0 = (int64_t)blockIdx.x * A8_THREADS + threadIdx.x; u0 - threadIdx.x % 32 < units; u0 += A8_UNITS * stride) {
+        A8Unit unit[A8_UNITS];
+        Pack16<T> raw[A8_UNITS] = {};
 #pragma unroll
-            for (int e = 0; e < 16; e++) top = max(top, mag_bits(v[e]));
+        for (int i = 0; i < A8_UNITS; i++) {
+            unit[i] = a8_unit(u0 + i * stride, units, units_per_row, cols, whole);
+            if (unit[i].live) raw[i].stream(x + unit[i].at);
         }
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (live) {
-            const A8Scale s = a8_scale(top);
-            uint4 w;
-            w.x = a8_pack4(v[0], v[1], v[2], v[3], s.inv);
-            w.y = a8_pack4(v[4], v[5], v[6], v[7], s.inv);
-            w.z = a8_pack4(v[8], v[9], v[10], v[11], s.inv);
-            w.w = a8_pack4(v[12], v[13], v[14], v[15], s.inv);
-            __stcs(reinterpret_cast<uint4*>(q + at), w);
-            if ((threadIdx.x & 7) == 0) scale[u >> 3] = s.scale;
-            if (GELU) {
+        for (int i = 0; i < A8_UNITS; i++) {
+            float2 v[8];
+            raw[i].to(v);
+            uint32_t top = 0;
 #pragma unroll
-                for (int e = 0; e < 16; e++) v[e] = gelu_terms(v[e]).y;
-                store_n<T, 16>(y + at, v);
+            for (int e = 0; e < 8; e++) top = max(top, max(mag_bits(v[e].x), mag_bits(v[e].y)));
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (unit[i].live) {
+                const A8Scale s = a8_scale(top);
+                __stcs(reinterpret_cast<uint4*>(q + unit[i].at), a8_pack16(v, s.inv));
+                if ((threadIdx.x & 7) == 0) scale[(u0 + i * stride) >> 3] = s.scale;
+                if (GELU) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = make_float2(gelu_terms(v[e].x).y, gelu_terms(v[e].y).y);
+                    store16(y + unit[i].at, v);
+                }
             }
         }
     }
@@ -177,7 +207,7 @@ a8_pack_generic_kernel(const T* x, T* y, int8_t* q, float* scale, int64_t rows, 
         for (int i = 0; i < 4; i++) {
             const int c = i * 32 + lane;
             if (c0 + c < cols) {
-                q[at + c] = (int8_t)(a8_pack4(v[i], 0.0f, 0.0f, 0.0f, s.inv) & 0xff);
+                q[at + c] = a8_pack1(v[i], s.inv);
                 if (GELU) y[at + c] = from_f32<T>(gelu_terms(v[i]).y);
             }
         }
@@ -191,33 +221,40 @@ __global__ void __launch_bounds__(A8_THREADS)
 a8_unpack_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, const T* dy, T* out, T* y, int64_t units, int units_per_row, int cols) {
     pdl_wait();
     const bool whole = (cols & (A8_BLOCK - 1)) == 0;
-    for (int64_t u = (int64_t)blockIdx.x * A8_THREADS + threadIdx.x; u < units; u += (int64_t)gridDim.x * A8_THREADS) {
-        int64_t at = u * 16;
-        if (!whole) {
-            const int64_t row = u / units_per_row;
-            const int c = (int)(u - row * units_per_row) * 16;
-            if (c >= cols) continue;
-            at = row * cols + c;
-        }
-        const uint4 w = __ldcs(reinterpret_cast<const uint4*>(q + at));
-        const float s = scale[u >> 3];
-        float g[16], v[16];
-        if (DY) load_n<T, 16>(dy + at, g);
-        a8_unpack4(w.x, s, v);
-        a8_unpack4(w.y, s, v + 4);
-        a8_unpack4(w.z, s, v + 8);
-        a8_unpack4(w.w, s, v + 12);
-        if (DY) {
+    const int64_t stride = (int64_t)gridDim.x * A8_THREADS;
+    for (int64_t u0 = (int64_t)blockIdx.x * A8_THREADS + threadIdx.x; u0 < units; u0 += A8_UNITS * stride) {
+        A8Unit unit[A8_UNITS];
+        Pack16<T> g[A8_UNITS];
+        uint4 w[A8_UNITS];
+        float s[A8_UNITS];
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const GeluTerms t = gelu_terms(v[e]);
-                g[e] *= t.dy;
-                v[e] = t.y;
+        for (int i = 0; i < A8_UNITS; i++) {
+            unit[i] = a8_unit(u0 + i * stride, units, units_per_row, cols, whole);
+            if (unit[i].live) {
+                w[i] = __ldcs(reinterpret_cast<const uint4*>(q + unit[i].at));
+                s[i] = scale[(u0 + i * stride) >> 3];
+                if (DY) g[i].stream(dy + unit[i].at);
             }
-            store_n<T, 16>(out + at, g);
-            if (y) store_n<T, 16>(y + at, v);
-        } else {
-            store_n<T, 16>(out + at, v);
+        }
+#pragma unroll
+        for (int i = 0; i < A8_UNITS; i++) {
+            if (!unit[i].live) continue;
+            float2 v[8];
+            a8_unpack16(w[i], s[i], v);
+            if (DY) {
+                float2 d[8];
+                g[i].to(d);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const GeluTerms t0 = gelu_terms(v[e].x), t1 = gelu_terms(v[e].y);
+                    d[e] = __fmul2_rn(d[e], make_float2(t0.dy, t1.dy));
+                    v[e] = make_float2(t0.y, t1.y);
+                }
+                store16(out + unit[i].at, d);
+                if (y) store16(y + unit[i].at, v);
+            } else {
+                store16(out + unit[i].at, v);
+            }
         }
     }
     pdl_launch_dependents();
@@ -287,15 +324,25 @@ static int a8_unpack(const int8_t* q, const float* scale, const void* dy, void* 
 }
 
 // ---- LayerNorm ---------------------------------------------------------------------------------------------------------
-// A thread owns 8 columns, so 16 neighbouring lanes are a block of 128; a row is owned by a team of `team` threads (a
-// multiple of 32, at most 1024: rows of up to 8192 columns), and a CTA holds blockDim.x / team teams that meet at named
-// barriers of their own and never wait for one another.
+// A thread owns 16 columns, so 8 neighbouring lanes are a block of 128; a row is owned by a team of `team` threads (a
+// multiple of 32, at most 512: rows of up to 8192 columns), and a CTA holds blockDim.x / team teams that meet at named
+// barriers of their own and never wait for one another.  Rows are fetched ahead into registers, still packed: the two
+// reductions of a row leave the memory system idle otherwise (without the fetch ahead [8192, 4096] fp16 took 61 us forward).
 constexpr int A8_LN_MAX_COLS = 8192;
+constexpr int A8_LN_THREADS = 512;
 
 __device__ __forceinline__ void team_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// Sum of a and b over the team; red: 64 floats of this team, used alternately by the caller (two buffers) so that one
-// barrier per reduction is enough.
+// Sums over the team; red: one cell per warp of the team, used alternately by the caller (two buffers) so that one barrier per
+// reduction is enough.
+__device__ __forceinline__ float team_sum(float a, float* red, int id, int team) {
+    a = warp_sum(a);
+    if (team == 32) return a;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x % team) >> 5, warps = team >> 5;
+    if (lane == 0) red[warp] = a;
+    team_barrier(id, team);
+    return warp_sum(lane < warps ? red[lane] : 0.0f);
+}
 __device__ __forceinline__ float2 team_sum2(float a, float b, float2* red, int id, int team) {
     a = warp_sum(a);
     b = warp_sum(b);
@@ -307,65 +354,82 @@ __device__ __forceinline__ float2 team_sum2(float a, float b, float2* red, int i
     return make_float2(warp_sum(t.x), warp_sum(t.y));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(1024)
+// gamma and beta wait in shared memory, in fp32: unpacking them again for every row took a quarter of the instructions.
+template <typename T, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS)
 a8_ln_fwd_kernel(const T* x, const T* __restrict__ gamma, const T* __restrict__ beta, T* y, int8_t* __restrict__ q,
                  float* __restrict__ scale, float* __restrict__ var, int64_t rows, int cols, float eps, int team) {
-    __shared__ float2 red[32][2];            // [warp of the CTA][buffer]: a team uses its own warps' cells
+    extern __shared__ __align__(16) float affine[];         // gamma [16 * team], beta [16 * team]
+    __shared__ float red[2][THREADS / 32];                  // [buffer][warp of the CTA]: a team uses its own warps' cells
     const int tid = threadIdx.x % team, group = threadIdx.x / team, groups = blockDim.x / team;
-    const int c = tid * 8, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
+    const int c = tid * 16, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
     const bool live = c < cols;
     const float inv_n = 1.0f / (float)cols;
-    float2* r0 = &red[0][0] + group * (team >> 5);
-    float2* r1 = r0 + 32;
-    float ga[8], be[8];
-    if (live) {
-        load_n<T, 8>(gamma + c, ga);
-        load_n<T, 8>(beta + c, be);
+    float* r0 = red[0] + group * (team >> 5);
+    float* r1 = red[1] + group * (team >> 5);
+    // column c + 4 i of thread t lies at [i][t]: neighbouring threads read neighbouring 16 bytes
+    float4* const ga = reinterpret_cast<float4*>(affine) + tid;
+    float4* const be = ga + 4 * team;
+    if (group == 0 && live) {
+        Pack16<T> raw;
+        float2 v[8];
+        raw.load(gamma + c);
+        raw.to(v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) ga[i * team] = make_float4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y);
+        raw.load(beta + c);
+        raw.to(v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) be[i * team] = make_float4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y);
     }
+    __syncthreads();
     pdl_wait();
-    for (int64_t row = (int64_t)blockIdx.x * groups + group; row < rows; row += (int64_t)gridDim.x * groups) {
-        float v[8];
-        if (live) {
-            load_n<T, 8>(x + row * cols + c, v);
-        } else {
+    Pack16<T> ahead[2] = {};
+    const int64_t step = (int64_t)gridDim.x * groups;
+    int64_t row = (int64_t)blockIdx.x * groups + group;
+    if (live && row < rows) ahead[0].stream(x + row * cols + c);
+    if (live && row + step < rows) ahead[1].stream(x + (row + step) * cols + c);
+    for (; row < rows; row += step) {
+        float2 v[8];
+        ahead[0].to(v);                                     // zeros beyond the last column
+        ahead[0] = ahead[1];
+        if (live && row + 2 * step < rows) ahead[1].stream(x + (row + 2 * step) * cols + c);
+        float2 s = v[0];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = 0.0f;
-        }
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) s += v[e];
-        const float mu = team_sum2(s, 0.0f, r0, group + 1, team).x * inv_n;
-        float d2 = 0.0f;
+        for (int e = 1; e < 8; e++) s = __fadd2_rn(s, v[e]);
+        const float mu = team_sum(s.x + s.y, r0, group + 1, team) * inv_n;
+        float2 d2 = both(0.0f);
         if (live) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                v[e] -= mu;
-                d2 = fmaf(v[e], v[e], d2);
+                v[e] = __fadd2_rn(v[e], both(-mu));
+                d2 = __ffma2_rn(v[e], v[e], d2);
             }
         }
-        const float va = fmaf(team_sum2(d2, 0.0f, r1, group + 1, team).x, inv_n, eps);
+        const float va = fmaf(team_sum(d2.x + d2.y, r1, group + 1, team), inv_n, eps);
         const float rstd = rsqrtf(va);
-        uint32_t top = 0;
+        float top = 0.0f;
         if (live) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                v[e] *= rstd;
-                top = max(top, mag_bits(v[e]));
+                v[e] = __fmul2_rn(v[e], both(rstd));
+                top = max3(top, fabsf(v[e].x), fabsf(v[e].y));
             }
         }
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (live) {
-            const A8Scale sc = a8_scale(top);
-            uint2 w;
-            w.x = a8_pack4(v[0], v[1], v[2], v[3], sc.inv);
-            w.y = a8_pack4(v[4], v[5], v[6], v[7], sc.inv);
-            __stcs(reinterpret_cast<uint2*>(q + row * cols + c), w);
-            if ((threadIdx.x & 15) == 0) scale[row * blocks + (c >> 7)] = sc.scale;
+            // a value that is not finite makes the row's variance so, and every normalised value with it
+            const A8Scale sc = a8_scale(va < INFINITY ? __float_as_uint(top) : 0x7fffffffu);
+            __stcs(reinterpret_cast<uint4*>(q + row * cols + c), a8_pack16(v, sc.inv));
+            if ((threadIdx.x & 7) == 0) scale[row * blocks + (c >> 7)] = sc.scale;
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = fmaf(v[e], ga[e], be[e]);
-            store_n<T, 8>(y + row * cols + c, v);
+            for (int i = 0; i < 4; i++) {
+                const float4 g = ga[i * team], b = be[i * team];
+                v[2 * i] = __ffma2_rn(v[2 * i], make_float2(g.x, g.y), make_float2(b.x, b.y));
+                v[2 * i + 1] = __ffma2_rn(v[2 * i + 1], make_float2(g.z, g.w), make_float2(b.z, b.w));
+            }
+            store16(y + row * cols + c, v);
         }
         if (tid == 0) var[row] = va;
     }
@@ -407,7 +471,7 @@ a8_ln_fwd_generic_kernel(const T* x, const T* gamma, const T* beta, T* y, int8_t
         for (int i = 0; i < 4; i++) {
             const int c = b * A8_BLOCK + i * 32 + lane;
             if (c < cols) {
-                q[row * cols + c] = (int8_t)(a8_pack4(v[i], 0.0f, 0.0f, 0.0f, sc.inv) & 0xff);
+                q[row * cols + c] = a8_pack1(v[i], sc.inv);
                 y[row * cols + c] = from_f32<T>(fmaf(v[i], to_f32(gamma[c]), to_f32(beta[c])));
             }
         }
@@ -419,46 +483,40 @@ a8_ln_fwd_generic_kernel(const T* x, const T* gamma, const T* beta, T* y, int8_t
 // Backward.  g = dy * gamma;  dx = rstd * (g - mean(g) - xhat * mean(g * xhat)) (+ residual);  the column sums of
 // dy * xhat and dy stay in the registers of the column's owner over all rows of the CTA, are added over the CTA's teams
 // through shared memory and leave as one row of `part` [gridDim.x][2][cols], which a second kernel adds in order.
-// The next row's packets are fetched before this row's barrier, so a row's latency passes behind the row before it.
+// The next row's packets are fetched before this row's barrier, so a row's latency passes behind the row before it; what is
+// needed on both sides of the barrier is unpacked twice rather than held in 32 bits, which would not fit the registers.
 template <typename T, bool RES, bool AGAIN>
-__global__ void __launch_bounds__(1024, 1)
+__global__ void __launch_bounds__(A8_LN_THREADS, 1)
 a8_ln_bwd_kernel(const T* dy, const T* __restrict__ gamma, const T* __restrict__ beta, const float* __restrict__ var,
                  const int8_t* __restrict__ q, const float* __restrict__ scale, const T* residual, T* dx, T* __restrict__ y,
                  float* __restrict__ part, int64_t rows, int cols, int team) {
-    constexpr int VN = Vec<T>::N, NP = 8 / VN;
     extern __shared__ float fold[];          // [teams - 1][2][cols]
-    __shared__ float2 red[2][32];
+    __shared__ float2 red[2][A8_LN_THREADS / 32];
     const int tid = threadIdx.x % team, group = threadIdx.x / team, groups = blockDim.x / team;
-    const int c = tid * 8, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
+    const int c = tid * 16, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
     const bool live = c < cols;
     const float inv_n = 1.0f / (float)cols;
     float2* r0 = red[0] + group * (team >> 5);
     float2* r1 = red[1] + group * (team >> 5);
-    float dg[8], db[8];
+    float2 dg[8], db[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) dg[e] = db[e] = 0.0f;
-    uint4 gam[NP], bet[NP];                  // kept packed: eight floats each would not fit the registers
+    for (int e = 0; e < 8; e++) dg[e] = db[e] = both(0.0f);
+    Pack16<T> gam = {}, bet = {};
     if (live) {
-#pragma unroll
-        for (int i = 0; i < NP; i++) {
-            gam[i] = ld_raw(gamma + c + i * VN);
-            if (AGAIN) bet[i] = ld_raw(beta + c + i * VN);
-        }
+        gam.load(gamma + c);
+        if (AGAIN) bet.load(beta + c);
     }
     pdl_wait();
 
-    uint4 n_dy[NP], n_res[NP];
-    uint2 n_q = make_uint2(0x80808080u, 0x80808080u);
+    Pack16<T> n_dy = {}, n_res = {};
+    uint4 n_q = make_uint4(0, 0, 0, 0);
     float n_scale = 0.0f, n_var = 1.0f;
     auto fetch = [&](int64_t row) {
         if (live) {
             const int64_t at = row * cols + c;
-#pragma unroll
-            for (int i = 0; i < NP; i++) {
-                n_dy[i] = ld_raw_stream(dy + at + i * VN);
-                if (RES) n_res[i] = ld_raw_stream(residual + at + i * VN);
-            }
-            n_q = __ldcs(reinterpret_cast<const uint2*>(q + at));
+            n_dy.stream(dy + at);
+            if (RES) n_res.stream(residual + at);
+            n_q = __ldcs(reinterpret_cast<const uint4*>(q + at));
             n_scale = scale[row * blocks + (c >> 7)];
         }
         n_var = var[row];
@@ -467,74 +525,68 @@ a8_ln_bwd_kernel(const T* dy, const T* __restrict__ gamma, const T* __restrict__
     int64_t row = (int64_t)blockIdx.x * groups + group;
     if (row < rows) fetch(row);
     for (int turn = 0; row < rows; row += step, turn ^= 1) {
-        float xh[8], g[8];
-        uint4 res[NP];
-        const float rstd = rsqrtf(n_var);
-        float a = 0.0f, b = 0.0f;
-        if (live) {
-            a8_unpack4(n_q.x, n_scale, xh);
-            a8_unpack4(n_q.y, n_scale, xh + 4);
+        const Pack16<T> p_dy = n_dy, p_res = n_res;
+        const uint4 w = n_q;
+        const float sc = n_scale, rstd = rsqrtf(n_var);
+        if (row + step < rows) fetch(row + step);
+        float2 a = both(0.0f), b = both(0.0f);
+        {
+            float2 xh[8], d[8], ga[8];
+            a8_unpack16(w, sc, xh);
+            p_dy.to(d);
+            gam.to(ga);
 #pragma unroll
-            for (int i = 0; i < NP; i++) {
-                Vec<T> d, w;
-                d.unpack(n_dy[i]);
-                w.unpack(gam[i]);
-                if (RES) res[i] = n_res[i];
-#pragma unroll
-                for (int e = 0; e < VN; e++) {
-                    const int j = i * VN + e;
-                    dg[j] = fmaf(d.v[e], xh[j], dg[j]);
-                    db[j] += d.v[e];
-                    g[j] = d.v[e] * w.v[e];
-                    a += g[j];
-                    b = fmaf(g[j], xh[j], b);
-                }
+            for (int e = 0; e < 8; e++) {
+                dg[e] = __ffma2_rn(d[e], xh[e], dg[e]);
+                db[e] = __fadd2_rn(db[e], d[e]);
+                const float2 g = __fmul2_rn(d[e], ga[e]);
+                a = __fadd2_rn(a, g);
+                b = __ffma2_rn(g, xh[e], b);
             }
         }
-        if (row + step < rows) fetch(row + step);
-        const float2 m = team_sum2(a, b, turn ? r1 : r0, group + 1, team);
+        const float2 m = team_sum2(a.x + a.y, b.x + b.y, turn ? r1 : r0, group + 1, team);
         if (live) {
-            const float mg = m.x * inv_n, mgx = m.y * inv_n;
+            const float2 mg = both(-rstd * m.x * inv_n), mgx = both(-rstd * m.y * inv_n);
             const int64_t at = row * cols + c;
+            float2 xh[8], o[8], ga[8];
+            a8_unpack16(w, sc, xh);
+            p_dy.to(o);
+            gam.to(ga);
 #pragma unroll
-            for (int i = 0; i < NP; i++) {
-                Vec<T> o, r;
-                if (RES) r.unpack(res[i]);
+            for (int e = 0; e < 8; e++) o[e] = __ffma2_rn(xh[e], mgx, __ffma2_rn(__fmul2_rn(o[e], ga[e]), both(rstd), mg));
+            if (RES) {
+                float2 r[8];
+                p_res.to(r);
 #pragma unroll
-                for (int e = 0; e < VN; e++) {
-                    const int j = i * VN + e;
-                    o.v[e] = rstd * (g[j] - mg - xh[j] * mgx);
-                    if (RES) o.v[e] += r.v[e];
-                }
-                o.store_stream(dx + at + i * VN);
-                if (AGAIN) {
-                    Vec<T> w, s;
-                    w.unpack(gam[i]);
-                    s.unpack(bet[i]);
+                for (int e = 0; e < 8; e++) o[e] = __fadd2_rn(o[e], r[e]);
+            }
+            store16(dx + at, o);
+            if (AGAIN) {
+                float2 be[8];
+                bet.to(be);
 #pragma unroll
-                    for (int e = 0; e < VN; e++) o.v[e] = fmaf(xh[i * VN + e], w.v[e], s.v[e]);
-                    o.store_stream(y + at + i * VN);
-                }
+                for (int e = 0; e < 8; e++) o[e] = __ffma2_rn(xh[e], ga[e], be[e]);
+                store16(y + at, o);
             }
         }
     }
     if (groups > 1) {
         if (group > 0 && live) {
-            float* f = fold + (int64_t)(group - 1) * 2 * cols + c;
+            float2* f = reinterpret_cast<float2*>(fold + (int64_t)(group - 1) * 2 * cols + c);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 f[e] = dg[e];
-                f[cols + e] = db[e];
+                f[cols / 2 + e] = db[e];
             }
         }
         __syncthreads();
         if (group == 0 && live) {
             for (int k = 0; k < groups - 1; k++) {
-                const float* f = fold + (int64_t)k * 2 * cols + c;
+                const float2* f = reinterpret_cast<const float2*>(fold + (int64_t)k * 2 * cols + c);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    dg[e] += f[e];
-                    db[e] += f[cols + e];
+                    dg[e] = __fadd2_rn(dg[e], f[e]);
+                    db[e] = __fadd2_rn(db[e], f[cols / 2 + e]);
                 }
             }
         }
@@ -542,9 +594,9 @@ a8_ln_bwd_kernel(const T* dy, const T* __restrict__ gamma, const T* __restrict__
     if (group == 0 && live) {
         float* p = part + (int64_t)blockIdx.x * 2 * cols + c;
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            *reinterpret_cast<float4*>(p + e) = make_float4(dg[e], dg[e + 1], dg[e + 2], dg[e + 3]);
-            *reinterpret_cast<float4*>(p + cols + e) = make_float4(db[e], db[e + 1], db[e + 2], db[e + 3]);
+        for (int e = 0; e < 8; e += 2) {
+            *reinterpret_cast<float4*>(p + 2 * e) = make_float4(dg[e].x, dg[e].y, dg[e + 1].x, dg[e + 1].y);
+            *reinterpret_cast<float4*>(p + cols + 2 * e) = make_float4(db[e].x, db[e].y, db[e + 1].x, db[e + 1].y);
         }
     }
     pdl_launch_dependents();
@@ -591,8 +643,10 @@ a8_ln_reduce_kernel(const float* part, T* dgamma, T* dbeta, int parts, int cols,
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t j = (int64_t)blockIdx.x * 32 + lane;
     float a = 0.0f;
-    if (j < 2 * (int64_t)cols)
+    if (j < 2 * (int64_t)cols) {
+#pragma unroll 8
         for (int k = warp; k < parts; k += 8) a += part[(int64_t)k * 2 * cols + j];
+    }
     s[warp][lane] = a;
     __syncthreads();
     if (warp == 0 && j < 2 * (int64_t)cols) {
@@ -602,19 +656,32 @@ a8_ln_reduce_kernel(const float* part, T* dgamma, T* dbeta, int parts, int cols,
     }
 }
 
-// threads that own a row of `cols` columns, 8 each
-static int a8_team(int64_t cols) { return (int)((cols + 255) / 256) * 32; }
+// threads that own a row of `cols` columns, 16 each
+static int a8_team(int64_t cols) { return (int)((cols + 511) / 512) * 32; }
 
 constexpr int A8_MAX_PARTS = 256;             // partial rows of the LayerNorm backward: one per CTA
 
 template <typename T>
 static int a8_ln_fwd(const void* x, const void* gamma, const void* beta, void* y, int8_t* q, float* scale, float* var, int64_t rows, int64_t cols,
                      float eps, cudaStream_t st) {
-    if (cols % 8 == 0 && cols <= A8_LN_MAX_COLS && aligned16(x) && aligned16(gamma) && aligned16(beta) && aligned16(y) && (reinterpret_cast<uintptr_t>(q) & 7) == 0) {
+    if (cols % 16 == 0 && cols <= A8_LN_MAX_COLS && aligned16(x) && aligned16(gamma) && aligned16(beta) && aligned16(y) && aligned16(q)) {
         const int team = a8_team(cols), groups = team >= 256 ? 1 : 256 / team;
-        const int64_t want = (rows + groups - 1) / groups, cap = (int64_t)sm_count() * (2048 / (team * groups));
-        const cudaError_t e = launch_pdl(a8_ln_fwd_kernel<T>, (int)(want < cap ? want : cap), team * groups, 0, st, (const T*)x, (const T*)gamma, (const T*)beta,
-                                         (T*)y, q, scale, var, rows, (int)cols, eps, team);
+        // as many CTAs as are resident at once; long rows need all of an SM's registers for one team
+        const int ctas = team > 256 ? 1 : 3;
+        const int64_t want = (rows + groups - 1) / groups, cap = (int64_t)sm_count() * ctas;
+        const int grid = (int)(want < cap ? want : cap);
+        const size_t smem = (size_t)team * 32 * sizeof(float);
+        cudaError_t e = cudaSuccess;
+        if (smem > 48 * 1024) e = cudaFuncSetAttribute(a8_ln_fwd_kernel<T, 512, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) {
+            set_cuda_error(e, "a8_ln_fwd smem attribute");
+            return BRK_CUDA_ERROR;
+        }
+        if (team > 256)
+            e = launch_pdl(a8_ln_fwd_kernel<T, 512, 1>, grid, team, smem, st, (const T*)x, (const T*)gamma, (const T*)beta, (T*)y, q, scale, var, rows, (int)cols, eps, team);
+        else
+            e = launch_pdl(a8_ln_fwd_kernel<T, 256, 3>, grid, team * groups, smem, st, (const T*)x, (const T*)gamma, (const T*)beta, (T*)y, q, scale, var, rows, (int)cols,
+                           eps, team);
         if (e != cudaSuccess) {
             set_cuda_error(e, "a8_ln_fwd_kernel");
             return BRK_CUDA_ERROR;
@@ -641,10 +708,10 @@ static int a8_ln_bwd(const void* dy_, const void* gamma_, const void* beta_, con
     const T *dy = (const T*)dy_, *gamma = (const T*)gamma_, *beta = (const T*)beta_, *residual = (const T*)residual_;
     T *dx = (T*)dx_, *y = (T*)y_;
     int parts;
-    if (cols % 8 == 0 && cols <= A8_LN_MAX_COLS && aligned16(dy) && aligned16(gamma) && aligned16(dx) && aligned16(part) && (!residual || aligned16(residual)) &&
-        (!y || (aligned16(y) && aligned16(beta))) && (reinterpret_cast<uintptr_t>(q) & 7) == 0) {
+    if (cols % 16 == 0 && cols <= A8_LN_MAX_COLS && aligned16(dy) && aligned16(gamma) && aligned16(dx) && aligned16(part) && (!residual || aligned16(residual)) &&
+        (!y || (aligned16(y) && aligned16(beta))) && aligned16(q)) {
         const int team = a8_team(cols);
-        int groups = 1024 / team;
+        int groups = A8_LN_THREADS / team;
         if ((int64_t)groups * sm_count() > rows) groups = (int)((rows + sm_count() - 1) / sm_count());      // few rows: spread them over the SMs
         if (groups > 15) groups = 15;                                                                      // named barriers 1..15
         const int64_t want = (rows + groups - 1) / groups;

@@ -32,7 +32,8 @@ def _ptr(t):
 
 
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the raw handle without a Stream object around it, which takes 3 us to make
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def layernorm(x, gamma, beta, eps=1e-5, out=None):
@@ -213,104 +214,123 @@ def gemm_f16(a, b, c, m, n, k, trans_a, trans_b, lda, ldb, ldc, bias=None, resid
 
 
 # --- packed documents ---
-def _chk_all(expect, **named):
-    """Each tensor (None passes): contiguous, on the current device, of its dtype and shape in `expect`."""
-    for name, t in named.items():
-        if t is None:
-            continue
-        _chk(t)
-        _chk_device(t)
-        dtype, shape = expect[name]
-        if t.dtype != dtype or tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-
-
-def _chk_device(t):
-    if t.device.index != torch.cuda.current_device():
+# These calls are short enough for their front end to be seen: one look at each tensor, and words only where one is refused.
+def _device(t):
+    """The current device, which `t` has to be on: the kernels are queued on its current stream."""
+    if not t.is_cuda:
+        raise RuntimeError("blackriver_b200 operators run on CUDA tensors only (no CPU path)")
+    device = torch.cuda.current_device()
+    if t.get_device() != device:
         raise RuntimeError("tensors must live on the current device, whose stream the kernels are queued on")
+    return device
+
+
+def _refuse(name, t, dtype, shape, device):
+    if not t.is_cuda:
+        raise RuntimeError("blackriver_b200 operators run on CUDA tensors only (no CPU path)")
+    if t.get_device() != device:
+        raise RuntimeError(f"{name} must live on the current device, whose stream the kernels are queued on")
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    raise RuntimeError("tensors must be contiguous")
+
+
+def _take(name, t, dtype, shape, device):
+    """Address of a contiguous tensor of that type and shape on that device; 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        _refuse(name, t, dtype, shape, device)
+    return t.data_ptr()
 
 
 def doc_plan(mask, prompt=None, ids=None):
     """Spans of packed documents: mask [batch, tokens] int32 numbers the documents (0 or less = padding), prompt marks
     the tokens of prompts.  Returns int32 spans [batch, tokens, 4] for doc_attn; with ids also the loss targets and their
     count: (spans, target, count)."""
-    if mask.dim() != 2:
+    device = _device(mask)
+    shape = mask.shape
+    if len(shape) != 2:
         raise ValueError("mask must be [batch, tokens]")
-    like = (torch.int32, mask.shape)
-    _chk_all({"mask": like, "prompt": like, "ids": like}, mask=mask, prompt=prompt, ids=ids)
-    b, t = mask.shape
-    spans = torch.empty((b, t, 4), dtype=torch.int32, device=mask.device)
-    target = count = None
-    if ids is not None:
-        target = torch.empty_like(ids)
-        count = torch.empty(1, dtype=torch.int32, device=ids.device)
-    brk.call("brk_doc_plan", _ptr(mask), _ptr(prompt), _ptr(ids), b, t, _ptr(spans), _ptr(target), _ptr(count), stream())
-    return spans if ids is None else (spans, target, count)
+    b, t = shape
+    a_mask, a_prompt, a_ids = (_take(n, x, torch.int32, shape, device) for n, x in (("mask", mask), ("prompt", prompt), ("ids", ids)))
+    spans = mask.new_empty((b, t, 4))
+    if ids is None:
+        brk.call("brk_doc_plan", a_mask, a_prompt, 0, b, t, spans.data_ptr(), 0, 0, stream())
+        return spans
+    target = torch.empty_like(ids)
+    count = ids.new_empty((1,))
+    brk.call("brk_doc_plan", a_mask, a_prompt, a_ids, b, t, spans.data_ptr(), target.data_ptr(), count.data_ptr(), stream())
+    return spans, target, count
 
 
-def _heads_view(name, t, batch, tokens, heads, dim):
-    """Row stride of a [batch, tokens, heads, head_dim] fp16 tensor whose heads lie side by side in a token's row."""
-    if not t.is_cuda:
-        raise RuntimeError("blackriver_b200 operators run on CUDA tensors only (no CPU path)")
-    _chk_device(t)
-    if t.dtype != torch.float16:
+def _heads(name, t, b, n, h, d, device):
+    """(address, row stride) of a [batch, tokens, heads, head_dim] fp16 tensor whose heads lie side by side in a token's row."""
+    if t.get_device() != device:
+        _refuse(name, t, t.dtype, t.shape, device)
+    if t.dtype is not torch.float16:
         raise TypeError(f"unsupported dtype {t.dtype}")
-    if t.dim() != 4 or t.shape[0] != batch or t.shape[1] != tokens or t.shape[3] != dim or (heads is not None and t.shape[2] != heads):
-        raise ValueError(f"{name} must be [{batch}, {tokens}, {heads or 'heads'}, {dim}], got {tuple(t.shape)}")
-    ld = t.stride(1) if tokens > 1 else t.stride(0) if batch > 1 else t.shape[2] * dim
-    if t.numel() and ((dim > 1 and t.stride(3) != 1) or (t.shape[2] > 1 and t.stride(2) != dim) or (batch > 1 and t.stride(0) != tokens * ld)):
+    if t.shape != (b, n, h, d):
+        raise ValueError(f"{name} must be [{b}, {n}, {h}, {d}], got {tuple(t.shape)}")
+    s = t.stride()
+    ld = s[1] if n > 1 else s[0] if b > 1 else h * d
+    if b * n and ((d > 1 and s[3] != 1) or (h > 1 and s[2] != d) or (b > 1 and s[0] != n * ld)):
         raise ValueError(f"{name}: heads must lie side by side and tokens at one stride")
-    return ld
+    return t.data_ptr(), ld
 
 
 def _doc_args(q, k, v, spans, slopes):
+    device = _device(q)
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q, k and v must be [batch, tokens, heads, head_dim]")
-    b, t, h, d = q.shape
+    b, n, h, d = q.shape
     hk = k.shape[2]
-    ld_q, ld_kv = _heads_view("q", q, b, t, h, d), _heads_view("k", k, b, t, hk, d)
-    if _heads_view("v", v, b, t, hk, d) != ld_kv:
+    a_q, ld_q = _heads("q", q, b, n, h, d, device)
+    a_k, ld_kv = _heads("k", k, b, n, hk, d, device)
+    a_v, ld_v = _heads("v", v, b, n, hk, d, device)
+    if ld_v != ld_kv:
         raise ValueError("k and v must have the same row stride")
-    _chk_all({"spans": (torch.int32, (b, t, 4)), "slopes": (torch.float32, (h,))}, spans=spans, slopes=slopes)
-    return b, t, h, hk, d, ld_q, ld_kv
+    return device, b, n, h, hk, d, a_q, a_k, a_v, ld_q, ld_kv, _take("spans", spans, torch.int32, (b, n, 4), device), _take("slopes", slopes, torch.float32, (h,), device)
 
 
 def doc_attn(q, k, v, spans, slopes=None, cap=0.0, out=None, lse=None):
     """Attention over packed documents: q [batch, tokens, heads, head_dim], k and v [batch, tokens, kv_heads, head_dim]
     fp16 (views of a fused projection are read in place), spans from doc_plan.  slopes [heads]: bias -slope * distance;
     cap: scores capped by cap * tanh(score / cap).  Returns (out, lse [batch, heads, tokens])."""
-    b, t, h, hk, d, ld_q, ld_kv = _doc_args(q, k, v, spans, slopes)
-    out = torch.empty((b, t, h, d), dtype=q.dtype, device=q.device) if out is None else out
-    lse = torch.empty((b, h, t), dtype=torch.float32, device=q.device) if lse is None else lse
-    ld_out = _heads_view("out", out, b, t, h, d)
-    _chk_all({"lse": (torch.float32, (b, h, t))}, lse=lse)
-    brk.call("brk_doc_attn_fwd", _ptr(q), _ptr(k), _ptr(v), ld_q, ld_kv, _ptr(out), ld_out, _ptr(lse), _ptr(spans), _ptr(slopes), float(cap),
-             b, t, h, hk, d, stream())
+    device, b, n, h, hk, d, a_q, a_k, a_v, ld_q, ld_kv, a_spans, a_slopes = _doc_args(q, k, v, spans, slopes)
+    if out is None:
+        out = q.new_empty((b, n, h, d))
+    if lse is None:
+        lse = q.new_empty((b, h, n), dtype=torch.float32)
+    a_out, ld_out = _heads("out", out, b, n, h, d, device)
+    brk.call("brk_doc_attn_fwd", a_q, a_k, a_v, ld_q, ld_kv, a_out, ld_out, _take("lse", lse, torch.float32, (b, h, n), device), a_spans, a_slopes, cap, b, n, h,
+             hk, d, stream())
     return out, lse
 
 
 def doc_attn_backward(d_out, q, k, v, out, lse, spans, slopes=None, cap=0.0, dq=None, dk=None, dv=None, workspace=None):
     """Gradients (dq, dk, dv) of doc_attn; without dq, dk and dv they are views of one fused [batch, tokens, heads + 2 kv_heads,
     head_dim] buffer, as the projection's backward wants them."""
-    b, t, h, hk, d, ld_q, ld_kv = _doc_args(q, k, v, spans, slopes)
-    ld_out = _heads_view("out", out, b, t, h, d)
-    if _heads_view("d_out", d_out, b, t, h, d) != ld_out:
+    device, b, n, h, hk, d, a_q, a_k, a_v, ld_q, ld_kv, a_spans, a_slopes = _doc_args(q, k, v, spans, slopes)
+    a_out, ld_out = _heads("out", out, b, n, h, d, device)
+    a_do, ld_do = _heads("d_out", d_out, b, n, h, d, device)
+    if ld_do != ld_out:
         raise ValueError("out and d_out must have the same row stride")
-    _chk_all({"lse": (torch.float32, (b, h, t))}, lse=lse)
+    a_lse = _take("lse", lse, torch.float32, (b, h, n), device)
     if dq is None and dk is None and dv is None:
-        fused = torch.empty((b, t, h + 2 * hk, d), dtype=q.dtype, device=q.device)
-        dq, dk, dv = fused[:, :, :h], fused[:, :, h:h + hk], fused[:, :, h + hk:]
+        dq, dk, dv = q.new_empty((b, n, h + 2 * hk, d)).split((h, hk, hk), 2)
     elif dq is None or dk is None or dv is None:
         raise ValueError("give all of dq, dk and dv, or none")
-    ld_dq, ld_dkv = _heads_view("dq", dq, b, t, h, d), _heads_view("dk", dk, b, t, hk, d)
-    if _heads_view("dv", dv, b, t, hk, d) != ld_dkv:
+    a_dq, ld_dq = _heads("dq", dq, b, n, h, d, device)
+    a_dk, ld_dkv = _heads("dk", dk, b, n, hk, d, device)
+    a_dv, ld_dv = _heads("dv", dv, b, n, hk, d, device)
+    if ld_dv != ld_dkv:
         raise ValueError("dk and dv must have the same row stride")
     if workspace is None:
-        workspace = torch.empty(max(brk.lib().brk_doc_attn_bwd_workspace_bytes(b, t, h), 16), dtype=torch.uint8, device=q.device)
-    _chk(workspace)
-    _chk_device(workspace)
-    brk.call("brk_doc_attn_bwd", _ptr(q), _ptr(k), _ptr(v), ld_q, ld_kv, _ptr(out), _ptr(d_out), ld_out, _ptr(lse), _ptr(dq), ld_dq, _ptr(dk),
-             _ptr(dv), ld_dkv, _ptr(spans), _ptr(slopes), float(cap), b, t, h, hk, d, _ptr(workspace), workspace.numel() * workspace.element_size(), stream())
+        workspace = q.new_empty((max(brk.lib().brk_doc_attn_bwd_workspace_bytes(b, n, h), 16),), dtype=torch.uint8)
+    a_ws = _take("workspace", workspace, workspace.dtype, workspace.shape, device)
+    brk.call("brk_doc_attn_bwd", a_q, a_k, a_v, ld_q, ld_kv, a_out, a_do, ld_out, a_lse, a_dq, ld_dq, a_dk, a_dv, ld_dkv, a_spans, a_slopes, cap, b, n, h, hk, d,
+             a_ws, workspace.numel() * workspace.element_size(), stream())
     return dq, dk, dv
 
 
@@ -318,102 +338,96 @@ def doc_attn_backward(d_out, q, k, v, out, lse, spans, slopes=None, cap=0.0, dq=
 ACT8_BLOCK = 128        # columns that share a scale
 
 
-def _act8_shapes(rows, cols):
-    return {"q": (torch.int8, (rows, cols)), "scale": (torch.float32, (rows, -(-cols // ACT8_BLOCK)))}
-
-
-def _act8_new(rows, cols, device):
-    return (torch.empty((rows, cols), dtype=torch.int8, device=device),
-            torch.empty((rows, -(-cols // ACT8_BLOCK)), dtype=torch.float32, device=device))
-
-
-def _rows_cols(t):
-    if t.dim() < 1 or t.shape[-1] == 0:
+def _act8_like(t):
+    """(device, rows, cols, address) of an activation tensor [..., cols]."""
+    device = _device(t)
+    shape = t.shape
+    if not shape or shape[-1] == 0:
         raise ValueError("activations need at least one column")
-    return t.numel() // t.shape[-1], t.shape[-1]
+    if not t.is_contiguous():
+        raise RuntimeError("tensors must be contiguous")
+    return device, t.numel() // shape[-1], shape[-1], t.data_ptr()
+
+
+def _act8_new(t, rows, cols):
+    q = torch.empty_like(t, dtype=torch.int8) if t.dim() == 2 else t.new_empty((rows, cols), dtype=torch.int8)
+    return q, t.new_empty((rows, -(-cols // ACT8_BLOCK)), dtype=torch.float32)
+
+
+def _act8_take(q, scale, rows, cols, device):
+    return _take("q", q, torch.int8, (rows, cols), device), _take("scale", scale, torch.float32, (rows, -(-cols // ACT8_BLOCK)), device)
 
 
 def act8_pack(x):
     """x [..., cols] -> (q int8 [rows, cols], scale fp32 [rows, ceil(cols / 128)])."""
-    _chk(x)
-    _chk_device(x)
-    rows, cols = _rows_cols(x)
-    q, scale = _act8_new(rows, cols, x.device)
-    brk.call("brk_act8_pack", _ptr(x), _ptr(q), _ptr(scale), rows, cols, _dt(x), stream())
+    device, rows, cols, a_x = _act8_like(x)
+    q, scale = _act8_new(x, rows, cols)
+    brk.call("brk_act8_pack", a_x, q.data_ptr(), scale.data_ptr(), rows, cols, _dt(x), stream())
     return q, scale
 
 
 def act8_unpack(q, scale, dtype=torch.float16, out=None):
     """The kept values, [rows, cols] of `dtype` (or into out)."""
-    rows, cols = _rows_cols(q)
-    _chk_all(_act8_shapes(rows, cols), q=q, scale=scale)
-    out = torch.empty((rows, cols), dtype=dtype, device=q.device) if out is None else out
-    _chk_all({"out": (out.dtype, q.shape)}, out=out)
-    brk.call("brk_act8_unpack", _ptr(q), _ptr(scale), _ptr(out), rows, cols, _dt(out), stream())
+    device, rows, cols, _ = _act8_like(q)
+    a_q, a_scale = _act8_take(q, scale, rows, cols, device)
+    if out is None:
+        out = torch.empty_like(q, dtype=dtype)
+    brk.call("brk_act8_unpack", a_q, a_scale, _take("out", out, out.dtype, q.shape, device), rows, cols, _dt(out), stream())
     return out
 
 
 def gelu_act8(x, out=None):
     """gelu(x) and x kept in 8 bits: (y, q, scale)."""
-    _chk(x, out)
-    _chk_device(x)
-    rows, cols = _rows_cols(x)
+    device, rows, cols, a_x = _act8_like(x)
     y = torch.empty_like(x) if out is None else out
-    _chk_all({"out": (x.dtype, x.shape)}, out=y)
-    q, scale = _act8_new(rows, cols, x.device)
-    brk.call("brk_gelu_fwd_act8", _ptr(x), _ptr(y), _ptr(q), _ptr(scale), rows, cols, _dt(x), stream())
+    q, scale = _act8_new(x, rows, cols)
+    brk.call("brk_gelu_fwd_act8", a_x, _take("out", y, x.dtype, x.shape, device), q.data_ptr(), scale.data_ptr(), rows, cols, _dt(x), stream())
     return y, q, scale
 
 
 def gelu_backward_act8(dy, q, scale, out=None, recompute=False):
     """dy * gelu'(kept x); with recompute also gelu(kept x) again: dx, or (dx, y)."""
-    _chk(dy, out)
-    _chk_device(dy)
-    rows, cols = _rows_cols(dy)
-    _chk_all(_act8_shapes(rows, cols), q=q, scale=scale)
+    device, rows, cols, a_dy = _act8_like(dy)
+    a_q, a_scale = _act8_take(q, scale, rows, cols, device)
     dx = torch.empty_like(dy) if out is None else out
-    _chk_all({"out": (dy.dtype, dy.shape)}, out=dx)
     y = torch.empty_like(dy) if recompute else None
-    brk.call("brk_gelu_bwd_act8", _ptr(dy), _ptr(q), _ptr(scale), _ptr(dx), _ptr(y), rows, cols, _dt(dy), stream())
+    brk.call("brk_gelu_bwd_act8", a_dy, a_q, a_scale, _take("out", dx, dy.dtype, dy.shape, device), _ptr(y), rows, cols, _dt(dy), stream())
     return (dx, y) if recompute else dx
 
 
 def layernorm_act8(x, gamma, beta, eps=1e-5, out=None):
     """LayerNorm that keeps the normalised rows in 8 bits: (y, q, scale, var)."""
-    _chk(x, out)
-    _chk_device(x)
-    rows, cols = _rows_cols(x)
-    vec = (x.dtype, (cols,))
-    _chk_all({"gamma": vec, "beta": vec}, gamma=gamma, beta=beta)
+    device, rows, cols, a_x = _act8_like(x)
+    a_gamma, a_beta = _take("gamma", gamma, x.dtype, (cols,), device), _take("beta", beta, x.dtype, (cols,), device)
     y = torch.empty_like(x) if out is None else out
-    _chk_all({"out": (x.dtype, x.shape)}, out=y)
-    q, scale = _act8_new(rows, cols, x.device)
-    var = torch.empty(rows, dtype=torch.float32, device=x.device)
-    brk.call("brk_layernorm_fwd_act8", _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(q), _ptr(scale), _ptr(var), rows, cols, eps, _dt(x), stream())
+    q, scale = _act8_new(x, rows, cols)
+    var = x.new_empty((rows,), dtype=torch.float32)
+    brk.call("brk_layernorm_fwd_act8", a_x, a_gamma, a_beta, _take("out", y, x.dtype, x.shape, device), q.data_ptr(), scale.data_ptr(), var.data_ptr(), rows, cols,
+             eps, _dt(x), stream())
     return y, q, scale, var
 
 
 def layernorm_backward_act8(dy, gamma, var, q, scale, beta=None, residual=None, dgamma=None, dbeta=None, dx=None, accumulate=False, workspace=None):
     """LayerNorm backward from the kept rows: (dgamma, dbeta, dx), and with beta the forward's output again as a fourth."""
-    _chk(dy)
-    _chk_device(dy)
-    rows, cols = _rows_cols(dy)
+    device, rows, cols, a_dy = _act8_like(dy)
     if accumulate and (dgamma is None or dbeta is None):
         raise ValueError("accumulate needs dgamma and dbeta")
-    vec, full = (dy.dtype, (cols,)), (dy.dtype, dy.shape)
-    dgamma = torch.empty(cols, dtype=dy.dtype, device=dy.device) if dgamma is None else dgamma
-    dbeta = torch.empty(cols, dtype=dy.dtype, device=dy.device) if dbeta is None else dbeta
-    dx = torch.empty_like(dy) if dx is None else dx
+    dtype, vec, full = dy.dtype, (cols,), dy.shape
+    a_q, a_scale = _act8_take(q, scale, rows, cols, device)
+    a_gamma, a_beta = _take("gamma", gamma, dtype, vec, device), _take("beta", beta, dtype, vec, device)
+    if dgamma is None:
+        dgamma = torch.empty_like(gamma)
+    if dbeta is None:
+        dbeta = torch.empty_like(gamma)
+    if dx is None:
+        dx = torch.empty_like(dy)
     y = torch.empty_like(dy) if beta is not None else None
-    _chk_all({"gamma": vec, "beta": vec, "dgamma": vec, "dbeta": vec, "var": (torch.float32, (rows,)), "residual": full, "dx": full, **_act8_shapes(rows, cols)},
-             gamma=gamma, beta=beta, dgamma=dgamma, dbeta=dbeta, var=var, residual=residual, dx=dx, q=q, scale=scale)
-    need = brk.lib().brk_layernorm_bwd_act8_workspace_bytes(rows, cols)
     if workspace is None:
-        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dy.device)
-    _chk(workspace)
-    _chk_device(workspace)
-    brk.call("brk_layernorm_bwd_act8", _ptr(dy), _ptr(gamma), _ptr(beta), _ptr(var), _ptr(q), _ptr(scale), _ptr(residual), _ptr(dgamma), _ptr(dbeta), _ptr(dx),
-             _ptr(y), rows, cols, _ptr(workspace), workspace.numel() * workspace.element_size(), int(accumulate), _dt(dy), stream())
+        workspace = dy.new_empty((max(brk.lib().brk_layernorm_bwd_act8_workspace_bytes(rows, cols), 16),), dtype=torch.uint8)
+    a_ws = _take("workspace", workspace, workspace.dtype, workspace.shape, device)
+    brk.call("brk_layernorm_bwd_act8", a_dy, a_gamma, a_beta, _take("var", var, torch.float32, (rows,), device), a_q, a_scale,
+             _take("residual", residual, dtype, full, device), _take("dgamma", dgamma, dtype, vec, device), _take("dbeta", dbeta, dtype, vec, device),
+             _take("dx", dx, dtype, full, device), _ptr(y), rows, cols, a_ws, workspace.numel() * workspace.element_size(), int(accumulate), _dt(dy), stream())
     return (dgamma, dbeta, dx) if y is None else (dgamma, dbeta, dx, y)
 
 

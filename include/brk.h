@@ -310,7 +310,7 @@ BRK_API int brk_doc_attn_status(void);
  * bloomz-7b/train.words:10-135).  Each block of 128 columns of a row (the last may be shorter) has one scale:
  *     top = largest magnitude of the block,  q = rint(x * 127 / top),  scale = top / 127,  kept value = q * scale
  * q [rows, cols] int8, scale [rows, ceil(cols / 128)] fp32.  A block with an infinity or a NaN gets the scale NaN (all of
- * it reads NaN); one whose largest magnitude is below 2^-119 is kept as zeros.  Any cols; cols a multiple of 16 (LayerNorm: 8
+ * it reads NaN); one whose largest magnitude is below 2^-119 is kept as zeros.  Any cols; cols a multiple of 16 (LayerNorm:
  * and at most 8192) with 16-byte aligned pointers takes the wide paths.  `dtype` is the storage type of all other tensors. */
 BRK_API int brk_act8_pack(const void* x, int8_t* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream);
 BRK_API int brk_act8_unpack(const int8_t* q, const float* scale, void* out, int64_t rows, int64_t cols, int dtype, void* stream);
