@@ -324,12 +324,73 @@ static int a8_unpack(const int8_t* q, const float* scale, const void* dy, void* 
 }
 
 // ---- LayerNorm ---------------------------------------------------------------------------------------------------------
-// A thread owns 16 columns, so 8 neighbouring lanes are a block of 128; a row is owned by a team of `team` threads (a
-// multiple of 32, at most 512: rows of up to 8192 columns), and a CTA holds blockDim.x / team teams that meet at named
-// barriers of their own and never wait for one another.  Rows are fetched ahead into registers, still packed: the two
-// reductions of a row leave the memory system idle otherwise (without the fetch ahead [8192, 4096] fp16 took 61 us forward).
+// A thread owns two groups of 8 columns, so 16 neighbouring lanes are a block of 128; a row is owned by a team of `team`
+// threads (a multiple of 32, at most 512: rows of up to 8192 columns), thread t with columns 8 t and 8 (team + t), and a CTA
+// holds blockDim.x / team teams that meet at named barriers of their own and never wait for one another.  Every thread copies
+// its own packets of the next rows into slots of its own with cp.async, several rows ahead and without a barrier: the two
+// reductions of a row leave the memory system idle otherwise, and registers hold one row ahead at most ([8192, 4096] fp16
+// backward: 85 us with one row ahead in registers).
 constexpr int A8_LN_MAX_COLS = 8192;
 constexpr int A8_LN_THREADS = 512;
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+    const uint32_t a = (uint32_t)__cvta_generic_to_shared(to);
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(a), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// 8 columns of storage type T
+template <typename T>
+struct Group8 {
+    static constexpr int N = 8 / Vec<T>::N;          // 16-byte packets
+    // slot p of a stage lies at [p][thread]
+    static __device__ __forceinline__ void fetch(uint4* slot, int threads, const T* from) {
+#pragma unroll
+        for (int i = 0; i < N; i++) copy_async<16>(slot + i * threads, from + i * Vec<T>::N);
+    }
+    static __device__ __forceinline__ void read(const uint4* slot, int threads, float2* o) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            Vec<T> x;
+            x.unpack(slot[i * threads]);
+#pragma unroll
+            for (int e = 0; e < Vec<T>::N; e += 2) o[(i * Vec<T>::N + e) / 2] = make_float2(x.v[e], x.v[e + 1]);
+        }
+    }
+    static __device__ __forceinline__ void write(T* to, const float2* x) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            Vec<T> v;
+#pragma unroll
+            for (int e = 0; e < Vec<T>::N; e += 2) {
+                v.v[e] = x[(i * Vec<T>::N + e) / 2].x;
+                v.v[e + 1] = x[(i * Vec<T>::N + e) / 2].y;
+            }
+            v.store_stream(to + i * Vec<T>::N);
+        }
+    }
+    static __device__ __forceinline__ void load(const T* from, float2* o) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            Vec<T> x;
+            x.load(from + i * Vec<T>::N);
+#pragma unroll
+            for (int e = 0; e < Vec<T>::N; e += 2) o[(i * Vec<T>::N + e) / 2] = make_float2(x.v[e], x.v[e + 1]);
+        }
+    }
+};
+__device__ __forceinline__ void a8_unpack8(const uint2& w, float scale, float2* o) {
+    const uint32_t x[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        o[2 * i] = __fmul2_rn(a8_bytes<0>(x[i]), both(scale));
+        o[2 * i + 1] = __fmul2_rn(a8_bytes<2>(x[i]), both(scale));
+    }
+}
 
 __device__ __forceinline__ void team_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
@@ -355,84 +416,106 @@ __device__ __forceinline__ float2 team_sum2(float a, float b, float2* red, int i
 }
 
 // gamma and beta wait in shared memory, in fp32: unpacking them again for every row took a quarter of the instructions.
+template <typename T>
+struct LnFwdSmem {
+    static constexpr int STAGES = 4;
+    static constexpr size_t PER_THREAD = STAGES * 16 * sizeof(T), PER_MEMBER = 32 * sizeof(float);       // a thread; a member of a team
+};
 template <typename T, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS)
 a8_ln_fwd_kernel(const T* x, const T* __restrict__ gamma, const T* __restrict__ beta, T* y, int8_t* __restrict__ q,
                  float* __restrict__ scale, float* __restrict__ var, int64_t rows, int cols, float eps, int team) {
-    extern __shared__ __align__(16) float affine[];         // gamma [16 * team], beta [16 * team]
+    using G = Group8<T>;
+    constexpr int STAGES = LnFwdSmem<T>::STAGES;
+    extern __shared__ __align__(16) unsigned char ln_smem[];
     __shared__ float red[2][THREADS / 32];                  // [buffer][warp of the CTA]: a team uses its own warps' cells
-    const int tid = threadIdx.x % team, group = threadIdx.x / team, groups = blockDim.x / team;
-    const int c = tid * 16, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
-    const bool live = c < cols;
+    const int threads = blockDim.x;
+    const int tid = threadIdx.x % team, group = threadIdx.x / team, groups = threads / team;
+    const int c0 = tid * 8, c1 = (team + tid) * 8, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
+    const bool live0 = c0 < cols, live1 = c1 < cols;
     const float inv_n = 1.0f / (float)cols;
     float* r0 = red[0] + group * (team >> 5);
     float* r1 = red[1] + group * (team >> 5);
-    // column c + 4 i of thread t lies at [i][t]: neighbouring threads read neighbouring 16 bytes
-    float4* const ga = reinterpret_cast<float4*>(affine) + tid;
-    float4* const be = ga + 4 * team;
-    if (group == 0 && live) {
-        Pack16<T> raw;
-        float2 v[8];
-        raw.load(gamma + c);
-        raw.to(v);
+    uint4* const slots = reinterpret_cast<uint4*>(ln_smem) + threadIdx.x;                          // [stage][group of columns][packet][thread]
+    float2* const ga = reinterpret_cast<float2*>(ln_smem + (size_t)threads * LnFwdSmem<T>::PER_THREAD) + tid;       // gamma [8][member], beta [8][member]
+    float2* const be = ga + 8 * team;
+    if (group == 0) {
+        float2 v[8] = {};
+        if (live0) G::load(gamma + c0, v);
+        if (live1) G::load(gamma + c1, v + 4);
 #pragma unroll
-        for (int i = 0; i < 4; i++) ga[i * team] = make_float4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y);
-        raw.load(beta + c);
-        raw.to(v);
+        for (int e = 0; e < 8; e++) ga[e * team] = v[e];
+        if (live0) G::load(beta + c0, v);
+        if (live1) G::load(beta + c1, v + 4);
 #pragma unroll
-        for (int i = 0; i < 4; i++) be[i * team] = make_float4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y);
+        for (int e = 0; e < 8; e++) be[e * team] = v[e];
     }
+    for (int i = 0; i < STAGES * 2 * G::N; i++)              // columns beyond the last stay zero
+        if (!((i / G::N) & 1 ? live1 : live0)) slots[i * threads] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     pdl_wait();
-    Pack16<T> ahead[2] = {};
     const int64_t step = (int64_t)gridDim.x * groups;
     int64_t row = (int64_t)blockIdx.x * groups + group;
-    if (live && row < rows) ahead[0].stream(x + row * cols + c);
-    if (live && row + step < rows) ahead[1].stream(x + (row + step) * cols + c);
-    for (; row < rows; row += step) {
+    auto fetch = [&](int64_t at, int stage) {
+        if (at < rows) {
+            uint4* slot = slots + stage * 2 * G::N * threads;
+            if (live0) G::fetch(slot, threads, x + at * cols + c0);
+            if (live1) G::fetch(slot + G::N * threads, threads, x + at * cols + c1);
+        }
+        copy_commit();
+    };
+    for (int i = 0; i < STAGES - 1; i++) fetch(row + i * step, i);
+    for (int stage = 0; row < rows; row += step, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+        copy_wait<STAGES - 2>();
+        fetch(row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
         float2 v[8];
-        ahead[0].to(v);                                     // zeros beyond the last column
-        ahead[0] = ahead[1];
-        if (live && row + 2 * step < rows) ahead[1].stream(x + (row + 2 * step) * cols + c);
+        const uint4* slot = slots + stage * 2 * G::N * threads;
+        G::read(slot, threads, v);
+        G::read(slot + G::N * threads, threads, v + 4);
         float2 s = v[0];
 #pragma unroll
         for (int e = 1; e < 8; e++) s = __fadd2_rn(s, v[e]);
         const float mu = team_sum(s.x + s.y, r0, group + 1, team) * inv_n;
-        float2 d2 = both(0.0f);
-        if (live) {
+        float2 d2[2] = {both(0.0f), both(0.0f)};
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[e] = __fadd2_rn(v[e], both(-mu));
-                d2 = __ffma2_rn(v[e], v[e], d2);
-            }
+        for (int e = 0; e < 8; e++) {
+            v[e] = __fadd2_rn(v[e], both(-mu));
+            if (e < 4 ? live0 : live1) d2[e & 1] = __ffma2_rn(v[e], v[e], d2[e & 1]);
         }
-        const float va = fmaf(team_sum(d2.x + d2.y, r1, group + 1, team), inv_n, eps);
+        d2[0] = __fadd2_rn(d2[0], d2[1]);
+        const float va = fmaf(team_sum(d2[0].x + d2[0].y, r1, group + 1, team), inv_n, eps);
         const float rstd = rsqrtf(va);
-        float top = 0.0f;
-        if (live) {
+        float top[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[e] = __fmul2_rn(v[e], both(rstd));
-                top = max3(top, fabsf(v[e].x), fabsf(v[e].y));
-            }
+        for (int e = 0; e < 8; e++) {
+            v[e] = __fmul2_rn(v[e], both(rstd));
+            top[e >> 2] = max3(top[e >> 2], fabsf(v[e].x), fabsf(v[e].y));
         }
+        if (!live0) top[0] = 0.0f;
+        if (!live1) top[1] = 0.0f;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (live) {
-            // a value that is not finite makes the row's variance so, and every normalised value with it
-            const A8Scale sc = a8_scale(va < INFINITY ? __float_as_uint(top) : 0x7fffffffu);
-            __stcs(reinterpret_cast<uint4*>(q + row * cols + c), a8_pack16(v, sc.inv));
-            if ((threadIdx.x & 7) == 0) scale[row * blocks + (c >> 7)] = sc.scale;
+        for (int o = 8; o > 0; o >>= 1) {
+            top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+            top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+        }
+        // a value that is not finite makes the row's variance so, and every normalised value with it
+        const bool finite = va < INFINITY;
+        const int64_t at = row * cols;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float4 g = ga[i * team], b = be[i * team];
-                v[2 * i] = __ffma2_rn(v[2 * i], make_float2(g.x, g.y), make_float2(b.x, b.y));
-                v[2 * i + 1] = __ffma2_rn(v[2 * i + 1], make_float2(g.z, g.w), make_float2(b.z, b.w));
-            }
-            store16(y + row * cols + c, v);
+        for (int k = 0; k < 2; k++) {
+            const int c = k ? c1 : c0;
+            if (!(k ? live1 : live0)) continue;
+            const A8Scale sc = a8_scale(finite ? __float_as_uint(top[k]) : 0x7fffffffu);
+            __stcs(reinterpret_cast<uint2*>(q + at + c), make_uint2(a8_pack4(v[4 * k], v[4 * k + 1], sc.inv), a8_pack4(v[4 * k + 2], v[4 * k + 3], sc.inv)));
+            if ((threadIdx.x & 15) == 0) scale[row * blocks + (c >> 7)] = sc.scale;
+            float2 o[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = __ffma2_rn(v[4 * k + e], ga[(4 * k + e) * team], be[(4 * k + e) * team]);
+            G::write(y + at + c, o);
         }
         if (tid == 0) var[row] = va;
     }
+    copy_wait<0>();
     pdl_launch_dependents();
 }
 
@@ -483,120 +566,147 @@ a8_ln_fwd_generic_kernel(const T* x, const T* gamma, const T* beta, T* y, int8_t
 // Backward.  g = dy * gamma;  dx = rstd * (g - mean(g) - xhat * mean(g * xhat)) (+ residual);  the column sums of
 // dy * xhat and dy stay in the registers of the column's owner over all rows of the CTA, are added over the CTA's teams
 // through shared memory and leave as one row of `part` [gridDim.x][2][cols], which a second kernel adds in order.
-// The next row's packets are fetched before this row's barrier, so a row's latency passes behind the row before it; what is
-// needed on both sides of the barrier is unpacked twice rather than held in 32 bits, which would not fit the registers.
+// What is needed on both sides of the barrier is unpacked twice rather than held in 32 bits, which would not fit the registers.
+template <typename T, bool RES>
+struct LnBwdSmem {
+    static constexpr int STAGES = sizeof(T) == 2 ? 4 : 2;          // what 227 KB hold of 512 threads' packets
+    static constexpr int PACKETS = (RES ? 2 : 1) * 2 * Group8<T>::N;       // dy, residual; then 8 bytes of q and a scale for each group
+    static constexpr size_t PER_THREAD = STAGES * (PACKETS * 16 + 2 * 8 + 2 * 4);
+};
 template <typename T, bool RES, bool AGAIN>
 __global__ void __launch_bounds__(A8_LN_THREADS, 1)
 a8_ln_bwd_kernel(const T* dy, const T* __restrict__ gamma, const T* __restrict__ beta, const float* __restrict__ var,
                  const int8_t* __restrict__ q, const float* __restrict__ scale, const T* residual, T* dx, T* __restrict__ y,
                  float* __restrict__ part, int64_t rows, int cols, int team) {
-    extern __shared__ float fold[];          // [teams - 1][2][cols]
+    using G = Group8<T>;
+    using S = LnBwdSmem<T, RES>;
+    extern __shared__ __align__(16) unsigned char ln_smem[];
     __shared__ float2 red[2][A8_LN_THREADS / 32];
-    const int tid = threadIdx.x % team, group = threadIdx.x / team, groups = blockDim.x / team;
-    const int c = tid * 16, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
-    const bool live = c < cols;
+    const int threads = blockDim.x;
+    const int tid = threadIdx.x % team, group = threadIdx.x / team, groups = threads / team;
+    const int c0 = tid * 8, c1 = (team + tid) * 8, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
+    const bool live0 = c0 < cols, live1 = c1 < cols;
     const float inv_n = 1.0f / (float)cols;
     float2* r0 = red[0] + group * (team >> 5);
     float2* r1 = red[1] + group * (team >> 5);
-    float2 dg[8], db[8];
+    uint4* const packets = reinterpret_cast<uint4*>(ln_smem) + threadIdx.x;                                                   // [stage][packet][thread]
+    uint2* const bytes = reinterpret_cast<uint2*>(ln_smem + (size_t)threads * S::STAGES * S::PACKETS * 16) + threadIdx.x;       // [stage][group][thread]
+    float* const scales = reinterpret_cast<float*>(ln_smem + (size_t)threads * S::STAGES * (S::PACKETS * 16 + 16)) + threadIdx.x;
+    float2 dg[8], db[8], ga[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) dg[e] = db[e] = both(0.0f);
-    Pack16<T> gam = {}, bet = {};
-    if (live) {
-        gam.load(gamma + c);
-        if (AGAIN) bet.load(beta + c);
+    for (int e = 0; e < 8; e++) dg[e] = db[e] = ga[e] = both(0.0f);
+    if (live0) G::load(gamma + c0, ga);
+    if (live1) G::load(gamma + c1, ga + 4);
+    for (int i = 0; i < S::STAGES * S::PACKETS; i++)          // columns beyond the last stay zero
+        if (!((i / G::N) & 1 ? live1 : live0)) packets[i * threads] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < S::STAGES * 2; i++) {
+        if (i & 1 ? live1 : live0) continue;
+        bytes[i * threads] = make_uint2(0, 0);
+        scales[i * threads] = 0.0f;
     }
     pdl_wait();
 
-    Pack16<T> n_dy = {}, n_res = {};
-    uint4 n_q = make_uint4(0, 0, 0, 0);
-    float n_scale = 0.0f, n_var = 1.0f;
-    auto fetch = [&](int64_t row) {
-        if (live) {
-            const int64_t at = row * cols + c;
-            n_dy.stream(dy + at);
-            if (RES) n_res.stream(residual + at);
-            n_q = __ldcs(reinterpret_cast<const uint4*>(q + at));
-            n_scale = scale[row * blocks + (c >> 7)];
-        }
-        n_var = var[row];
-    };
     const int64_t step = (int64_t)gridDim.x * groups;
     int64_t row = (int64_t)blockIdx.x * groups + group;
-    if (row < rows) fetch(row);
-    for (int turn = 0; row < rows; row += step, turn ^= 1) {
-        const Pack16<T> p_dy = n_dy, p_res = n_res;
-        const uint4 w = n_q;
-        const float sc = n_scale, rstd = rsqrtf(n_var);
-        if (row + step < rows) fetch(row + step);
-        float2 a = both(0.0f), b = both(0.0f);
-        {
-            float2 xh[8], d[8], ga[8];
-            a8_unpack16(w, sc, xh);
-            p_dy.to(d);
-            gam.to(ga);
+    auto fetch = [&](int64_t r, int stage) {
+        if (r < rows) {
+            const int64_t at = r * cols;
+            uint4* slot = packets + stage * S::PACKETS * threads;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                dg[e] = __ffma2_rn(d[e], xh[e], dg[e]);
-                db[e] = __fadd2_rn(db[e], d[e]);
-                const float2 g = __fmul2_rn(d[e], ga[e]);
-                a = __fadd2_rn(a, g);
-                b = __ffma2_rn(g, xh[e], b);
+            for (int k = 0; k < 2; k++) {
+                const int c = k ? c1 : c0;
+                if (!(k ? live1 : live0)) continue;
+                G::fetch(slot + k * G::N * threads, threads, dy + at + c);
+                if (RES) G::fetch(slot + (2 + k) * G::N * threads, threads, residual + at + c);
+                copy_async<8>(bytes + (stage * 2 + k) * threads, q + at + c);
+                copy_async<4>(scales + (stage * 2 + k) * threads, scale + r * blocks + (c >> 7));
             }
         }
+        copy_commit();
+    };
+    for (int i = 0; i < S::STAGES - 1; i++) fetch(row + i * step, i);
+    float n_var = row < rows ? var[row] : 1.0f;
+    for (int stage = 0, turn = 0; row < rows; row += step, turn ^= 1, stage = stage + 1 == S::STAGES ? 0 : stage + 1) {
+        copy_wait<S::STAGES - 2>();
+        fetch(row + (S::STAGES - 1) * step, stage == 0 ? S::STAGES - 1 : stage - 1);
+        const float rstd = rsqrtf(n_var);
+        if (row + step < rows) n_var = var[row + step];
+        const uint4* slot = packets + stage * S::PACKETS * threads;
+        const uint2 w0 = bytes[stage * 2 * threads], w1 = bytes[(stage * 2 + 1) * threads];
+        const float s0 = scales[stage * 2 * threads], s1 = scales[(stage * 2 + 1) * threads];
+        float2 a = both(0.0f), b = both(0.0f), g[8], xh[8];
+        G::read(slot, threads, g);
+        G::read(slot + G::N * threads, threads, g + 4);
+        a8_unpack8(w0, s0, xh);
+        a8_unpack8(w1, s1, xh + 4);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            dg[e] = __ffma2_rn(g[e], xh[e], dg[e]);
+            db[e] = __fadd2_rn(db[e], g[e]);
+            g[e] = __fmul2_rn(g[e], ga[e]);
+            a = __fadd2_rn(a, g[e]);
+            b = __ffma2_rn(g[e], xh[e], b);
+        }
         const float2 m = team_sum2(a.x + a.y, b.x + b.y, turn ? r1 : r0, group + 1, team);
-        if (live) {
-            const float2 mg = both(-rstd * m.x * inv_n), mgx = both(-rstd * m.y * inv_n);
-            const int64_t at = row * cols + c;
-            float2 xh[8], o[8], ga[8];
-            a8_unpack16(w, sc, xh);
-            p_dy.to(o);
-            gam.to(ga);
+        const float2 mg = both(-rstd * m.x * inv_n), mgx = both(-rstd * m.y * inv_n);
+        const int64_t at = row * cols;
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = __ffma2_rn(xh[e], mgx, __ffma2_rn(__fmul2_rn(o[e], ga[e]), both(rstd), mg));
+        for (int k = 0; k < 2; k++) {
+            const int c = k ? c1 : c0;
+            if (!(k ? live1 : live0)) continue;
+            float2 o[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = __ffma2_rn(xh[4 * k + e], mgx, __ffma2_rn(g[4 * k + e], both(rstd), mg));
             if (RES) {
-                float2 r[8];
-                p_res.to(r);
+                float2 r[4];
+                G::read(slot + (2 + k) * G::N * threads, threads, r);
 #pragma unroll
-                for (int e = 0; e < 8; e++) o[e] = __fadd2_rn(o[e], r[e]);
+                for (int e = 0; e < 4; e++) o[e] = __fadd2_rn(o[e], r[e]);
             }
-            store16(dx + at, o);
+            G::write(dx + at + c, o);
             if (AGAIN) {
-                float2 be[8];
-                bet.to(be);
+                float2 be[4];
+                G::load(beta + c, be);                     // the same for every row: in the first-level cache
 #pragma unroll
-                for (int e = 0; e < 8; e++) o[e] = __ffma2_rn(xh[e], ga[e], be[e]);
-                store16(y + at, o);
+                for (int e = 0; e < 4; e++) o[e] = __ffma2_rn(xh[4 * k + e], ga[4 * k + e], be[e]);
+                G::write(y + at + c, o);
             }
         }
     }
+    copy_wait<0>();
+    float* const fold = reinterpret_cast<float*>(ln_smem);          // [teams - 1][2][8 pairs][member]: the slots are done with
     if (groups > 1) {
-        if (group > 0 && live) {
-            float2* f = reinterpret_cast<float2*>(fold + (int64_t)(group - 1) * 2 * cols + c);
+        __syncthreads();
+        float2* const mine = reinterpret_cast<float2*>(fold) + tid;
+        if (group > 0) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                f[e] = dg[e];
-                f[cols / 2 + e] = db[e];
+                mine[((group - 1) * 16 + e) * team] = dg[e];
+                mine[((group - 1) * 16 + 8 + e) * team] = db[e];
             }
         }
         __syncthreads();
-        if (group == 0 && live) {
+        if (group == 0) {
             for (int k = 0; k < groups - 1; k++) {
-                const float2* f = reinterpret_cast<const float2*>(fold + (int64_t)k * 2 * cols + c);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    dg[e] = __fadd2_rn(dg[e], f[e]);
-                    db[e] = __fadd2_rn(db[e], f[cols / 2 + e]);
+                    dg[e] = __fadd2_rn(dg[e], mine[(k * 16 + e) * team]);
+                    db[e] = __fadd2_rn(db[e], mine[(k * 16 + 8 + e) * team]);
                 }
             }
         }
     }
-    if (group == 0 && live) {
-        float* p = part + (int64_t)blockIdx.x * 2 * cols + c;
+    if (group == 0) {
+        float* const p = part + (int64_t)blockIdx.x * 2 * cols;
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            *reinterpret_cast<float4*>(p + 2 * e) = make_float4(dg[e].x, dg[e].y, dg[e + 1].x, dg[e + 1].y);
-            *reinterpret_cast<float4*>(p + cols + 2 * e) = make_float4(db[e].x, db[e].y, db[e + 1].x, db[e + 1].y);
+        for (int k = 0; k < 2; k++) {
+            const int c = k ? c1 : c0;
+            if (!(k ? live1 : live0)) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                *reinterpret_cast<float4*>(p + c + 2 * e) = make_float4(dg[4 * k + e].x, dg[4 * k + e].y, dg[4 * k + e + 1].x, dg[4 * k + e + 1].y);
+                *reinterpret_cast<float4*>(p + cols + c + 2 * e) = make_float4(db[4 * k + e].x, db[4 * k + e].y, db[4 * k + e + 1].x, db[4 * k + e + 1].y);
+            }
         }
     }
     pdl_launch_dependents();
@@ -659,6 +769,11 @@ a8_ln_reduce_kernel(const float* part, T* dgamma, T* dbeta, int parts, int cols,
 // threads that own a row of `cols` columns, 16 each
 static int a8_team(int64_t cols) { return (int)((cols + 511) / 512) * 32; }
 
+// more than the 48 KB of dynamic shared memory that need no leave
+static cudaError_t a8_allow_smem(const void* kernel, size_t bytes) {
+    return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
+}
+
 constexpr int A8_MAX_PARTS = 256;             // partial rows of the LayerNorm backward: one per CTA
 
 template <typename T>
@@ -666,13 +781,12 @@ static int a8_ln_fwd(const void* x, const void* gamma, const void* beta, void* y
                      float eps, cudaStream_t st) {
     if (cols % 16 == 0 && cols <= A8_LN_MAX_COLS && aligned16(x) && aligned16(gamma) && aligned16(beta) && aligned16(y) && aligned16(q)) {
         const int team = a8_team(cols), groups = team >= 256 ? 1 : 256 / team;
-        // as many CTAs as are resident at once; long rows need all of an SM's registers for one team
-        const int ctas = team > 256 ? 1 : 3;
+        // as many CTAs as are resident at once
+        const int ctas = team > 256 ? 1 : sizeof(T) == 2 ? 3 : 2;
         const int64_t want = (rows + groups - 1) / groups, cap = (int64_t)sm_count() * ctas;
         const int grid = (int)(want < cap ? want : cap);
-        const size_t smem = (size_t)team * 32 * sizeof(float);
-        cudaError_t e = cudaSuccess;
-        if (smem > 48 * 1024) e = cudaFuncSetAttribute(a8_ln_fwd_kernel<T, 512, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const size_t smem = (size_t)team * groups * LnFwdSmem<T>::PER_THREAD + (size_t)team * LnFwdSmem<T>::PER_MEMBER;
+        cudaError_t e = a8_allow_smem(team > 256 ? (const void*)a8_ln_fwd_kernel<T, 512, 1> : (const void*)a8_ln_fwd_kernel<T, 256, 3>, smem);
         if (e != cudaSuccess) {
             set_cuda_error(e, "a8_ln_fwd smem attribute");
             return BRK_CUDA_ERROR;
@@ -693,12 +807,13 @@ static int a8_ln_fwd(const void* x, const void* gamma, const void* beta, void* y
 }
 
 template <typename T, bool RES, bool AGAIN>
-static cudaError_t a8_launch_ln_bwd(int grid, int block, size_t smem, cudaStream_t st, const T* dy, const T* gamma, const T* beta, const float* var,
+static cudaError_t a8_launch_ln_bwd(int grid, int block, cudaStream_t st, const T* dy, const T* gamma, const T* beta, const float* var,
                                     const int8_t* q, const float* scale, const T* residual, T* dx, T* y, float* part, int64_t rows, int cols, int team) {
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(a8_ln_bwd_kernel<T, RES, AGAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
+    const size_t smem = (size_t)block * LnBwdSmem<T, RES>::PER_THREAD;
+    static_assert(A8_LN_THREADS * LnBwdSmem<T, RES>::PER_THREAD <= 230000, "the slots must fit the 227 KB a CTA can have");
+    static_assert(LnBwdSmem<T, RES>::PER_THREAD >= 128, "a team's column sums are folded in its slots");
+    const cudaError_t e = a8_allow_smem((const void*)a8_ln_bwd_kernel<T, RES, AGAIN>, smem);
+    if (e != cudaSuccess) return e;
     return launch_pdl(a8_ln_bwd_kernel<T, RES, AGAIN>, grid, block, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, cols, team);
 }
 
@@ -717,14 +832,13 @@ static int a8_ln_bwd(const void* dy_, const void* gamma_, const void* beta_, con
         const int64_t want = (rows + groups - 1) / groups;
         int grid = sm_count() < A8_MAX_PARTS ? sm_count() : A8_MAX_PARTS;
         if (want < grid) grid = (int)want;
-        const size_t smem = (size_t)(groups - 1) * 2 * cols * sizeof(float);
         cudaError_t e;
         if (residual)
-            e = y ? a8_launch_ln_bwd<T, true, true>(grid, team * groups, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team)
-                  : a8_launch_ln_bwd<T, true, false>(grid, team * groups, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team);
+            e = y ? a8_launch_ln_bwd<T, true, true>(grid, team * groups, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team)
+                  : a8_launch_ln_bwd<T, true, false>(grid, team * groups, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team);
         else
-            e = y ? a8_launch_ln_bwd<T, false, true>(grid, team * groups, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team)
-                  : a8_launch_ln_bwd<T, false, false>(grid, team * groups, smem, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team);
+            e = y ? a8_launch_ln_bwd<T, false, true>(grid, team * groups, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team)
+                  : a8_launch_ln_bwd<T, false, false>(grid, team * groups, st, dy, gamma, beta, var, q, scale, residual, dx, y, part, rows, (int)cols, team);
         if (e != cudaSuccess) {
             set_cuda_error(e, "a8_ln_bwd_kernel");
             return BRK_CUDA_ERROR;
