@@ -31,6 +31,9 @@ __device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x
 struct A8Scale {
     float inv, scale;
 };
+// EXACT: the quotient correctly rounded, for inputs whose ratios to the block's largest are simple fractions (halves of it
+// lie between two steps); normalised rows have none, and a rounding of 2^-22 there saves 20 instructions a block.
+template <bool EXACT = true>
 __device__ __forceinline__ A8Scale a8_scale(uint32_t top_bits) {
     A8Scale s;
     const float top = __uint_as_float(top_bits);
@@ -41,7 +44,7 @@ __device__ __forceinline__ A8Scale a8_scale(uint32_t top_bits) {
         s.inv = 0.0f;
         s.scale = 0.0f;
     } else {
-        s.inv = __fdiv_rn(127.0f, top);
+        s.inv = EXACT ? __fdiv_rn(127.0f, top) : __fdividef(127.0f, top);
         s.scale = top * (1.0f / 127.0f);
     }
     return s;
@@ -324,8 +327,8 @@ static int a8_unpack(const int8_t* q, const float* scale, const void* dy, void* 
 }
 
 // ---- LayerNorm ---------------------------------------------------------------------------------------------------------
-// A thread owns two groups of 8 columns, so 16 neighbouring lanes are a block of 128; a row is owned by a team of `team`
-// threads (a multiple of 32, at most 512: rows of up to 8192 columns), thread t with columns 8 t and 8 (team + t), and a CTA
+// A thread owns groups of 8 columns, so 16 neighbouring lanes are a block of 128; a row (of up to 8192 columns) is owned by
+// a team of `team` threads, a multiple of 32, thread t with the columns from 8 t, 8 (team + t) and so on, and a CTA
 // holds blockDim.x / team teams that meet at named barriers of their own and never wait for one another.  Every thread copies
 // its own packets of the next rows into slots of its own with cp.async, several rows ahead and without a barrier: the two
 // reductions of a row leave the memory system idle otherwise, and registers hold one row ahead at most ([8192, 4096] fp16
@@ -415,52 +418,60 @@ __device__ __forceinline__ float2 team_sum2(float a, float b, float2* red, int i
     return make_float2(warp_sum(t.x), warp_sum(t.y));
 }
 
-// gamma and beta wait in shared memory, in fp32: unpacking them again for every row took a quarter of the instructions.
+// Forward: a thread owns four groups of 8 columns (8 (k * team + t) on), which halves what the reductions cost an element
+// against two.  gamma and beta wait in shared memory, in fp32: unpacking them for every row took a quarter of the time.
 template <typename T>
-struct LnFwdSmem {
-    static constexpr int STAGES = 4;
-    static constexpr size_t PER_THREAD = STAGES * 16 * sizeof(T), PER_MEMBER = 32 * sizeof(float);       // a thread; a member of a team
+struct LnFwd {
+    static constexpr int K = 4, STAGES = 4, THREADS = 256;
+    static constexpr int CTAS = sizeof(T) == 2 ? 2 : 1;             // resident on an SM
+    static constexpr size_t PER_THREAD = STAGES * K * 8 * sizeof(T), PER_MEMBER = 2 * K * 8 * sizeof(float);       // bytes of a thread; of a member of a team
 };
-template <typename T, int THREADS, int CTAS>
-__global__ void __launch_bounds__(THREADS, CTAS)
+template <typename T>
+__global__ void __launch_bounds__(256, LnFwd<T>::CTAS)
 a8_ln_fwd_kernel(const T* x, const T* __restrict__ gamma, const T* __restrict__ beta, T* y, int8_t* __restrict__ q,
                  float* __restrict__ scale, float* __restrict__ var, int64_t rows, int cols, float eps, int team) {
     using G = Group8<T>;
-    constexpr int STAGES = LnFwdSmem<T>::STAGES;
+    constexpr int STAGES = LnFwd<T>::STAGES, K = LnFwd<T>::K, E = 4 * K;       // E: pairs of columns
     extern __shared__ __align__(16) unsigned char ln_smem[];
-    __shared__ float red[2][THREADS / 32];                  // [buffer][warp of the CTA]: a team uses its own warps' cells
+    __shared__ float red[2][LnFwd<T>::THREADS / 32];        // [buffer][warp of the CTA]: a team uses its own warps' cells
     const int threads = blockDim.x;
     const int tid = threadIdx.x % team, group = threadIdx.x / team, groups = threads / team;
-    const int c0 = tid * 8, c1 = (team + tid) * 8, blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
-    const bool live0 = c0 < cols, live1 = c1 < cols;
+    const int blocks = (cols + A8_BLOCK - 1) / A8_BLOCK;
+    const int c0 = tid * 8, cstep = team * 8;
     const float inv_n = 1.0f / (float)cols;
     float* r0 = red[0] + group * (team >> 5);
     float* r1 = red[1] + group * (team >> 5);
     uint4* const slots = reinterpret_cast<uint4*>(ln_smem) + threadIdx.x;                          // [stage][group of columns][packet][thread]
-    float2* const ga = reinterpret_cast<float2*>(ln_smem + (size_t)threads * LnFwdSmem<T>::PER_THREAD) + tid;       // gamma [8][member], beta [8][member]
-    float2* const be = ga + 8 * team;
+    float2* const ga = reinterpret_cast<float2*>(ln_smem + (size_t)threads * LnFwd<T>::PER_THREAD) + tid;       // gamma [E][member], beta [E][member]
+    float2* const be = ga + E * team;
     if (group == 0) {
-        float2 v[8] = {};
-        if (live0) G::load(gamma + c0, v);
-        if (live1) G::load(gamma + c1, v + 4);
 #pragma unroll
-        for (int e = 0; e < 8; e++) ga[e * team] = v[e];
-        if (live0) G::load(beta + c0, v);
-        if (live1) G::load(beta + c1, v + 4);
+        for (int k = 0; k < K; k++) {
+            float2 g[4] = {}, b[4] = {};
+            if (c0 + k * cstep < cols) {
+                G::load(gamma + c0 + k * cstep, g);
+                G::load(beta + c0 + k * cstep, b);
+            }
 #pragma unroll
-        for (int e = 0; e < 8; e++) be[e * team] = v[e];
+            for (int e = 0; e < 4; e++) {
+                ga[(4 * k + e) * team] = g[e];
+                be[(4 * k + e) * team] = b[e];
+            }
+        }
     }
-    for (int i = 0; i < STAGES * 2 * G::N; i++)              // columns beyond the last stay zero
-        if (!((i / G::N) & 1 ? live1 : live0)) slots[i * threads] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < STAGES * K * G::N; i++)              // columns beyond the last stay zero
+        if (c0 + (i / G::N) % K * cstep >= cols) slots[i * threads] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     pdl_wait();
     const int64_t step = (int64_t)gridDim.x * groups;
     int64_t row = (int64_t)blockIdx.x * groups + group;
     auto fetch = [&](int64_t at, int stage) {
         if (at < rows) {
-            uint4* slot = slots + stage * 2 * G::N * threads;
-            if (live0) G::fetch(slot, threads, x + at * cols + c0);
-            if (live1) G::fetch(slot + G::N * threads, threads, x + at * cols + c1);
+            const T* from = x + at * cols;
+            uint4* slot = slots + stage * K * G::N * threads;
+#pragma unroll
+            for (int k = 0; k < K; k++)
+                if (c0 + k * cstep < cols) G::fetch(slot + k * G::N * threads, threads, from + c0 + k * cstep);
         }
         copy_commit();
     };
@@ -468,50 +479,56 @@ a8_ln_fwd_kernel(const T* x, const T* __restrict__ gamma, const T* __restrict__ 
     for (int stage = 0; row < rows; row += step, stage = stage + 1 == STAGES ? 0 : stage + 1) {
         copy_wait<STAGES - 2>();
         fetch(row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
-        float2 v[8];
-        const uint4* slot = slots + stage * 2 * G::N * threads;
-        G::read(slot, threads, v);
-        G::read(slot + G::N * threads, threads, v + 4);
-        float2 s = v[0];
+        float2 v[E];
+        const uint4* slot = slots + stage * K * G::N * threads;
 #pragma unroll
-        for (int e = 1; e < 8; e++) s = __fadd2_rn(s, v[e]);
-        const float mu = team_sum(s.x + s.y, r0, group + 1, team) * inv_n;
+        for (int k = 0; k < K; k++) G::read(slot + k * G::N * threads, threads, v + 4 * k);
+        float2 s[2] = {v[0], v[1]};
+#pragma unroll
+        for (int e = 2; e < E; e++) s[e & 1] = __fadd2_rn(s[e & 1], v[e]);
+        s[0] = __fadd2_rn(s[0], s[1]);
+        const float mu = team_sum(s[0].x + s[0].y, r0, group + 1, team) * inv_n;
         float2 d2[2] = {both(0.0f), both(0.0f)};
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
+        for (int e = 0; e < E; e++) {
             v[e] = __fadd2_rn(v[e], both(-mu));
-            if (e < 4 ? live0 : live1) d2[e & 1] = __ffma2_rn(v[e], v[e], d2[e & 1]);
+            if (c0 + e / 4 * cstep < cols) d2[e & 1] = __ffma2_rn(v[e], v[e], d2[e & 1]);
         }
         d2[0] = __fadd2_rn(d2[0], d2[1]);
         const float va = fmaf(team_sum(d2[0].x + d2[0].y, r1, group + 1, team), inv_n, eps);
         const float rstd = rsqrtf(va);
-        float top[2] = {0.0f, 0.0f};
+        float top[K];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            v[e] = __fmul2_rn(v[e], both(rstd));
-            top[e >> 2] = max3(top[e >> 2], fabsf(v[e].x), fabsf(v[e].y));
-        }
-        if (!live0) top[0] = 0.0f;
-        if (!live1) top[1] = 0.0f;
+        for (int k = 0; k < K; k++) {
+            top[k] = 0.0f;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) {
-            top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
-            top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+            for (int e = 4 * k; e < 4 * k + 4; e++) {
+                v[e] = __fmul2_rn(v[e], both(rstd));
+                top[k] = max3(top[k], fabsf(v[e].x), fabsf(v[e].y));
+            }
+            if (c0 + k * cstep >= cols) top[k] = 0.0f;
         }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < K; k++) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
         // a value that is not finite makes the row's variance so, and every normalised value with it
         const bool finite = va < INFINITY;
         const int64_t at = row * cols;
+        int8_t* const qr = q + at;
+        T* const yr = y + at;
+        float* const sr = scale + row * blocks;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int c = k ? c1 : c0;
-            if (!(k ? live1 : live0)) continue;
-            const A8Scale sc = a8_scale(finite ? __float_as_uint(top[k]) : 0x7fffffffu);
-            __stcs(reinterpret_cast<uint2*>(q + at + c), make_uint2(a8_pack4(v[4 * k], v[4 * k + 1], sc.inv), a8_pack4(v[4 * k + 2], v[4 * k + 3], sc.inv)));
-            if ((threadIdx.x & 15) == 0) scale[row * blocks + (c >> 7)] = sc.scale;
+        for (int k = 0; k < K; k++) {
+            const int c = c0 + k * cstep;
+            if (c >= cols) continue;
+            const A8Scale sc = a8_scale<false>(finite ? __float_as_uint(top[k]) : 0x7fffffffu);
+            __stcs(reinterpret_cast<uint2*>(qr + c), make_uint2(a8_pack4(v[4 * k], v[4 * k + 1], sc.inv), a8_pack4(v[4 * k + 2], v[4 * k + 3], sc.inv)));
+            if ((threadIdx.x & 15) == 0) sr[c >> 7] = sc.scale;
             float2 o[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = __ffma2_rn(v[4 * k + e], ga[(4 * k + e) * team], be[(4 * k + e) * team]);
-            G::write(y + at + c, o);
+            G::write(yr + c, o);
         }
         if (tid == 0) var[row] = va;
     }
@@ -766,7 +783,7 @@ a8_ln_reduce_kernel(const float* part, T* dgamma, T* dbeta, int parts, int cols,
     }
 }
 
-// threads that own a row of `cols` columns, 16 each
+// threads that own a row of `cols` columns in the backward, 16 each
 static int a8_team(int64_t cols) { return (int)((cols + 511) / 512) * 32; }
 
 // more than the 48 KB of dynamic shared memory that need no leave
@@ -780,22 +797,16 @@ template <typename T>
 static int a8_ln_fwd(const void* x, const void* gamma, const void* beta, void* y, int8_t* q, float* scale, float* var, int64_t rows, int64_t cols,
                      float eps, cudaStream_t st) {
     if (cols % 16 == 0 && cols <= A8_LN_MAX_COLS && aligned16(x) && aligned16(gamma) && aligned16(beta) && aligned16(y) && aligned16(q)) {
-        const int team = a8_team(cols), groups = team >= 256 ? 1 : 256 / team;
-        // as many CTAs as are resident at once
-        const int ctas = team > 256 ? 1 : sizeof(T) == 2 ? 3 : 2;
-        const int64_t want = (rows + groups - 1) / groups, cap = (int64_t)sm_count() * ctas;
+        const int team = (int)((cols + 1023) / 1024) * 32, groups = LnFwd<T>::THREADS / team;       // 32 columns a thread
+        const int64_t want = (rows + groups - 1) / groups, cap = (int64_t)sm_count() * LnFwd<T>::CTAS;
         const int grid = (int)(want < cap ? want : cap);
-        const size_t smem = (size_t)team * groups * LnFwdSmem<T>::PER_THREAD + (size_t)team * LnFwdSmem<T>::PER_MEMBER;
-        cudaError_t e = a8_allow_smem(team > 256 ? (const void*)a8_ln_fwd_kernel<T, 512, 1> : (const void*)a8_ln_fwd_kernel<T, 256, 3>, smem);
+        const size_t smem = (size_t)team * groups * LnFwd<T>::PER_THREAD + (size_t)team * LnFwd<T>::PER_MEMBER;
+        cudaError_t e = a8_allow_smem((const void*)a8_ln_fwd_kernel<T>, smem);
         if (e != cudaSuccess) {
             set_cuda_error(e, "a8_ln_fwd smem attribute");
             return BRK_CUDA_ERROR;
         }
-        if (team > 256)
-            e = launch_pdl(a8_ln_fwd_kernel<T, 512, 1>, grid, team, smem, st, (const T*)x, (const T*)gamma, (const T*)beta, (T*)y, q, scale, var, rows, (int)cols, eps, team);
-        else
-            e = launch_pdl(a8_ln_fwd_kernel<T, 256, 3>, grid, team * groups, smem, st, (const T*)x, (const T*)gamma, (const T*)beta, (T*)y, q, scale, var, rows, (int)cols,
-                           eps, team);
+        e = launch_pdl(a8_ln_fwd_kernel<T>, grid, team * groups, smem, st, (const T*)x, (const T*)gamma, (const T*)beta, (T*)y, q, scale, var, rows, (int)cols, eps, team);
         if (e != cudaSuccess) {
             set_cuda_error(e, "a8_ln_fwd_kernel");
             return BRK_CUDA_ERROR;
