@@ -46,6 +46,7 @@ def rows(batch, tokens, docs, seed, prompts=True):
 @pytest.mark.parametrize("batch,tokens,docs", [
     (1, 1, [[1]]), (1, 1, [[-1]]), (3, 2, [[1, 1], [2], [-1, 1]]), (2, 31, [[31], [5, -3, 7]]), (5, 33, [[33], [1] * 33]),
     (2, 255, [[100, 100], [-255]]), (3, 1024, [[300, 1, 500], [1024], [10, -100, 900]]), (1, 9001, [[4000, 2, 5000]]), (7, 8193, [[8000], [1, -8000, 192]]),
+    (3, 5000, [[17] * 300, [-1, 4990], [2500, 2500]]), (9, 8191, [[8000], [1, -8000, 190], [3] * 3000]),
 ])
 def test_plan(batch, tokens, docs):
     o = ops()
@@ -58,6 +59,10 @@ def test_plan(batch, tokens, docs):
         assert spans.tolist() == [[list(s) for s in r] for r in want[0]]
         assert target.tolist() == want[1] and count.tolist() == [want[2]]
         assert torch.equal(o.doc_plan(cu(mask), None if p is None else cu(p)), spans)
+        if batch * tokens > 1:               # inputs that start on 4-byte boundaries only
+            shift = lambda x: torch.cat([torch.zeros(1, dtype=torch.int32, device="cuda"), cu(x).flatten()])[1:].view(batch, tokens)  # noqa: E731
+            again = o.doc_plan(shift(mask), None if p is None else shift(p), shift(ids))
+            assert all(torch.equal(x, y) for x, y in zip(again, (spans, target, count)))
     # a 0/1 mask without prompts is the padded sequence of the other calls
     one = [[1] * (tokens - b) + [0] * b for b in range(batch)] if tokens > batch else [[1] * tokens] * batch
     t1, c1 = o.loss_targets(cu(ids), cu(one))
