@@ -30,10 +30,7 @@ __device__ int g_doc_error = 0;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-// Three warpgroups: a producer warp and an MMA warp in the first (its other two warps only make it whole), eight row-owner
-// warps in the other two, which take most of the first one's registers: 128 * (56 + 2 * 224) of the launch's 384 * 168.
-constexpr int DA_THREADS = 384;
-constexpr int DA_REGS_FEW = 56, DA_REGS_MANY = 224;
+constexpr int DA_THREADS = 64 + 512;        // producer warp, MMA warp, sixteen row-owner warps
 constexpr int DA_SORT = 512;                // tiles whose order a CTA sorts; more are taken as they come
 
 struct DocAttn {
@@ -421,10 +418,8 @@ struct FwdSmem {
     static constexpr size_t BYTES = 1024 + TILE * (2 + 2 * STAGES) + sizeof(DaTable) + 256 + 2 * 4 * 2 * 128 * sizeof(float);
 };
 
-constexpr int DA_FWD_THREADS = 64 + 512;        // producer warp, MMA warp, sixteen row-owner warps
-
 template <int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(DA_FWD_THREADS, 1)
+__global__ void __launch_bounds__(DA_THREADS, 1)
 doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                     const __grid_constant__ DocAttn p) {
     using S = FwdSmem<D>;
@@ -904,10 +899,10 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 8);
+            mbar_init(&p_full[i], 16);
         }
         mbar_init(acc_full, 1);
-        mbar_init(acc_empty, 8);
+        mbar_init(acc_empty, 16);
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -931,7 +926,6 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         return true;
     };
 
-    if (warp < 4) give_registers<DA_REGS_FEW>();
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
@@ -1014,11 +1008,11 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         if (issuer) {
 #pragma unroll
                             for (int kk = 0; kk < DA_SUB / 16; kk++)      // dV += P^T dO (contraction over the 64 queries)
-                                umma_f16_ts(tmem_base + 256, tmem_base + sb * DA_SUB + (kk >> 1) * 32 + (kk & 1) * 8, dod + kk * 128, IDESC_ACC,
+                                umma_f16_ts(tmem_base + 256, tmem_base + sb * DA_SUB + kk * 16, dod + kk * 128, IDESC_ACC,
                                             n != 1 || kk != 0 ? 1u : 0u);
 #pragma unroll
                             for (int kk = 0; kk < DA_SUB / 16; kk++)      // dK += dS^T Q
-                                umma_f16_ts(tmem_base + 256 + D, tmem_base + 128 + sb * DA_SUB + (kk >> 1) * 32 + (kk & 1) * 8, qd + kk * 128, IDESC_ACC,
+                                umma_f16_ts(tmem_base + 256 + D, tmem_base + 128 + sb * DA_SUB + kk * 16, qd + kk * 128, IDESC_ACC,
                                             n != 1 || kk != 0 ? 1u : 0u);
                             umma_commit(&q_empty[s]);
                         }
@@ -1030,11 +1024,10 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             }
             if (!ok && issuer) atomicExch(&g_doc_error, 12);
         }
-    } else if (warp >= 4) {
-        // ---------------- row owners: two threads per key, 32 of the 64 query columns each ----------------
-        take_registers<DA_REGS_MANY>();
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
-        const int r = quarter * 32 + lane, c0 = half * 32;
+    } else {
+        // ---------------- row owners: four threads per key, 16 of the 64 query columns each ----------------
+        const int quarter = warp & 3, part = (warp - 2) >> 2;
+        const int r = quarter * 32 + lane, c0 = part * 16;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
         bool ok = true;
         uint32_t it0 = 0, items = 0;
@@ -1046,9 +1039,9 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             __half* dkrow = p.dk + row * p.ld_dkv + m.head * D;
             __half* dvrow = p.dv + row * p.ld_dkv + m.head * D;
             if (m.n == 0) {
-                if (half == 0 && live) {
-                    da_zero_row(dkrow, D);
-                    da_zero_row(dvrow, D);
+                if (live) {
+                    da_zero_row(dkrow + part * (D / 4), D / 4);
+                    da_zero_row(dvrow + part * (D / 4), D / 4);
                 }
                 continue;
             }
@@ -1060,7 +1053,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             int blk = m.r0.begin, h = m.head * group;
             auto fetch = [&]() {
                 const int c = r & 63, i = blk * DA_SUB + c;
-                if (half == 1 || i >= p.tokens) return 0.0f;
+                if (part != 0 || i >= p.tokens) return 0.0f;
                 const int64_t at = ((int64_t)m.b * p.heads + h) * p.tokens + i;
                 if (r >= 64) return -p.delta[at];
                 const float lse2 = p.lse_in[at] * -LOG2E;
@@ -1071,7 +1064,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 const uint32_t i = it0 + n;
                 const int sb = i & 1, q0 = blk * DA_SUB;
                 const float slope2 = BIAS ? p.slopes[h] * LOG2E : 0.0f;
-                if (half == 0) stat[sb * 128 + r] = mine;
+                if (part == 0) stat[sb * 128 + r] = mine;
                 if (++blk == m.r0.end) {
                     blk = m.r0.begin;
                     h++;
@@ -1079,30 +1072,30 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 if (n + 1 < m.n) mine = fetch();
                 // orders this step's writes after every thread's reads two steps ago; every owner reaches it in every step,
                 // also one whose bounded wait gave up (it only skips the work)
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                asm volatile("bar.sync 1, 512;" ::: "memory");
                 if (ok) ok = mbar_wait(&s_full[sb], (i >> 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) continue;
                 tcgen05_fence_after();
                 const float4* nlse = reinterpret_cast<const float4*>(stat + sb * 128 + c0);
                 const float4* ndelta = nlse + 16;
-                float2 x[16], g[16];
-                tmem_ld_32x32b_x32(tm + sb * DA_SUB + c0, reinterpret_cast<float*>(x));
-                tmem_ld_32x32b_x32(tm + 128 + sb * DA_SUB + c0, reinterpret_cast<float*>(g));
+                float2 x[8], g[8];
+                tmem_ld_32x32b_x16(tm + sb * DA_SUB + c0, reinterpret_cast<float*>(x));
+                tmem_ld_32x32b_x16(tm + 128 + sb * DA_SUB + c0, reinterpret_cast<float*>(g));
                 tmem_ld_wait();
                 const float2 bias = both(slope2 * (float)(kj - q0));       // minus slope * (query - q0), which nlse holds
-                const bool inner = qlo <= q0 + c0 && qhi >= q0 + c0 + 32 && (!BIAS || kj <= q0 + c0);
+                const bool inner = qlo <= q0 + c0 && qhi >= q0 + c0 + 16 && (!BIAS || kj <= q0 + c0);
                 const bool plain = __all_sync(0xffffffffu, inner);
                 bool near = true;
                 if (CAP) {
                     float wide = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) wide = max3(wide, fabsf(x[e].x), fabsf(x[e].y));
+                    for (int e = 0; e < 8; e++) wide = max3(wide, fabsf(x[e].x), fabsf(x[e].y));
                     near = __all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH);
                 }
                 auto step = [&](auto edge, auto reach) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
+                    for (int e = 0; e < 8; e++) {
                         const float4 l4 = nlse[e >> 1], d4 = ndelta[e >> 1];
                         float2 off = e & 1 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
                         const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
@@ -1137,14 +1130,14 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 } else {
                     step(Flag<true>(), Flag<false>());
                 }
-                uint32_t wp[16], wd[16];
+                uint32_t wp[8], wd[8];
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
+                for (int e = 0; e < 8; e++) {
                     wp[e] = __float_as_uint(x[e].x);
                     wd[e] = __float_as_uint(g[e].x);
                 }
-                tmem_st_32x32b_x16(tm + sb * DA_SUB + c0, wp);
-                tmem_st_32x32b_x16(tm + 128 + sb * DA_SUB + c0, wd);
+                tmem_st_32x32b_x8(tm + sb * DA_SUB + c0, wp);
+                tmem_st_32x32b_x8(tm + 128 + sb * DA_SUB + c0, wd);
                 tmem_st_wait();
                 tcgen05_fence_before();
                 warp_arrive(&p_full[sb]);
@@ -1157,37 +1150,41 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             const bool none = qlo >= qhi;
             if (ok) {
                 tcgen05_fence_after();
-#pragma unroll 1
-                for (int d0 = half * (D / 2); d0 < (half + 1) * (D / 2); d0 += 32) {
-                    uint32_t a[32], c[32];
-                    tmem_ld_32x32b_x32(tm + 256 + d0, a);
-                    tmem_ld_32x32b_x32(tm + 256 + D + d0, c);
+#pragma unroll
+                for (int d0 = part * (D / 4); d0 < (part + 1) * (D / 4); d0 += 16) {
+                    float2 a[8], c[8];
+                    tmem_ld_32x32b_x16(tm + 256 + d0, reinterpret_cast<float*>(a));
+                    tmem_ld_32x32b_x16(tm + 256 + D + d0, reinterpret_cast<float*>(c));
                     tmem_ld_wait();
                     if (live) {
 #pragma unroll
-                        for (int g = 0; g < 4; g++) {
+                        for (int i = 0; i < 8; i += 4) {
                             Vec<__half> o1, o2;
 #pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                const float x = __uint_as_float(a[g * 8 + e]), y = __uint_as_float(c[g * 8 + e]);
-                                bad = fmaf(x, 0.0f, fmaf(y, 0.0f, bad));
-                                o1.v[e] = none ? 0.0f : x;
-                                o2.v[e] = none ? 0.0f : y * p.scale;
+                            for (int e = 0; e < 4; e++) {
+                                const float2 x = a[i + e], y = c[i + e];
+                                bad = fmaf(x.x, 0.0f, fmaf(x.y, 0.0f, fmaf(y.x, 0.0f, fmaf(y.y, 0.0f, bad))));
+                                o1.v[2 * e] = none ? 0.0f : x.x;
+                                o1.v[2 * e + 1] = none ? 0.0f : x.y;
+                                o2.v[2 * e] = none ? 0.0f : y.x * p.scale;
+                                o2.v[2 * e + 1] = none ? 0.0f : y.y * p.scale;
                             }
-                            o1.store(dvrow + d0 + g * 8);
-                            o2.store(dkrow + d0 + g * 8);
+                            o1.store(dvrow + d0 + i * 2);
+                            o2.store(dkrow + d0 + i * 2);
                         }
                     }
                 }
                 tcgen05_fence_before();
                 warp_arrive(acc_empty);            // the accumulators may take the next item's first products
             }
-            // evaluated again by the warps of the rows' first owners, after both owners' stores (the barrier orders them)
-            stat[half * 128 + r] = bad;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            const bool redo = live && !none && (stat[r] != 0.0f || stat[128 + r] != 0.0f);
-            if (half == 0 && __any_sync(0xffffffffu, redo)) da_mend_dkv<D, CAP>(p, m.b, m.head, kj, qlo, qhi, redo);
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            // evaluated again by the warps of the rows' first owners, after all owners' stores (the barrier orders them)
+            if (part == 0) stat[r] = 0.0f;
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            if (bad != 0.0f) stat[r] = 1.0f;
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            const bool redo = live && !none && stat[r] != 0.0f;
+            if (part == 0 && __any_sync(0xffffffffu, redo)) da_mend_dkv<D, CAP>(p, m.b, m.head, kj, qlo, qhi, redo);
+            asm volatile("bar.sync 1, 512;" ::: "memory");
         }
         if (!ok && lane == 0) atomicExch(&g_doc_error, 13);
     }
@@ -1253,12 +1250,12 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&ds_full[i], 8);
+            mbar_init(&ds_full[i], 16);
         }
         mbar_init(dp_full, 1);
-        mbar_init(dp_empty, 8);
+        mbar_init(dp_empty, 16);
         mbar_init(acc_full, 1);
-        mbar_init(acc_empty, 8);
+        mbar_init(acc_empty, 16);
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -1282,7 +1279,6 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         return true;
     };
 
-    if (warp < 4) give_registers<DA_REGS_FEW>();
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
@@ -1368,7 +1364,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                         if (issuer) {
 #pragma unroll
                             for (int kk = 0; kk < 8; kk++)            // dQ += dS K : dS [128 q x 128 keys] in tensor memory, K [128 keys x d], d contiguous
-                                umma_f16_ts(tmem_base + 384, tmem_base + sb * 128 + (kk >> 2) * 64 + (kk & 3) * 8, kd + kk * 128, IDESC_DQ,
+                                umma_f16_ts(tmem_base + 384, tmem_base + sb * 128 + (kk >> 1) * 32 + (kk & 1) * 8, kd + kk * 128, IDESC_DQ,
                                             n != 1 || kk != 0 ? 1u : 0u);
                             umma_commit(&k_empty[s]);
                         }
@@ -1380,11 +1376,10 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             if (!ok && issuer) atomicExch(&g_doc_error, 22);
         }
-    } else if (warp >= 4) {
-        // ---------------- row owners: two threads per query, 64 of the 128 key columns each ----------------
-        take_registers<DA_REGS_MANY>();
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
-        const int r = quarter * 32 + lane, c0 = half * 64;
+    } else {
+        // ---------------- row owners: four threads per query, 32 of the 128 key columns each ----------------
+        const int quarter = warp & 3, part = (warp - 2) >> 2;
+        const int r = quarter * 32 + lane, c0 = part * 32;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
         bool ok = true;
         uint32_t it0 = 0, items = 0;
@@ -1395,7 +1390,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const int64_t row = (int64_t)m.b * p.tokens + qi;
             __half* dqrow = p.dq + row * p.ld_dq + m.head * D;
             if (m.n == 0) {
-                if (half == 0 && live) da_zero_row(dqrow, D);
+                if (live) da_zero_row(dqrow + part * (D / 4), D / 4);
                 continue;
             }
             int4 span = make_int4(0, 0x7fffffff, 0, 0);
@@ -1415,64 +1410,75 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sb], (i >> 1) & 1) && mbar_wait(dp_full, i & 1));
                 if (!ok) break;
                 tcgen05_fence_after();
-                const bool inner = lo <= kbase && hi >= kbase + 64 && (!BIAS || kbase + 63 <= qi || !ahead);
+                const bool inner = lo <= kbase && hi >= kbase + 32 && (!BIAS || kbase + 31 <= qi || !ahead);
                 const bool plain = __all_sync(0xffffffffu, inner);
                 const float dist = (float)(kbase - qi);
-                const float2 base = both(fmaf(slope2, dist, -lse2));
+                const float base = fmaf(slope2, dist, -lse2);
                 const int from = lo - kbase, to = hi - kbase;
-                uint32_t w[2][16];
-#pragma unroll
+                const bool none_here = __all_sync(0xffffffffu, !(lo < kbase + 32 && hi > kbase));      // a corner that no row of the warp sees
+                const uint32_t seen = span_bits(from, to);
+                // 16 columns at a time: more do not fit the registers
+#pragma unroll 1
                 for (int c = 0; c < 2; c++) {
-                    float2 x[16], g[16];
-                    tmem_ld_32x32b_x32(tm + sb * 128 + c0 + c * 32, reinterpret_cast<float*>(x));
-                    tmem_ld_32x32b_x32(tm + 256 + c0 + c * 32, reinterpret_cast<float*>(g));
-                    tmem_ld_wait();
+                    uint32_t w[8];
+                    float2 x[8], g[8];
+                    if (!none_here) {
+                        tmem_ld_32x32b_x16(tm + sb * 128 + c0 + c * 16, reinterpret_cast<float*>(x));
+                        tmem_ld_32x32b_x16(tm + 256 + c0 + c * 16, reinterpret_cast<float*>(g));
+                        tmem_ld_wait();
+                    }
                     if (c == 1) {
                         tcgen05_fence_before();
                         warp_arrive(dp_empty);
                     }
-                    bool near = true;
-                    if (CAP) {
-                        float wide = 0.0f;
+                    if (none_here) {
 #pragma unroll
-                        for (int e = 0; e < 16; e++) wide = max3(wide, fabsf(x[e].x), fabsf(x[e].y));
-                        near = __all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH);
-                    }
-                    auto step = [&](auto edge, auto reach) {
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            const int k = c * 32 + 2 * e;
-                            float2 off = base, s, t;
-                            if (BIAS) {
-                                if (edge)
-                                    off = make_float2(fmaf(-slope2, fabsf(dist + (float)k), -lse2), fmaf(-slope2, fabsf(dist + (float)(k + 1)), -lse2));
-                                else
-                                    off = __ffma2_rn(both(slope2), pair_of(c * 16 + e), base);
-                            }
-                            if (CAP) {
-                                t = da_capped(x[e], p, reach);
-                                s = __ffma2_rn(t, both(p.cap_log2), off);
-                            } else {
-                                s = __ffma2_rn(x[e], both(p.scale_log2), off);
-                            }
-                            float2 de = __fmul2_rn(make_float2(fast_exp2(s.x), fast_exp2(s.y)), __fadd2_rn(g[e], both(-dlt)));
-                            if (CAP) de = __fmul2_rn(de, __ffma2_rn(neg2(t), t, both(1.0f)));
-                            if (edge) {
-                                if (!(k >= from && k < to)) de.x = 0.0f;
-                                if (!(k + 1 >= from && k + 1 < to)) de.y = 0.0f;
-                            }
-                            w[c][e] = da_half2(de.x, de.y);
-                        }
-                    };
-                    if (near) {
-                        if (plain) step(Flag<false>(), Flag<true>());
-                        else step(Flag<true>(), Flag<true>());
+                        for (int e = 0; e < 8; e++) w[e] = 0;
                     } else {
-                        step(Flag<true>(), Flag<false>());
+                        bool near = true;
+                        if (CAP) {
+                            float wide = 0.0f;
+#pragma unroll
+                            for (int e = 0; e < 8; e++) wide = max3(wide, fabsf(x[e].x), fabsf(x[e].y));
+                            near = __all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH);
+                        }
+                        auto step = [&](auto edge, auto reach) {
+                            const float d0 = dist + (float)(c * 16);
+                            const float2 at = both(BIAS ? fmaf(slope2, (float)(c * 16), base) : base);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                float2 off = at, s, t;
+                                if (BIAS) {
+                                    if (edge)
+                                        off = make_float2(fmaf(-slope2, fabsf(d0 + (float)(2 * e)), -lse2), fmaf(-slope2, fabsf(d0 + (float)(2 * e + 1)), -lse2));
+                                    else
+                                        off = __ffma2_rn(both(slope2), pair_of(e), at);
+                                }
+                                if (CAP) {
+                                    t = da_capped(x[e], p, reach);
+                                    s = __ffma2_rn(t, both(p.cap_log2), off);
+                                } else {
+                                    s = __ffma2_rn(x[e], both(p.scale_log2), off);
+                                }
+                                float2 de = __fmul2_rn(make_float2(fast_exp2(s.x), fast_exp2(s.y)), __fadd2_rn(g[e], both(-dlt)));
+                                if (CAP) de = __fmul2_rn(de, __ffma2_rn(neg2(t), t, both(1.0f)));
+                                if (edge) {
+                                    const uint32_t bits = seen >> (c * 16 + 2 * e);
+                                    if (!(bits & 1)) de.x = 0.0f;
+                                    if (!(bits & 2)) de.y = 0.0f;
+                                }
+                                w[e] = da_half2(de.x, de.y);
+                            }
+                        };
+                        if (near) {
+                            if (plain) step(Flag<false>(), Flag<true>());
+                            else step(Flag<true>(), Flag<true>());
+                        } else {
+                            step(Flag<true>(), Flag<false>());
+                        }
                     }
+                    tmem_st_32x32b_x8(tm + sb * 128 + c0 + c * 8, w);
                 }
-                tmem_st_32x32b_x16(tm + sb * 128 + c0, w[0]);
-                tmem_st_32x32b_x16(tm + sb * 128 + c0 + 16, w[1]);
                 tmem_st_wait();
                 tcgen05_fence_before();
                 warp_arrive(&ds_full[sb]);
@@ -1486,33 +1492,34 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             if (ok) {
                 tcgen05_fence_after();
 #pragma unroll 1
-                for (int d0 = half * (D / 2); d0 < (half + 1) * (D / 2); d0 += 32) {
-                    uint32_t a[32];
-                    tmem_ld_32x32b_x32(tm + 384 + d0, a);
+                for (int d0 = part * (D / 4); d0 < (part + 1) * (D / 4); d0 += 16) {
+                    float2 a[8];
+                    tmem_ld_32x32b_x16(tm + 384 + d0, reinterpret_cast<float*>(a));
                     tmem_ld_wait();
                     if (live) {
 #pragma unroll
-                        for (int g = 0; g < 4; g++) {
+                        for (int i = 0; i < 8; i += 4) {
                             Vec<__half> o;
 #pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                const float x = __uint_as_float(a[g * 8 + e]);
-                                bad = fmaf(x, 0.0f, bad);
-                                o.v[e] = none ? 0.0f : x * p.scale;
+                            for (int e = 0; e < 4; e++) {
+                                bad = fmaf(a[i + e].x, 0.0f, fmaf(a[i + e].y, 0.0f, bad));
+                                o.v[2 * e] = none ? 0.0f : a[i + e].x * p.scale;
+                                o.v[2 * e + 1] = none ? 0.0f : a[i + e].y * p.scale;
                             }
-                            o.store(dqrow + d0 + g * 8);
+                            o.store(dqrow + d0 + i * 2);
                         }
                     }
                 }
                 tcgen05_fence_before();
                 warp_arrive(acc_empty);
             }
-            // evaluated again by the warps of the rows' first owners, after both owners' stores (the barrier orders them)
-            again[half * 128 + r] = bad;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            const bool redo = live && !none && (again[r] != 0.0f || again[128 + r] != 0.0f);
-            if (half == 0 && __any_sync(0xffffffffu, redo)) da_mend_dq<D, CAP>(p, m.b, m.head, qi, lo, hi, redo);
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            // evaluated again by the warps of the rows' first owners, after all owners' stores (the barrier orders them)
+            if (part == 0) again[r] = 0.0f;
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            if (bad != 0.0f) again[r] = 1.0f;
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            const bool redo = live && !none && again[r] != 0.0f;
+            if (part == 0 && __any_sync(0xffffffffu, redo)) da_mend_dq<D, CAP>(p, m.b, m.head, qi, lo, hi, redo);
         }
         if (!ok && lane == 0) atomicExch(&g_doc_error, 23);
     }
@@ -1552,7 +1559,7 @@ static int da_fwd(const DocMaps& t, const DocAttn& p, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     const int rc = da_allow_smem(doc_attn_fwd_kernel<D, CAP, BIAS>, smem, done, "doc_attn_fwd smem attribute");
     if (rc) return rc;
-    doc_attn_fwd_kernel<D, CAP, BIAS><<<da_grid((int64_t)p.batch * ((p.tokens + 255) / 256) * p.heads), DA_FWD_THREADS, smem, st>>>(t.q, t.k, t.v, p);
+    doc_attn_fwd_kernel<D, CAP, BIAS><<<da_grid((int64_t)p.batch * ((p.tokens + 255) / 256) * p.heads), DA_THREADS, smem, st>>>(t.q, t.k, t.v, p);
     return launch_status("doc_attn_fwd_kernel");
 }
 template <int D, bool CAP, bool BIAS>
