@@ -41,6 +41,7 @@ struct DocAttn {
     int batch, tokens, heads, kv_heads;
     float scale, scale_log2;                // 1/sqrt(d), times log2(e)
     float cap_log2, cap_in;                 // cap log2(e); 1 / (sqrt(d) cap)
+    float cap_curve;                        // -1 / cap_log2^2: the tanh's derivative is 1 + cap_curve s^2 of the capped score s
     float cap_poly[5];                      // coefficients of the capped score, see da_capped_near
     // forward
     bool wide_out;                          // rows of out start on 32-byte boundaries
@@ -101,7 +102,6 @@ __device__ __forceinline__ float da_score(float raw, const DocAttn& p, float& sl
     slope_of_tanh = fmaf(-t, t, 1.0f);
     return t * p.cap_log2;
 }
-__device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
 // bits [from, to) of 32, whatever lies outside of them
 __device__ __forceinline__ uint32_t span_bits(int from, int to) {
     from = min(max(from, 0), 32);
@@ -610,15 +610,23 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         };
         bool have = item_of(0, m);
         int4 span = make_int4(0, 0, 0, 0);
-        if (have) span = span_of();
+        float slope = 0.0f;
+        if (have) {
+            span = span_of();
+            if (BIAS) slope = p.slopes[m.head];
+        }
         for (int round = 1; have; round++) {
             const Range blocks = t == 0 ? m.r0 : m.r1;
             const int head = m.head, b = m.b, qi = m.t0 + t * 128 + r;
             const bool live = qi < p.tokens;
             const int64_t row = (int64_t)b * p.tokens + qi;
             const int lo = max(span.x, 0), hi = live ? min(span.y, p.tokens) : span.y;
-            have = item_of(round, m);                   // the next item's span travels while this one is worked on
-            if (have) span = span_of();
+            const float slope2 = slope * LOG2E;
+            have = item_of(round, m);                   // the next item's span and slope travel while this one is worked on
+            if (have) {
+                span = span_of();
+                if (BIAS) slope = p.slopes[m.head];
+            }
             __half* o = p.out + row * p.ld_out + head * D + half * (D / 2);
             float* lse = p.lse && half == 0 ? p.lse + ((int64_t)b * p.heads + head) * p.tokens + qi : nullptr;
             if (blocks.end == blocks.begin) {
@@ -628,7 +636,6 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 }
                 continue;
             }
-            const float slope2 = BIAS ? p.slopes[head] * LOG2E : 0.0f;
             const bool ahead = BIAS && __any_sync(0xffffffffu, live && hi > qi + 1);      // some row sees keys behind itself: the prompt's
             float m_ref = -INFINITY;
             float2 l = both(0.0f);
@@ -1048,28 +1055,28 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             int4 span = make_int4(0, 0, 0, 0x7fffffff);              // rows behind the sequence never force the masked path
             if (live) span = p.spans[row];
             const int qlo = max(span.z, 0), qhi = live ? min(span.w, p.tokens) : span.w;
-            // a step's 64 log-sum-exps (log2 units, with the query's share of the bias) and 64 deltas, all negated: one for each of
-            // the first owners, fetched a step ahead so that the load's latency passes behind the step before it
+            // a step's 64 log-sum-exps and 64 deltas, one for each of the first owners, fetched a step ahead as they are: arithmetic on
+            // them would wait for the load where it is issued
             int blk = m.r0.begin, h = m.head * group;
+            float next = 0.0f, next_slope = 0.0f;
             auto fetch = [&]() {
-                const int c = r & 63, i = blk * DA_SUB + c;
-                if (part != 0 || i >= p.tokens) return 0.0f;
-                const int64_t at = ((int64_t)m.b * p.heads + h) * p.tokens + i;
-                if (r >= 64) return -p.delta[at];
-                const float lse2 = p.lse_in[at] * -LOG2E;
-                return BIAS ? fmaf(p.slopes[h] * -LOG2E, (float)c, lse2) : lse2;
+                const int i = blk * DA_SUB + (r & 63);
+                next = 0.0f;
+                if (part == 0 && i < p.tokens) next = (r < 64 ? p.lse_in : p.delta)[((int64_t)m.b * p.heads + h) * p.tokens + i];
+                if (BIAS) next_slope = p.slopes[h];
             };
-            float mine = fetch();
+            fetch();
             for (int n = 0; n < m.n; n++) {
                 const uint32_t i = it0 + n;
                 const int sb = i & 1, q0 = blk * DA_SUB;
-                const float slope2 = BIAS ? p.slopes[h] * LOG2E : 0.0f;
-                if (part == 0) stat[sb * 128 + r] = mine;
+                const float slope2 = next_slope * LOG2E;
+                // negated, and the log-sum-exp in log2 units with the query's share of the bias
+                if (part == 0) stat[sb * 128 + r] = r < 64 ? fmaf(next, -LOG2E, -slope2 * (float)r) : -next;
                 if (++blk == m.r0.end) {
                     blk = m.r0.begin;
                     h++;
                 }
-                if (n + 1 < m.n) mine = fetch();
+                if (n + 1 < m.n) fetch();
                 // orders this step's writes after every thread's reads two steps ago; every owner reaches it in every step,
                 // also one whose bounded wait gave up (it only skips the work)
                 asm volatile("bar.sync 1, 512;" ::: "memory");
@@ -1107,14 +1114,14 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         }
                         float2 s, t;
                         if (CAP) {
-                            t = da_capped(x[e], p, reach);
-                            s = __ffma2_rn(t, both(p.cap_log2), off);
+                            t = reach ? da_capped_near(x[e], p, both(0.0f)) : __fmul2_rn(da_capped(x[e], p, false), both(p.cap_log2));
+                            s = __fadd2_rn(t, off);
                         } else {
                             s = __ffma2_rn(x[e], both(p.scale_log2), off);
                         }
                         float2 pe = make_float2(fast_exp2(s.x), fast_exp2(s.y));
                         float2 de = __fmul2_rn(pe, __fadd2_rn(g[e], nd));
-                        if (CAP) de = __fmul2_rn(de, __ffma2_rn(neg2(t), t, both(1.0f)));
+                        if (CAP) de = __fmul2_rn(de, __ffma2_rn(__fmul2_rn(t, both(p.cap_curve)), t, both(1.0f)));
                         if (edge) {
                             const int qi = q0 + c0 + 2 * e;
                             if (!(qlo <= qi && qi < qhi)) pe.x = de.x = 0.0f;
@@ -1383,26 +1390,38 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
         bool ok = true;
         uint32_t it0 = 0, items = 0;
-        Item m;
-        for (int round = 0; item_of(round, m); round++) {
+        Item m = {}, following = {};
+        int4 next_span = make_int4(0, 0, 0, 0);
+        float next_lse = 0.0f, next_delta = 0.0f, next_slope = 0.0f;
+        auto fetch = [&]() {
+            const int qi = following.t0 + r;
+            next_span = make_int4(0, 0x7fffffff, 0, 0);
+            next_lse = next_delta = 0.0f;
+            if (qi < p.tokens) {
+                const int64_t at = ((int64_t)following.b * p.heads + following.head) * p.tokens + qi;
+                next_span = p.spans[(int64_t)following.b * p.tokens + qi];
+                next_lse = p.lse_in[at];
+                next_delta = p.delta[at];
+            }
+            if (BIAS) next_slope = p.slopes[following.head];
+        };
+        bool have = item_of(0, following);
+        if (have) fetch();
+        for (int round = 1; have; round++) {
+            m = following;
             const int qi = m.t0 + r;
             const bool live = qi < p.tokens;
             const int64_t row = (int64_t)m.b * p.tokens + qi;
+            const int4 span = next_span;
+            const float lse2 = next_lse * LOG2E, dlt = next_delta, slope2 = next_slope * LOG2E;
+            have = item_of(round, following);           // the next item's row data travels while this one is worked on
+            if (have) fetch();
             __half* dqrow = p.dq + row * p.ld_dq + m.head * D;
             if (m.n == 0) {
                 if (live) da_zero_row(dqrow + part * (D / 4), D / 4);
                 continue;
             }
-            int4 span = make_int4(0, 0x7fffffff, 0, 0);
-            float lse2 = 0.0f, dlt = 0.0f;
-            if (live) {
-                const int64_t at = ((int64_t)m.b * p.heads + m.head) * p.tokens + qi;
-                span = p.spans[row];
-                lse2 = p.lse_in[at] * LOG2E;
-                dlt = p.delta[at];
-            }
             const int lo = max(span.x, 0), hi = live ? min(span.y, p.tokens) : span.y;
-            const float slope2 = BIAS ? p.slopes[m.head] * LOG2E : 0.0f;
             const bool ahead = BIAS && __any_sync(0xffffffffu, live && hi > qi + 1);
             for (int n = 0; n < m.n && ok; n++) {
                 const uint32_t i = it0 + n;
@@ -1455,13 +1474,13 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                                         off = __ffma2_rn(both(slope2), pair_of(e), at);
                                 }
                                 if (CAP) {
-                                    t = da_capped(x[e], p, reach);
-                                    s = __ffma2_rn(t, both(p.cap_log2), off);
+                                    t = reach ? da_capped_near(x[e], p, both(0.0f)) : __fmul2_rn(da_capped(x[e], p, false), both(p.cap_log2));
+                                    s = __fadd2_rn(t, off);
                                 } else {
                                     s = __ffma2_rn(x[e], both(p.scale_log2), off);
                                 }
                                 float2 de = __fmul2_rn(make_float2(fast_exp2(s.x), fast_exp2(s.y)), __fadd2_rn(g[e], both(-dlt)));
-                                if (CAP) de = __fmul2_rn(de, __ffma2_rn(neg2(t), t, both(1.0f)));
+                                if (CAP) de = __fmul2_rn(de, __ffma2_rn(__fmul2_rn(t, both(p.cap_curve)), t, both(1.0f)));
                                 if (edge) {
                                     const uint32_t bits = seen >> (c * 16 + 2 * e);
                                     if (!(bits & 1)) de.x = 0.0f;
@@ -1619,6 +1638,7 @@ static DocAttn da_params(const void* q, const void* k, const void* v, int64_t ld
     p.scale_log2 = (float)(scale * log2e);
     p.cap_log2 = (float)(cap * log2e);
     p.cap_in = cap > 0.0f ? (float)(scale / cap) : 0.0f;
+    p.cap_curve = cap > 0.0f ? (float)(-1.0 / (cap * log2e * cap * log2e)) : 0.0f;
     const double tanh_poly[5] = {TANH_1, TANH_3, TANH_5, TANH_7, TANH_9};
     for (int i = 0; i < 5; i++) p.cap_poly[i] = (float)(tanh_poly[i] * cap * log2e);
     return p;
