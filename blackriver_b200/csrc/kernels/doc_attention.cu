@@ -44,7 +44,6 @@ struct DocAttn {
     float cap_curve;                        // -1 / cap_log2^2: the tanh's derivative is 1 + cap_curve s^2 of the capped score s
     float cap_poly[5];                      // coefficients of the capped score, see da_capped_near
     // forward
-    bool wide_out;                          // rows of out start on 32-byte boundaries
     __half* out;
     float* lse;                             // [batch, heads, tokens], natural log
     // backward
@@ -210,6 +209,62 @@ __device__ __forceinline__ int da_plan_items(DaTable* table, int n_tiles, int n_
     return listed;
 }
 
+// ---- results ---------------------------------------------------------------------------------------------------------------
+
+// one arrival for the whole warp
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+__device__ __forceinline__ void da_zero_row(__half* row, int d) {
+    for (int e = 0; e < d; e += 8) *reinterpret_cast<uint4*>(row + e) = make_uint4(0, 0, 0, 0);
+}
+// Results leave through shared memory: a warp writes 32 rows x 32 columns into 2 KB of its own, and its first lane stores them
+// with the TMA, which clips the box at the end of the row of the batch.  Stores by the owners themselves, whose neighbouring
+// lanes hold rows 24 KB apart, kept the load/store unit busy for 4000 to 7000 clocks an item.
+constexpr int DA_PATCH = 2048;                  // bytes a warp stages
+// 16-byte piece `piece` of row `row` of a patch whose rows are COLS columns: 64-byte swizzle for 32 columns, none for 16
+template <int COLS>
+__device__ __forceinline__ void da_stage(unsigned char* patch, int row, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const int at = COLS == 32 ? row * 64 + ((piece ^ ((row >> 1) & 3)) << 4) : row * 32 + piece * 16;
+    *reinterpret_cast<uint4*>(patch + at) = make_uint4(a, b, c, d);
+}
+// the warp's patch may be written again
+__device__ __forceinline__ void da_patch_free() {
+    if ((threadIdx.x & 31) == 0) bulk_wait_read<0>();
+    __syncwarp();
+}
+__device__ __forceinline__ void da_patch_store(const CUtensorMap* map, const unsigned char* patch, int x, int y, int z, int tokens) {
+    fence_proxy_async();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0 && y < tokens) {
+        tma_store_3d(map, patch, x, y, z);
+        bulk_commit();
+    }
+}
+// what the warp has stored is written, so that it can be written again by plain stores
+__device__ __forceinline__ void da_patch_written() {
+    if ((threadIdx.x & 31) == 0) bulk_wait_all();
+    __syncwarp();
+}
+// whether `x` holds for any thread of those that meet at the barrier
+__device__ __forceinline__ bool barrier_any(int id, int threads, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "barrier.cta.red.or.pred p, %2, %3, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)x), "r"(id), "r"(threads)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ uint32_t da_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // ---- rows evaluated again without the tensor core (see the top) ------------------------------------------------------------
 // Called by whole warps with one row per lane, `bad` where the row's accumulator is not finite.  A row that sees an operand
 // that is not finite keeps what it has (32 partners are looked at at a time, one per lane, until every bad row has found
@@ -370,33 +425,6 @@ __device__ __noinline__ void da_mend_dkv(const DocAttn& p, int b, int kh, int j,
     }
 }
 
-// one arrival for the whole warp
-__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
-__device__ __forceinline__ void da_zero_row(__half* row, int d) {
-    for (int e = 0; e < d; e += 8) *reinterpret_cast<uint4*>(row + e) = make_uint4(0, 0, 0, 0);
-}
-// 64 bytes of a row.  Neighbouring lanes write rows far apart, so a lane writes whole sectors of 32 bytes where the row is
-// aligned to them.
-__device__ __forceinline__ void da_store64(__half* to, const uint32_t (&w)[16], bool wide) {
-    if (wide) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 8)
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + i * 2), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]),
-                         "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
-                         : "memory");
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(to + i * 2) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-    }
-}
-__device__ __forceinline__ uint32_t da_half2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // ==========================================================================================================================
 // forward
 //
@@ -414,13 +442,14 @@ __device__ __forceinline__ uint32_t da_half2(float a, float b) {
 template <int D>
 struct FwdSmem {
     static constexpr uint32_t TILE = 128 * D * 2;
-    static constexpr int STAGES = 2;                    // of K and of V each
-    static constexpr size_t BYTES = 1024 + TILE * (2 + 2 * STAGES) + sizeof(DaTable) + 256 + 2 * 4 * 2 * 128 * sizeof(float);
+    static constexpr int SLOTS = 3;                     // of the ring that K and V tiles pass through in turn
+    static constexpr size_t BYTES = 1024 + TILE * (2 + SLOTS) + 16 * DA_PATCH + sizeof(DaTable) + 256 + 2 * 4 * 2 * 128 * sizeof(float);
 };
 
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(DA_THREADS, 1)
 doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                    const __grid_constant__ CUtensorMap tmap_out,
                     const __grid_constant__ DocAttn p) {
     using S = FwdSmem<D>;
     constexpr uint32_t TMEM_COLS = 512;                 // S0 [0,128)  S1 [128,256)  O0 [256,256+D)  O1 [256+D,256+2D)
@@ -431,16 +460,14 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* sQ = base;                           // two tiles
-    unsigned char* sK = sQ + 2 * S::TILE;
-    unsigned char* sV = sK + S::STAGES * S::TILE;
-    DaTable* table = reinterpret_cast<DaTable*>(sV + S::STAGES * S::TILE);
+    unsigned char* sKV = sQ + 2 * S::TILE;              // the ring: K V K V ..
+    unsigned char* sOut = sKV + S::SLOTS * S::TILE;     // a patch for each owner warp
+    DaTable* table = reinterpret_cast<DaTable*>(sOut + 16 * DA_PATCH);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + 1);
     uint64_t* q_full = bars;                 // 2 (per tile)
     uint64_t* q_empty = bars + 2;            // 2
-    uint64_t* k_full = bars + 4;             // STAGES
-    uint64_t* k_empty = bars + 6;
-    uint64_t* v_full = bars + 8;
-    uint64_t* v_empty = bars + 10;
+    uint64_t* kv_full = bars + 4;            // SLOTS
+    uint64_t* kv_empty = bars + 8;           // SLOTS
     uint64_t* s_full = bars + 12;            // 2 (per tile)
     uint64_t* p_full = bars + 14;            // 2
     uint64_t* o_done = bars + 16;            // 2: a P V product of the tile is complete
@@ -452,13 +479,13 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const int per_row = (p.tokens + 255) / 256, n_tiles = p.batch * per_row;
 
     if (threadIdx.x == 0) {
+        for (int i = 0; i < S::SLOTS; i++) {
+            mbar_init(&kv_full[i], 1);
+            mbar_init(&kv_empty[i], 1);
+        }
         for (int t = 0; t < 2; t++) {
             mbar_init(&q_full[t], 1);
             mbar_init(&q_empty[t], 1);
-            mbar_init(&k_full[t], 1);
-            mbar_init(&k_empty[t], 1);
-            mbar_init(&v_full[t], 1);
-            mbar_init(&v_empty[t], 1);
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 8);
             mbar_init(&o_done[t], 1);
@@ -497,7 +524,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         // ---------------- TMA producer ----------------
         if (lane == 0) {
             bool ok = true;
-            uint32_t it = 0, q_count0 = 0, q_count1 = 0;
+            uint32_t u = 0, q_count0 = 0, q_count1 = 0;         // loads through the ring: K of block n is 2n, V is 2n + 1
             Item m;
             for (int round = 0; ok && item_of(round, m); round++) {
                 const int row = m.b * p.tokens, col = m.head * D, kcol = m.head / group * D;
@@ -509,21 +536,20 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     for (int a = 0; a < D / 64; a++) tma_load_2d(sQ + t * S::TILE + a * 16384, &tmap_q, &q_full[t], col + a * 64, row + m.t0 + t * 128);
                     return true;
                 };
-                ok = load_q(0, m.r0, q_count0) && load_q(1, m.r1, q_count1);
-                for (int n = 0; n < m.n && ok; n++, it++) {
-                    const int s = it % S::STAGES, y = row + (m.last - n) * 128;
-                    const uint32_t par = ((it / S::STAGES) & 1) ^ 1;
-                    ok = mbar_wait(&k_empty[s], par);
-                    if (!ok) break;
-                    mbar_arrive_expect_tx(&k_full[s], S::TILE);
+                auto load = [&](const CUtensorMap* map, int y) {
+                    const int s = u % S::SLOTS;
+                    if (!mbar_wait(&kv_empty[s], ((u / S::SLOTS) & 1) ^ 1)) return false;
+                    u++;
+                    mbar_arrive_expect_tx(&kv_full[s], S::TILE);
 #pragma unroll
-                    for (int a = 0; a < D / 64; a++) tma_load_2d(sK + s * S::TILE + a * 16384, &tmap_k, &k_full[s], kcol + a * 64, y);
-                    ok = mbar_wait(&v_empty[s], par);
-                    if (!ok) break;
-                    mbar_arrive_expect_tx(&v_full[s], S::TILE);
-#pragma unroll
-                    for (int a = 0; a < D / 64; a++) tma_load_2d(sV + s * S::TILE + a * 16384, &tmap_v, &v_full[s], kcol + a * 64, y);
-                }
+                    for (int a = 0; a < D / 64; a++) tma_load_2d(sKV + s * S::TILE + a * 16384, map, &kv_full[s], kcol + a * 64, y);
+                    return true;
+                };
+                // the second tile begins first, where its keys reach further
+                const bool second = m.r1.end > m.r0.end;
+                if (second) ok = load_q(1, m.r1, q_count1) && load_q(0, m.r0, q_count0);
+                else ok = load_q(0, m.r0, q_count0) && load_q(1, m.r1, q_count1);
+                for (int n = 0; n < m.n && ok; n++) ok = load(&tmap_k, row + (m.last - n) * 128) && load(&tmap_v, row + (m.last - n) * 128);
             }
             if (!ok) atomicExch(&g_doc_error, 1);
         }
@@ -534,18 +560,19 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             const bool issuer = elect_one();
             bool ok = true;
             uint32_t it = 0, q_count0 = 0, q_count1 = 0, p_count0 = 0, p_count1 = 0;        // blocks, and per tile: items, blocks
-            const uint64_t q_desc = make_smem_desc_sw128(smem_u32(sQ), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(sK), 16, 1024);
-            const uint64_t v_desc = make_smem_desc_sw128(smem_u32(sV), 16384, 1024);
+            const uint64_t q_desc = make_smem_desc_sw128(smem_u32(sQ), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(sKV), 16, 1024);
+            const uint64_t v_desc = make_smem_desc_sw128(smem_u32(sKV), 16384, 1024);
             Item m;
             for (int round = 0; ok && item_of(round, m); round++) {
                 m.last = uniform(m.last), m.n = uniform(m.n);
                 m.r0.begin = uniform(m.r0.begin), m.r0.end = uniform(m.r0.end), m.r1.begin = uniform(m.r1.begin), m.r1.end = uniform(m.r1.end);
                 for (int n = -1; n < m.n && ok; n++) {
-                    const int vs = (it + n) % S::STAGES, ks = (it + n + 1) % S::STAGES;        // n == -1 uses no V
+                    const uint32_t v_load = 2 * (it + n) + 1, k_load = v_load + 1;               // n == -1 uses no V
+                    const int vs = v_load % S::SLOTS, ks = k_load % S::SLOTS;
                     const bool more = n + 1 < m.n;
                     const int blk = m.last - n;
-                    if (n >= 0) ok = mbar_wait(&v_full[vs], ((it + n) / S::STAGES) & 1);
-                    if (ok && more) ok = mbar_wait(&k_full[ks], ((it + n + 1) / S::STAGES) & 1);
+                    if (n >= 0) ok = mbar_wait(&kv_full[vs], (v_load / S::SLOTS) & 1);
+                    if (ok && more) ok = mbar_wait(&kv_full[ks], (k_load / S::SLOTS) & 1);
                     // P V of block n and then the scores of block n + 1; the index is a constant, so that nothing lands in local memory
                     auto step = [&](auto tile, const Range& r, uint32_t& q_count, uint32_t& p_count) {
                         constexpr int t = decltype(tile)::value;
@@ -582,8 +609,8 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     ok = ok && step(std::integral_constant<int, 0>(), m.r0, q_count0, p_count0) && step(std::integral_constant<int, 1>(), m.r1, q_count1, p_count1);
                     if (!ok) break;
                     if (issuer) {
-                        if (n >= 0) umma_commit(&v_empty[vs]);
-                        if (more) umma_commit(&k_empty[ks]);
+                        if (n >= 0) umma_commit(&kv_empty[vs]);
+                        if (more) umma_commit(&kv_empty[ks]);
                     }
                 }
                 it += m.n;
@@ -598,6 +625,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
         const uint32_t tm_s = tm + t * 128 + half * 64, tm_o = tm + 256 + t * D + half * (D / 2);
         float* const cells = exchange + t * 1024 + r;
+        unsigned char* const patch = sOut + (warp - 2) * DA_PATCH;
         // The owners of 32 rows meet once a block.  Every owner reaches it in every block, also one whose bounded wait gave up.
         auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quarter) : "memory"); };
         bool ok = true;
@@ -627,11 +655,10 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 span = span_of();
                 if (BIAS) slope = p.slopes[m.head];
             }
-            __half* o = p.out + row * p.ld_out + head * D + half * (D / 2);
             float* lse = p.lse && half == 0 ? p.lse + ((int64_t)b * p.heads + head) * p.tokens + qi : nullptr;
             if (blocks.end == blocks.begin) {
                 if (live) {
-                    da_zero_row(o, D / 2);
+                    da_zero_row(p.out + row * p.ld_out + head * D + half * (D / 2), D / 2);
                     if (lse) *lse = 0.0f;
                 }
                 continue;
@@ -785,6 +812,10 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     float2 x[16];
                     tmem_ld_32x32b_x32(tm_o + c, reinterpret_cast<float*>(x));
                     tmem_ld_wait();
+                    if (c + 32 == D / 2) {
+                        tcgen05_fence_before();
+                        warp_arrive(&o_empty[t]);
+                    }
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
@@ -793,20 +824,26 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         bad[i & 1] = __hfma2(*reinterpret_cast<const __half2*>(&w[i]), __float2half2_rn(0.0f), bad[i & 1]);      // a NaN, once something is not finite
                         if (none) w[i] = 0;
                     }
-                    if (live) da_store64(o + c, w, p.wide_out);
+                    da_patch_free();
+#pragma unroll
+                    for (int i = 0; i < 4; i++) da_stage<32>(patch, lane, i, w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    da_patch_store(&tmap_out, patch, head * D + half * (D / 2) + c, qi - lane, b, p.tokens);
                 }
-                tcgen05_fence_before();
-                warp_arrive(&o_empty[t]);
                 if (live && lse) *lse = none ? 0.0f : lse2 * LN2;
             }
             const __half2 any = __hadd2(bad[0], bad[1]);
-            const bool again = live && !none && fabsf(lse2) < INFINITY && (__hisnan(__low2half(any)) || __hisnan(__high2half(any)));
-            float* const flags = cells + 768;
-            flags[half * 128] = again ? 1.0f : 0.0f;
-            meet();                                     // orders both owners' stores before a row is written again
-            const bool redo = flags[0] + flags[128] != 0.0f;
-            if (half == 0 && __any_sync(0xffffffffu, redo)) da_mend_out<D, CAP>(p, b, head, qi, lo, hi, lse2, redo);
+            const bool again = ok && live && !none && fabsf(lse2) < INFINITY && (__hisnan(__low2half(any)) || __hisnan(__high2half(any)));
+            if (barrier_any(1 + t * 4 + quarter, 64, again)) {
+                float* const flags = cells + 768;
+                flags[half * 128] = again ? 1.0f : 0.0f;
+                da_patch_written();
+                meet();                                 // orders both owners' stores before a row is written again
+                const bool redo = flags[0] + flags[128] != 0.0f;
+                if (half == 0) da_mend_out<D, CAP>(p, b, head, qi, lo, hi, lse2, redo);
+                meet();
+            }
         }
+        da_patch_free();                                // the patch is read before the CTA's shared memory goes
         if (!ok && lane == 0) atomicExch(&g_doc_error, 3);
     }
 
@@ -858,8 +895,8 @@ constexpr uint32_t DA_SUB_ATOM = DA_SUB * 128;
 template <int D>
 struct DkvSmem {
     static constexpr uint32_t KV = 128 * D * 2, SUB = DA_SUB * D * 2;
-    static constexpr int STAGES = 4;
-    static constexpr size_t BYTES = 1024 + 2 * KV + 2 * STAGES * SUB + 2 * 2 * DA_SUB * sizeof(float) + sizeof(DaTable) + 256;
+    static constexpr int STAGES = 3;
+    static constexpr size_t BYTES = 1024 + 2 * KV + 2 * STAGES * SUB + 16 * DA_PATCH + 2 * 2 * DA_SUB * sizeof(float) + sizeof(DaTable) + 256;
 };
 
 // Transposed scores S^T = K Q^T and dP^T = V dO^T (a row owner is a key), so that P^T and dS^T are the A operands of
@@ -868,7 +905,8 @@ struct DkvSmem {
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(DA_THREADS, 1)
 doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                    const __grid_constant__ CUtensorMap tmap_do, const __grid_constant__ DocAttn p) {
+                    const __grid_constant__ CUtensorMap tmap_do, const __grid_constant__ CUtensorMap tmap_dk, const __grid_constant__ CUtensorMap tmap_dv,
+                    const __grid_constant__ DocAttn p) {
     using S = DkvSmem<D>;
     constexpr uint32_t TMEM_COLS = 512;     // S^T x2 [0,128)  dP^T x2 [128,256)  dV [256,256+D)  dK [256+D,256+2D)
     constexpr uint32_t IDESC_ST = make_idesc_f16_f32(128, DA_SUB, 0, 0);
@@ -880,7 +918,8 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     unsigned char* sV = sK + S::KV;
     unsigned char* sQ = sV + S::KV;
     unsigned char* sDO = sQ + S::STAGES * S::SUB;
-    float* stat = reinterpret_cast<float*>(sDO + S::STAGES * S::SUB);       // [2][lse2 x 64 | delta x 64]
+    unsigned char* sOut = sDO + S::STAGES * S::SUB;     // a patch for each owner warp
+    float* stat = reinterpret_cast<float*>(sOut + 16 * DA_PATCH);       // [2][lse2 x 64 | delta x 64]
     DaTable* table = reinterpret_cast<DaTable*>(stat + 2 * 2 * DA_SUB);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + 1);
     uint64_t* kv_full = bars;
@@ -1036,36 +1075,48 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         const int quarter = warp & 3, part = (warp - 2) >> 2;
         const int r = quarter * 32 + lane, c0 = part * 16;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        unsigned char* const patch = sOut + (warp - 2) * DA_PATCH;
         bool ok = true;
         uint32_t it0 = 0, items = 0;
-        Item m;
-        for (int round = 0; item_of(round, m); round++) {
+        Item m = {}, following = {};
+        int4 next_span = make_int4(0, 0, 0, 0);
+        float next = 0.0f, next_slope = 0.0f;
+        // A step's 64 log-sum-exps and 64 deltas, one for each of the first owners, fetched a step ahead as they are: arithmetic on
+        // them would wait for the load where it is issued.
+        auto fetch = [&](const Item& of, int blk, int h) {
+            const int i = blk * DA_SUB + (r & 63);
+            next = 0.0f;
+            if (part == 0 && i < p.tokens) next = (r < 64 ? p.lse_in : p.delta)[((int64_t)of.b * p.heads + h) * p.tokens + i];
+            if (BIAS) next_slope = p.slopes[h];
+        };
+        auto fetch_span = [&]() {
+            const int kj = following.t0 + r;
+            // rows behind the sequence never force the masked path
+            next_span = kj < p.tokens ? p.spans[(int64_t)following.b * p.tokens + kj] : make_int4(0, 0, 0, 0x7fffffff);
+        };
+        bool have = item_of(0, following);
+        if (have) {
+            fetch_span();
+            if (following.n > 0) fetch(following, following.r0.begin, following.head * group);
+        }
+        for (int round = 1; have; round++) {
+            m = following;
+            const int4 span = next_span;
+            have = item_of(round, following);           // the next item's span and first statistics travel while this one is worked on
+            if (have) fetch_span();
             const int kj = m.t0 + r;
             const bool live = kj < p.tokens;
             const int64_t row = (int64_t)m.b * p.tokens + kj;
-            __half* dkrow = p.dk + row * p.ld_dkv + m.head * D;
-            __half* dvrow = p.dv + row * p.ld_dkv + m.head * D;
             if (m.n == 0) {
                 if (live) {
-                    da_zero_row(dkrow + part * (D / 4), D / 4);
-                    da_zero_row(dvrow + part * (D / 4), D / 4);
+                    da_zero_row(p.dk + row * p.ld_dkv + m.head * D + part * (D / 4), D / 4);
+                    da_zero_row(p.dv + row * p.ld_dkv + m.head * D + part * (D / 4), D / 4);
                 }
+                if (have && following.n > 0) fetch(following, following.r0.begin, following.head * group);
                 continue;
             }
-            int4 span = make_int4(0, 0, 0, 0x7fffffff);              // rows behind the sequence never force the masked path
-            if (live) span = p.spans[row];
             const int qlo = max(span.z, 0), qhi = live ? min(span.w, p.tokens) : span.w;
-            // a step's 64 log-sum-exps and 64 deltas, one for each of the first owners, fetched a step ahead as they are: arithmetic on
-            // them would wait for the load where it is issued
             int blk = m.r0.begin, h = m.head * group;
-            float next = 0.0f, next_slope = 0.0f;
-            auto fetch = [&]() {
-                const int i = blk * DA_SUB + (r & 63);
-                next = 0.0f;
-                if (part == 0 && i < p.tokens) next = (r < 64 ? p.lse_in : p.delta)[((int64_t)m.b * p.heads + h) * p.tokens + i];
-                if (BIAS) next_slope = p.slopes[h];
-            };
-            fetch();
             for (int n = 0; n < m.n; n++) {
                 const uint32_t i = it0 + n;
                 const int sb = i & 1, q0 = blk * DA_SUB;
@@ -1076,7 +1127,8 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     blk = m.r0.begin;
                     h++;
                 }
-                if (n + 1 < m.n) fetch();
+                if (n + 1 < m.n) fetch(m, blk, h);
+                else if (have && following.n > 0) fetch(following, following.r0.begin, following.head * group);
                 // orders this step's writes after every thread's reads two steps ago; every owner reaches it in every step,
                 // also one whose bounded wait gave up (it only skips the work)
                 asm volatile("bar.sync 1, 512;" ::: "memory");
@@ -1158,41 +1210,43 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             if (ok) {
                 tcgen05_fence_after();
 #pragma unroll
-                for (int d0 = part * (D / 4); d0 < (part + 1) * (D / 4); d0 += 16) {
-                    float2 a[8], c[8];
-                    tmem_ld_32x32b_x16(tm + 256 + d0, reinterpret_cast<float*>(a));
-                    tmem_ld_32x32b_x16(tm + 256 + D + d0, reinterpret_cast<float*>(c));
-                    tmem_ld_wait();
-                    if (live) {
+                for (int k = 0; k < 2; k++) {              // dV, then dK: D / 4 columns of each
+                    uint32_t w[D / 8];
 #pragma unroll
-                        for (int i = 0; i < 8; i += 4) {
-                            Vec<__half> o1, o2;
+                    for (int c = 0; c < D / 4; c += 16) {
+                        float2 a[8];
+                        tmem_ld_32x32b_x16(tm + 256 + k * D + part * (D / 4) + c, reinterpret_cast<float*>(a));
+                        tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const float2 x = a[i + e], y = c[i + e];
-                                bad = fmaf(x.x, 0.0f, fmaf(x.y, 0.0f, fmaf(y.x, 0.0f, fmaf(y.y, 0.0f, bad))));
-                                o1.v[2 * e] = none ? 0.0f : x.x;
-                                o1.v[2 * e + 1] = none ? 0.0f : x.y;
-                                o2.v[2 * e] = none ? 0.0f : y.x * p.scale;
-                                o2.v[2 * e + 1] = none ? 0.0f : y.y * p.scale;
-                            }
-                            o1.store(dvrow + d0 + i * 2);
-                            o2.store(dkrow + d0 + i * 2);
+                        for (int i = 0; i < 8; i++) {
+                            bad = fmaf(a[i].x, 0.0f, fmaf(a[i].y, 0.0f, bad));
+                            w[c / 2 + i] = none ? 0 : k == 0 ? da_half2(a[i].x, a[i].y) : da_half2(a[i].x * p.scale, a[i].y * p.scale);
                         }
                     }
+                    if (k == 1) {
+                        tcgen05_fence_before();
+                        warp_arrive(acc_empty);            // the accumulators may take the next item's first products
+                    }
+                    da_patch_free();
+#pragma unroll
+                    for (int i = 0; i < D / 32; i++) da_stage<D / 4>(patch, lane, i, w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    da_patch_store(k == 0 ? &tmap_dv : &tmap_dk, patch, m.head * D + part * (D / 4), kj - lane, m.b, p.tokens);
                 }
-                tcgen05_fence_before();
-                warp_arrive(acc_empty);            // the accumulators may take the next item's first products
             }
-            // evaluated again by the warps of the rows' first owners, after all owners' stores (the barrier orders them)
-            if (part == 0) stat[r] = 0.0f;
-            asm volatile("bar.sync 1, 512;" ::: "memory");
-            if (bad != 0.0f) stat[r] = 1.0f;
-            asm volatile("bar.sync 1, 512;" ::: "memory");
-            const bool redo = live && !none && stat[r] != 0.0f;
-            if (part == 0 && __any_sync(0xffffffffu, redo)) da_mend_dkv<D, CAP>(p, m.b, m.head, kj, qlo, qhi, redo);
-            asm volatile("bar.sync 1, 512;" ::: "memory");
+            // evaluated again by the warps of the rows' first owners, after all owners' stores
+            const bool again = ok && live && !none && bad != 0.0f;
+            if (barrier_any(1, 512, again)) {
+                if (part == 0) stat[r] = 0.0f;
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                if (again) stat[r] = 1.0f;
+                da_patch_written();
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                const bool redo = stat[r] != 0.0f;
+                if (part == 0 && __any_sync(0xffffffffu, redo)) da_mend_dkv<D, CAP>(p, m.b, m.head, kj, qlo, qhi, redo);
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+            }
         }
+        da_patch_free();                                // the patch is read before the CTA's shared memory goes
         if (!ok && lane == 0) atomicExch(&g_doc_error, 13);
     }
     tcgen05_fence_before();
@@ -1207,7 +1261,8 @@ template <int D>
 struct DqSmem {
     static constexpr uint32_t TILE = 128 * D * 2;
     static constexpr int STAGES = 2;
-    static constexpr size_t BYTES = 1024 + 2 * TILE + 2 * STAGES * TILE + 2 * 128 * sizeof(float) + sizeof(DaTable) + 256;
+    static constexpr int PATCH = DA_PATCH / 2;          // 16 columns at a time: Q, dO and two stages of K and V leave no more
+    static constexpr size_t BYTES = 1024 + 2 * TILE + 2 * STAGES * TILE + 16 * PATCH + 2 * 128 * sizeof(float) + sizeof(DaTable) + 256;
 };
 
 // S = Q K^T (two buffers), dP = dO V^T (one), dQ += dS K over blocks of 128 keys.  dS goes over the scores it came from,
@@ -1215,7 +1270,7 @@ struct DqSmem {
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(DA_THREADS, 1)
 doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                   const __grid_constant__ CUtensorMap tmap_do, const __grid_constant__ DocAttn p) {
+                   const __grid_constant__ CUtensorMap tmap_do, const __grid_constant__ CUtensorMap tmap_dq, const __grid_constant__ DocAttn p) {
     using S = DqSmem<D>;
     constexpr uint32_t TMEM_COLS = 512;     // S x2 [0,256)  dP [256,384)  dQ [384,384+D)
     constexpr uint32_t IDESC_S = make_idesc_f16_f32(128, 128, 0, 0);
@@ -1227,7 +1282,8 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     unsigned char* sDO = sQ + S::TILE;
     unsigned char* sK = sDO + S::TILE;
     unsigned char* sV = sK + S::STAGES * S::TILE;
-    float* again = reinterpret_cast<float*>(sV + S::STAGES * S::TILE);     // [2 owners][128]
+    unsigned char* sOut = sV + S::STAGES * S::TILE;     // a patch for each owner warp
+    float* again = reinterpret_cast<float*>(sOut + 16 * S::PATCH);     // [2 owners][128]
     DaTable* table = reinterpret_cast<DaTable*>(again + 2 * 128);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + 1);
     uint64_t* q_full = bars;
@@ -1388,6 +1444,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         const int quarter = warp & 3, part = (warp - 2) >> 2;
         const int r = quarter * 32 + lane, c0 = part * 32;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        unsigned char* const patch = sOut + (warp - 2) * S::PATCH;
         bool ok = true;
         uint32_t it0 = 0, items = 0;
         Item m = {}, following = {};
@@ -1416,9 +1473,8 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const float lse2 = next_lse * LOG2E, dlt = next_delta, slope2 = next_slope * LOG2E;
             have = item_of(round, following);           // the next item's row data travels while this one is worked on
             if (have) fetch();
-            __half* dqrow = p.dq + row * p.ld_dq + m.head * D;
             if (m.n == 0) {
-                if (live) da_zero_row(dqrow + part * (D / 4), D / 4);
+                if (live) da_zero_row(p.dq + row * p.ld_dq + m.head * D + part * (D / 4), D / 4);
                 continue;
             }
             const int lo = max(span.x, 0), hi = live ? min(span.y, p.tokens) : span.y;
@@ -1510,36 +1566,41 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             float bad = 0.0f;
             if (ok) {
                 tcgen05_fence_after();
-#pragma unroll 1
-                for (int d0 = part * (D / 4); d0 < (part + 1) * (D / 4); d0 += 16) {
+#pragma unroll
+                for (int c = 0; c < D / 4; c += 16) {
                     float2 a[8];
-                    tmem_ld_32x32b_x16(tm + 384 + d0, reinterpret_cast<float*>(a));
+                    tmem_ld_32x32b_x16(tm + 384 + part * (D / 4) + c, reinterpret_cast<float*>(a));
                     tmem_ld_wait();
-                    if (live) {
-#pragma unroll
-                        for (int i = 0; i < 8; i += 4) {
-                            Vec<__half> o;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                bad = fmaf(a[i + e].x, 0.0f, fmaf(a[i + e].y, 0.0f, bad));
-                                o.v[2 * e] = none ? 0.0f : a[i + e].x * p.scale;
-                                o.v[2 * e + 1] = none ? 0.0f : a[i + e].y * p.scale;
-                            }
-                            o.store(dqrow + d0 + i * 2);
-                        }
+                    if (c + 16 == D / 4) {
+                        tcgen05_fence_before();
+                        warp_arrive(acc_empty);
                     }
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        bad = fmaf(a[i].x, 0.0f, fmaf(a[i].y, 0.0f, bad));
+                        w[i] = none ? 0 : da_half2(a[i].x * p.scale, a[i].y * p.scale);
+                    }
+                    da_patch_free();
+#pragma unroll
+                    for (int i = 0; i < 2; i++) da_stage<16>(patch, lane, i, w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    da_patch_store(&tmap_dq, patch, m.head * D + part * (D / 4) + c, qi - lane, m.b, p.tokens);
                 }
-                tcgen05_fence_before();
-                warp_arrive(acc_empty);
             }
-            // evaluated again by the warps of the rows' first owners, after all owners' stores (the barrier orders them)
-            if (part == 0) again[r] = 0.0f;
-            asm volatile("bar.sync 1, 512;" ::: "memory");
-            if (bad != 0.0f) again[r] = 1.0f;
-            asm volatile("bar.sync 1, 512;" ::: "memory");
-            const bool redo = live && !none && again[r] != 0.0f;
-            if (part == 0 && __any_sync(0xffffffffu, redo)) da_mend_dq<D, CAP>(p, m.b, m.head, qi, lo, hi, redo);
+            // evaluated again by the warps of the rows' first owners, after all owners' stores
+            const bool redo_any = ok && live && !none && bad != 0.0f;
+            if (barrier_any(1, 512, redo_any)) {
+                if (part == 0) again[r] = 0.0f;
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                if (redo_any) again[r] = 1.0f;
+                da_patch_written();
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                const bool redo = again[r] != 0.0f;
+                if (part == 0 && __any_sync(0xffffffffu, redo)) da_mend_dq<D, CAP>(p, m.b, m.head, qi, lo, hi, redo);
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+            }
         }
+        da_patch_free();                                // the patch is read before the CTA's shared memory goes
         if (!ok && lane == 0) atomicExch(&g_doc_error, 23);
     }
     tcgen05_fence_before();
@@ -1568,7 +1629,8 @@ static int da_allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done, co
 static unsigned da_grid(int64_t items) { return (unsigned)(items < sm_count() ? items : sm_count()); }       // persistent: one CTA per SM walks the items
 
 struct DocMaps {
-    CUtensorMap q, k, v, d_out, q64, do64;
+    CUtensorMap q, k, v, d_out, q64, do64;      // operands
+    CUtensorMap out, dq, dk, dv;                // results, [batch, tokens, columns]
 };
 
 template <int D, bool CAP, bool BIAS>
@@ -1578,7 +1640,7 @@ static int da_fwd(const DocMaps& t, const DocAttn& p, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     const int rc = da_allow_smem(doc_attn_fwd_kernel<D, CAP, BIAS>, smem, done, "doc_attn_fwd smem attribute");
     if (rc) return rc;
-    doc_attn_fwd_kernel<D, CAP, BIAS><<<da_grid((int64_t)p.batch * ((p.tokens + 255) / 256) * p.heads), DA_THREADS, smem, st>>>(t.q, t.k, t.v, p);
+    doc_attn_fwd_kernel<D, CAP, BIAS><<<da_grid((int64_t)p.batch * ((p.tokens + 255) / 256) * p.heads), DA_THREADS, smem, st>>>(t.q, t.k, t.v, t.out, p);
     return launch_status("doc_attn_fwd_kernel");
 }
 template <int D, bool CAP, bool BIAS>
@@ -1590,10 +1652,10 @@ static int da_bwd(const DocMaps& t, const DocAttn& p, cudaStream_t st) {
     if (!rc) rc = da_allow_smem(doc_attn_dq_kernel<D, CAP, BIAS>, smem_q, done_q, "doc_attn_dq smem attribute");
     if (rc) return rc;
     const int64_t tiles = (int64_t)p.batch * ((p.tokens + 127) / 128);
-    doc_attn_dkv_kernel<D, CAP, BIAS><<<da_grid(tiles * p.kv_heads), DA_THREADS, smem_kv, st>>>(t.q64, t.k, t.v, t.do64, p);
+    doc_attn_dkv_kernel<D, CAP, BIAS><<<da_grid(tiles * p.kv_heads), DA_THREADS, smem_kv, st>>>(t.q64, t.k, t.v, t.do64, t.dk, t.dv, p);
     rc = launch_status("doc_attn_dkv_kernel");
     if (rc) return rc;
-    doc_attn_dq_kernel<D, CAP, BIAS><<<da_grid(tiles * p.heads), DA_THREADS, smem_q, st>>>(t.q, t.k, t.v, t.d_out, p);
+    doc_attn_dq_kernel<D, CAP, BIAS><<<da_grid(tiles * p.heads), DA_THREADS, smem_q, st>>>(t.q, t.k, t.v, t.d_out, t.dq, p);
     return launch_status("doc_attn_dq_kernel");
 }
 template <int D, bool CAP>
@@ -1605,6 +1667,16 @@ static int da_dispatch(bool forward, int d, const DocMaps& t, const DocAttn& p, 
     const bool cap = p.cap_log2 > 0.0f;
     if (d == 128) return cap ? da_run<128, true>(forward, t, p, st) : da_run<128, false>(forward, t, p, st);
     return cap ? da_run<64, true>(forward, t, p, st) : da_run<64, false>(forward, t, p, st);
+}
+
+// [batch, tokens, cols] fp16 with rows `ld` elements apart, boxes of 32 tokens x `box_cols` columns as da_stage lays them out
+static bool da_result_map(CUtensorMap* out, void* base, int batch, int tokens, int64_t cols, int64_t ld, int box_cols) {
+    const EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)tokens, (cuuint64_t)batch}, strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)ld * 2 * (cuuint64_t)tokens};
+    const cuuint32_t box[3] = {(cuuint32_t)box_cols, 32, 1}, one[3] = {1, 1, 1};
+    return enc(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // sizes, strides and alignment that both directions share
@@ -1658,12 +1730,11 @@ extern "C" int brk_doc_attn_fwd(const void* q, const void* k, const void* v, int
     if (!out) return BRK_OUTPUT_ERROR;
     DocAttn p = da_params(q, k, v, ld_q, ld_kv, ld_out, spans, slopes, cap, batch, tokens, heads, kv_heads, head_dim);
     p.out = (__half*)out;
-    p.wide_out = (reinterpret_cast<uintptr_t>(out) & 31) == 0 && ld_out % 16 == 0;
     p.lse = lse;
     const uint64_t rows = (uint64_t)batch * tokens, qc = (uint64_t)heads * head_dim, kc = (uint64_t)kv_heads * head_dim;
     DocMaps t;
     if (!make_tmap_2d_f16(&t.q, q, rows, qc, (uint64_t)ld_q, 64, 128) || !make_tmap_2d_f16(&t.k, k, rows, kc, (uint64_t)ld_kv, 64, 128) ||
-        !make_tmap_2d_f16(&t.v, v, rows, kc, (uint64_t)ld_kv, 64, 128)) {
+        !make_tmap_2d_f16(&t.v, v, rows, kc, (uint64_t)ld_kv, 64, 128) || !da_result_map(&t.out, out, batch, tokens, (int64_t)qc, ld_out, 32)) {
         set_error_message("brk_doc_attn_fwd: could not encode a tensor map");
         return BRK_CUDA_ERROR;
     }
@@ -1701,7 +1772,9 @@ extern "C" int brk_doc_attn_bwd(const void* q, const void* k, const void* v, int
     DocMaps t;
     if (!make_tmap_2d_f16(&t.q, q, rows, qc, (uint64_t)ld_q, 64, 128) || !make_tmap_2d_f16(&t.k, k, rows, kc, (uint64_t)ld_kv, 64, 128) ||
         !make_tmap_2d_f16(&t.v, v, rows, kc, (uint64_t)ld_kv, 64, 128) || !make_tmap_2d_f16(&t.d_out, d_out, rows, qc, (uint64_t)ld_out, 64, 128) ||
-        !make_tmap_2d_f16(&t.q64, q, rows, qc, (uint64_t)ld_q, 64, DA_SUB) || !make_tmap_2d_f16(&t.do64, d_out, rows, qc, (uint64_t)ld_out, 64, DA_SUB)) {
+        !make_tmap_2d_f16(&t.q64, q, rows, qc, (uint64_t)ld_q, 64, DA_SUB) || !make_tmap_2d_f16(&t.do64, d_out, rows, qc, (uint64_t)ld_out, 64, DA_SUB) ||
+        !da_result_map(&t.dq, dq, batch, tokens, (int64_t)qc, ld_dq, 16) || !da_result_map(&t.dk, dk, batch, tokens, (int64_t)kc, ld_dkv, head_dim / 4) ||
+        !da_result_map(&t.dv, dv, batch, tokens, (int64_t)kc, ld_dkv, head_dim / 4)) {
         set_error_message("brk_doc_attn_bwd: could not encode a tensor map");
         return BRK_CUDA_ERROR;
     }
