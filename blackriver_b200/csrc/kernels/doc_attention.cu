@@ -109,8 +109,24 @@ __device__ __forceinline__ uint32_t span_bits(int from, int to) {
 }
 template <bool B>
 using Flag = std::integral_constant<bool, B>;
-// key (or query) numbers 2i and 2i + 1 of a chunk
-__device__ __forceinline__ float2 pair_of(int i) { return make_float2((float)(2 * i), (float)(2 * i + 1)); }
+// The straight line at + slope * e over a chunk's columns, two at a time.  Four running pairs: as fused multiply-adds on the
+// numbers of the columns it took a register pair for each of them.
+struct Line {
+    float2 v[4], step;
+    __device__ __forceinline__ Line(float slope, float at) {
+        const float2 first = make_float2(at, at + slope), two = both(2.0f * slope);
+        v[0] = first;
+#pragma unroll
+        for (int i = 1; i < 4; i++) v[i] = __fadd2_rn(v[i - 1], two);
+        step = both(8.0f * slope);
+    }
+    // columns 2i and 2i + 1; i in order
+    __device__ __forceinline__ float2 next(int i) {
+        const float2 r = v[i & 3];
+        v[i & 3] = __fadd2_rn(r, step);
+        return r;
+    }
+};
 
 // ---- tiles ---------------------------------------------------------------------------------------------------------------
 
@@ -698,17 +714,17 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     }
                     auto fill = [&](auto line) {        // line: the bias as a straight line in the key's number
                         constexpr bool LINE = BIAS && decltype(line)::value;
-                        const float2 at = both(LINE ? fmaf(slope2, (float)(c * 32), slant) + shift : shift);
-                        auto off = [&](int i) { return LINE ? __ffma2_rn(both(slope2), pair_of(i), at) : at; };
+                        const float2 at = both(shift);
+                        Line bias(LINE ? slope2 : 0.0f, LINE ? fmaf(slope2, (float)(c * 32), slant) + shift : 0.0f);
                         if (CAP && near) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = da_capped_near(x[i], p, off(i));
+                            for (int i = 0; i < 16; i++) x[i] = da_capped_near(x[i], p, LINE ? bias.next(i) : at);
                         } else if (CAP) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = __ffma2_rn(da_capped(x[i], p, false), both(p.cap_log2), off(i));
+                            for (int i = 0; i < 16; i++) x[i] = __ffma2_rn(da_capped(x[i], p, false), both(p.cap_log2), LINE ? bias.next(i) : at);
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = __ffma2_rn(x[i], both(p.scale_log2), off(i));
+                            for (int i = 0; i < 16; i++) x[i] = __ffma2_rn(x[i], both(p.scale_log2), LINE ? bias.next(i) : at);
                         }
                     };
                     if (whole >> c & 1) {
@@ -1519,15 +1535,15 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                         }
                         auto step = [&](auto edge, auto reach) {
                             const float d0 = dist + (float)(c * 16);
-                            const float2 at = both(BIAS ? fmaf(slope2, (float)(c * 16), base) : base);
+                            Line bias(BIAS ? slope2 : 0.0f, BIAS ? fmaf(slope2, (float)(c * 16), base) : base);
 #pragma unroll
                             for (int e = 0; e < 8; e++) {
-                                float2 off = at, s, t;
+                                float2 off = both(base), s, t;
                                 if (BIAS) {
                                     if (edge)
                                         off = make_float2(fmaf(-slope2, fabsf(d0 + (float)(2 * e)), -lse2), fmaf(-slope2, fabsf(d0 + (float)(2 * e + 1)), -lse2));
                                     else
-                                        off = __ffma2_rn(both(slope2), pair_of(e), at);
+                                        off = bias.next(e);
                                 }
                                 if (CAP) {
                                     t = reach ? da_capped_near(x[e], p, both(0.0f)) : __fmul2_rn(da_capped(x[e], p, false), both(p.cap_log2));
