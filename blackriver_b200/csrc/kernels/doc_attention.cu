@@ -168,10 +168,11 @@ struct DaTable {
 template <typename R>
 __device__ __forceinline__ bool da_find_item(int round, int n_tiles, int n_heads, int per_row, int tile_tokens, const DaTable* table, R ranges, DaItem& m) {
     const uint32_t G = gridDim.x, c = blockIdx.x;
-    const uint64_t idx = (uint64_t)round * G + ((round & 1) ? G - 1 - c : c);
-    if (idx >= (uint64_t)n_tiles * n_heads) return false;
+    const uint64_t at = (uint64_t)round * G + ((round & 1) ? G - 1 - c : c);
+    if (at >= (uint64_t)n_tiles * n_heads) return false;
+    const uint32_t idx = (uint32_t)at;                  // tiles times heads stay below 2^32: checked before the launch
     const int place = (int)(idx / (uint32_t)n_heads);
-    m.head = (int)(idx - (uint64_t)place * n_heads);
+    m.head = (int)(idx - (uint32_t)place * n_heads);
     const bool sorted = n_tiles <= DA_SORT;
     const int tile = sorted ? table->order[place] : n_tiles - 1 - place;
     m.b = tile / per_row;
@@ -212,11 +213,11 @@ __device__ __forceinline__ int da_plan_items(DaTable* table, int n_tiles, int n_
         }
         __syncthreads();
     }
-    const uint64_t items = (uint64_t)n_tiles * n_heads;
-    const uint64_t full = items / gridDim.x, rest = items - full * gridDim.x;
+    const uint32_t items = (uint32_t)n_tiles * n_heads;
+    const uint32_t full = items / gridDim.x, rest = items - full * gridDim.x;
     // rounds this CTA has an item in: all full ones, and the last one if it is dealt that far
-    const uint64_t mine = full + ((full & 1) ? (blockIdx.x >= gridDim.x - rest) : (blockIdx.x < rest));
-    const int listed = (int)(mine < (uint64_t)DA_LIST ? mine : (uint64_t)DA_LIST);
+    const uint32_t mine = full + ((full & 1) ? (blockIdx.x >= gridDim.x - rest) : (blockIdx.x < rest));
+    const int listed = (int)min(mine, (uint32_t)DA_LIST);
     for (int i = threadIdx.x; i < listed; i += blockDim.x) {
         DaItem m = {};
         da_find_item(i, n_tiles, n_heads, per_row, tile_tokens, table, ranges, m);
@@ -516,6 +517,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         tmem_alloc(tmem_base_smem, TMEM_COLS);
         tmem_relinquish();
     }
+    pdl_wait();
     auto ranges = [&](int b, int t0, bool second) { return da_blocks<true>(p, b, second ? t0 + 128 : t0, 128); };
     const int listed = da_plan_items(table, n_tiles, p.heads, per_row, 256, ranges);
     tcgen05_fence_before();
@@ -883,26 +885,29 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 // owner overwrites what the other has yet to read.  They are rounded to fp16 there, as operands have to be.
 // ==========================================================================================================================
 
-// delta_i = sum_d dO_id O_id per query and head: d / 8 neighbouring lanes own one head of one row
+// delta_i = sum_d dO_id O_id per query and head: a CTA per token, d / 8 neighbouring lanes own one head
 __global__ void __launch_bounds__(256)
-doc_delta_kernel(const __half* out, const __half* dout, int64_t ld, float* delta, int batch, int tokens, int heads, int d) {
-    const int lanes = d >> 3;
-    const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t grp = t / lanes;
-    const int part = (int)(t % lanes);
-    const bool live = grp < (int64_t)batch * tokens * heads;
-    const int h = (int)(grp % heads);
-    const int64_t row = grp / heads;
-    float s = 0.0f;
-    if (live) {
-        Vec<__half> a, c;
-        a.load(out + row * ld + (int64_t)h * d + part * 8);
-        c.load(dout + row * ld + (int64_t)h * d + part * 8);
+doc_delta_kernel(const __half* out, const __half* dout, int64_t ld, float* delta, int tokens, int heads, int d) {
+    const int lanes = d >> 3, pieces = heads * lanes, row = blockIdx.x;
+    const int b = row / tokens;
+    float* const to = delta + (int64_t)b * heads * tokens + (row - b * tokens);
+    pdl_wait();
+    pdl_launch_dependents();
+    const __half* o = out + row * ld;
+    const __half* g = dout + row * ld;
+    for (int i0 = 0; i0 < pieces; i0 += 256) {
+        const int i = i0 + threadIdx.x;
+        float2 s = make_float2(0.0f, 0.0f);
+        if (i < pieces) {
+            const uint4 a = ld_raw(o + i * 8), c = ld_raw(g + i * 8);
+            const __half2 *x = reinterpret_cast<const __half2*>(&a), *y = reinterpret_cast<const __half2*>(&c);
 #pragma unroll
-        for (int e = 0; e < 8; e++) s = fmaf(a.v[e], c.v[e], s);
+            for (int e = 0; e < 4; e++) s = __ffma2_rn(__half22float2(x[e]), __half22float2(y[e]), s);
+        }
+        float sum = s.x + s.y;
+        for (int w = lanes >> 1; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (i < pieces && (i & (lanes - 1)) == 0) to[(int64_t)(i / lanes) * tokens] = sum;
     }
-    for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (live && part == 0) delta[((row / tokens) * heads + h) * tokens + row % tokens] = s;
 }
 
 constexpr int DA_SUB = 64;                  // queries per step of the dK / dV kernel
@@ -973,6 +978,10 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     }
     auto ranges = [&](int b, int t0, bool second) { return second ? Range{0, 0} : da_blocks<false>(p, b, t0, DA_SUB); };
     const int listed = da_plan_items(table, n_tiles, p.kv_heads, per_row, 128, ranges);
+    // Everything before the delta kernel is complete when this one starts: only delta is waited for.  The dQ kernel needs nothing of
+    // this one and may take over each SM that is done here.
+    pdl_wait();
+    pdl_launch_dependents();
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -1619,6 +1628,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         da_patch_free();                                // the patch is read before the CTA's shared memory goes
         if (!ok && lane == 0) atomicExch(&g_doc_error, 23);
     }
+    pdl_wait();                                          // what follows in the stream waits for this kernel and so for the dK / dV kernel too
     tcgen05_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -1642,7 +1652,16 @@ static int da_allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done, co
     set_cuda_error(e, where);
     return BRK_CUDA_ERROR;
 }
-static unsigned da_grid(int64_t items) { return (unsigned)(items < sm_count() ? items : sm_count()); }       // persistent: one CTA per SM walks the items
+// persistent: one CTA per SM walks the items
+template <typename K, typename... Args>
+static int da_launch(const char* name, K kernel, int64_t items, size_t smem, cudaStream_t st, const Args&... args) {
+    const cudaError_t e = launch_pdl(kernel, (int)(items < sm_count() ? items : sm_count()), DA_THREADS, smem, st, args...);
+    if (e != cudaSuccess) {
+        set_cuda_error(e, name);
+        return BRK_CUDA_ERROR;
+    }
+    return launch_status(name);
+}
 
 struct DocMaps {
     CUtensorMap q, k, v, d_out, q64, do64;      // operands
@@ -1656,8 +1675,7 @@ static int da_fwd(const DocMaps& t, const DocAttn& p, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     const int rc = da_allow_smem(doc_attn_fwd_kernel<D, CAP, BIAS>, smem, done, "doc_attn_fwd smem attribute");
     if (rc) return rc;
-    doc_attn_fwd_kernel<D, CAP, BIAS><<<da_grid((int64_t)p.batch * ((p.tokens + 255) / 256) * p.heads), DA_THREADS, smem, st>>>(t.q, t.k, t.v, t.out, p);
-    return launch_status("doc_attn_fwd_kernel");
+    return da_launch("doc_attn_fwd_kernel", doc_attn_fwd_kernel<D, CAP, BIAS>, (int64_t)p.batch * ((p.tokens + 255) / 256) * p.heads, smem, st, t.q, t.k, t.v, t.out, p);
 }
 template <int D, bool CAP, bool BIAS>
 static int da_bwd(const DocMaps& t, const DocAttn& p, cudaStream_t st) {
@@ -1668,11 +1686,9 @@ static int da_bwd(const DocMaps& t, const DocAttn& p, cudaStream_t st) {
     if (!rc) rc = da_allow_smem(doc_attn_dq_kernel<D, CAP, BIAS>, smem_q, done_q, "doc_attn_dq smem attribute");
     if (rc) return rc;
     const int64_t tiles = (int64_t)p.batch * ((p.tokens + 127) / 128);
-    doc_attn_dkv_kernel<D, CAP, BIAS><<<da_grid(tiles * p.kv_heads), DA_THREADS, smem_kv, st>>>(t.q64, t.k, t.v, t.do64, t.dk, t.dv, p);
-    rc = launch_status("doc_attn_dkv_kernel");
+    rc = da_launch("doc_attn_dkv_kernel", doc_attn_dkv_kernel<D, CAP, BIAS>, tiles * p.kv_heads, smem_kv, st, t.q64, t.k, t.v, t.do64, t.dk, t.dv, p);
     if (rc) return rc;
-    doc_attn_dq_kernel<D, CAP, BIAS><<<da_grid(tiles * p.heads), DA_THREADS, smem_q, st>>>(t.q, t.k, t.v, t.d_out, t.dq, p);
-    return launch_status("doc_attn_dq_kernel");
+    return da_launch("doc_attn_dq_kernel", doc_attn_dq_kernel<D, CAP, BIAS>, tiles * p.heads, smem_q, st, t.q, t.k, t.v, t.d_out, t.dq, p);
 }
 template <int D, bool CAP>
 static int da_run(bool forward, const DocMaps& t, const DocAttn& p, cudaStream_t st) {
@@ -1700,6 +1716,7 @@ static int da_check(const void* q, const void* k, const void* v, int64_t ld_q, i
                     int batch, int tokens, int heads, int kv_heads, int d) {
     if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || (d != 64 && d != 128)) return BRK_ATTR_ERROR;
     if (heads > 4096 || tokens > (1 << 22) || (int64_t)batch * tokens > (1 << 30)) return BRK_ATTR_ERROR;
+    if ((int64_t)batch * ((tokens + 127) / 128) * heads > 0x7fffffff) return BRK_ATTR_ERROR;
     if (!(cap >= 0.0f) || cap > 1e4f) return BRK_ATTR_ERROR;
     if (ld_q % 8 != 0 || ld_kv % 8 != 0 || ld_out % 8 != 0 || ld_q < (int64_t)heads * d || ld_kv < (int64_t)kv_heads * d || ld_out < (int64_t)heads * d)
         return BRK_ATTR_ERROR;
@@ -1794,9 +1811,11 @@ extern "C" int brk_doc_attn_bwd(const void* q, const void* k, const void* v, int
         set_error_message("brk_doc_attn_bwd: could not encode a tensor map");
         return BRK_CUDA_ERROR;
     }
-    const int64_t threads = (int64_t)batch * tokens * heads * (head_dim / 8);
-    doc_delta_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>((const __half*)out, (const __half*)d_out, ld_out, (float*)workspace, batch, tokens, heads,
-                                                                       head_dim);
+    const cudaError_t e = launch_pdl(doc_delta_kernel, batch * tokens, 256, 0, st, (const __half*)out, (const __half*)d_out, ld_out, (float*)workspace, tokens, heads, head_dim);
+    if (e != cudaSuccess) {
+        set_cuda_error(e, "doc_delta_kernel");
+        return BRK_CUDA_ERROR;
+    }
     rc = launch_status("doc_delta_kernel");
     if (rc) return rc;
     return da_dispatch(false, head_dim, t, p, st);
