@@ -840,6 +840,166 @@ ComputingReturn CUDATensor<DT>::op_randn(tensor_t self, float mean, float std, u
     return ret(brk_init_normal(mem_, (int64_t)self->items(), mean, std, seed, brk_dtype<DT>(), sptr()));
 }
 
+// ---- packed documents --------------------------------------------------------------------------------------------
+// self = the documents' numbers; the call is routed here through the backend of `spans`
+template <DataType DT>
+ComputingReturn CUDATensor<DT>::op_doc_plan(tensor_t self, tensor_t prompt, tensor_t ids, tensor_t spans, tensor_t target) {
+    ProfScope prof("doc_plan");
+    if (DT != DataType::Int) return OP_TODO_ERROR;
+    if (self->dtype() != DataType::Int || self->shape().dim() != 2) return OP_INPUT_ERROR;
+    const int64_t n = (int64_t)self->items();
+    if (prompt && (prompt->dtype() != DataType::Int || (int64_t)prompt->items() != n)) return OP_INPUT_ERROR;
+    if (ids && (ids->dtype() != DataType::Int || (int64_t)ids->items() != n)) return OP_INPUT_ERROR;
+    if (!dev_ok<DT>({spans}) || (int64_t)spans->items() != 4 * n) return OP_OUTPUT_ERROR;
+    if ((ids == nullptr) != (target == nullptr) || (target && (!dev_ok<DT>({target}) || (int64_t)target->items() != n))) return OP_OUTPUT_ERROR;
+    Scratch sc;
+    const int32_t* mask = int_on_device(self, sc);
+    const int32_t* marks = prompt ? int_on_device(prompt, sc) : nullptr;
+    const int32_t* tokens = ids ? int_on_device(ids, sc) : nullptr;
+    return ret(brk_doc_plan(mask, marks, tokens, (int)self->shape()[0], (int)self->shape()[1], (int32_t*)spans->data(),
+                            target ? (int32_t*)target->data() : nullptr, nullptr, sptr()));
+}
+
+namespace {
+
+// the head width of a fused projection [B, T, (heads + 2 kv_heads) d], 0 where the shape or the spans do not fit
+inline int doc_head_dim(const tensor_t& qkv, const tensor_t& spans, int heads, int kv_heads) {
+    if (qkv->shape().dim() != 3 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return 0;
+    const int64_t parts = (int64_t)heads + 2 * (int64_t)kv_heads, width = (int64_t)qkv->shape()[2];
+    if (width % parts != 0 || width / parts > 128) return 0;
+    if (!dev_ok<DataType::Int>({spans}) || (int64_t)spans->items() != 4 * (int64_t)(qkv->shape()[0] * qkv->shape()[1])) return 0;
+    return (int)(width / parts);
+}
+
+}  // namespace
+
+template <DataType DT>
+ComputingReturn CUDATensor<DT>::op_doc_attn(tensor_t self, tensor_t spans, tensor_t out, tensor_t lse, int heads, int kv_heads, int distance,
+                                            float cap) {
+    ProfScope prof("doc_attention_fwd");
+    if (DT != DataType::F16) return OP_TODO_ERROR;
+    const int d = doc_head_dim(self, spans, heads, kv_heads);
+    if (d == 0) return OP_INPUT_ERROR;
+    const int batch = (int)self->shape()[0], tokens = (int)self->shape()[1];
+    const int64_t row = (int64_t)self->shape()[2], n = (int64_t)batch * tokens, q_cols = (int64_t)heads * d, kv_cols = (int64_t)kv_heads * d;
+    if (!dev_ok<DT>({out}) || (int64_t)out->items() != n * q_cols) return OP_OUTPUT_ERROR;
+    if (!dev_ok<DataType::Float>({lse}) || (int64_t)lse->items() < n * heads) return OP_OUTPUT_ERROR;
+    const __half* q = (const __half*)mem_;
+    return ret(brk_doc_attn_fwd(q, q + q_cols, q + q_cols + kv_cols, row, row, out->data(), q_cols, (float*)lse->data(), (const int32_t*)spans->data(),
+                                distance ? device_slopes(heads) : nullptr, cap, batch, tokens, heads, kv_heads, d, sptr()));
+}
+
+template <DataType DT>
+ComputingReturn CUDATensor<DT>::op_doc_attn_backward(tensor_t self, tensor_t qkv, tensor_t out, tensor_t lse, tensor_t spans, tensor_t dqkv,
+                                                     int heads, int kv_heads, int distance, float cap) {
+    ProfScope prof("doc_attention_bwd");
+    if (DT != DataType::F16) return OP_TODO_ERROR;
+    if (!dev_ok<DT>({qkv, out}) || !dev_ok<DataType::Float>({lse})) return OP_INPUT_ERROR;
+    const int d = doc_head_dim(qkv, spans, heads, kv_heads);
+    if (d == 0) return OP_INPUT_ERROR;
+    const int batch = (int)qkv->shape()[0], tokens = (int)qkv->shape()[1];
+    const int64_t row = (int64_t)qkv->shape()[2], n = (int64_t)batch * tokens, q_cols = (int64_t)heads * d, kv_cols = (int64_t)kv_heads * d;
+    if ((int64_t)out->items() != n * q_cols || self->items() != out->items() || (int64_t)lse->items() < n * heads) return OP_INPUT_ERROR;
+    if (!dev_ok<DT>({dqkv}) || dqkv->items() != qkv->items()) return OP_OUTPUT_ERROR;
+    const size_t need = brk_doc_attn_bwd_workspace_bytes(batch, tokens, heads);
+    if (need > ComputingContext::workspace_size) return OP_ATTR_ERROR;
+    const __half* q = (const __half*)qkv->data();
+    __half* g = (__half*)dqkv->data();
+    return ret(brk_doc_attn_bwd(q, q + q_cols, q + q_cols + kv_cols, row, row, out->data(), mem_, q_cols, (const float*)lse->data(), g, row,
+                                g + q_cols, g + q_cols + kv_cols, row, (const int32_t*)spans->data(), distance ? device_slopes(heads) : nullptr,
+                                cap, batch, tokens, heads, kv_heads, d, ComputingContext::cuda_workspace, ComputingContext::workspace_size, sptr()));
+}
+
+// ---- activations kept in 8 bits ------------------------------------------------------------------------------------
+namespace {
+
+struct KeptShape {
+    int64_t rows, cols;
+};
+inline KeptShape kept_shape(const tensor_t& x) {
+    const int64_t cols = (int64_t)x->shape().vec().back();
+    return {cols > 0 ? (int64_t)x->items() / cols : 0, cols};
+}
+// `kept` has room for a byte per value and `steps` for a scale per 128 columns
+inline bool kept_fits(const KeptShape& s, const tensor_t& kept, const tensor_t& steps) {
+    return dev_ok<DataType::Int>({kept}) && dev_ok<DataType::Float>({steps}) && (int64_t)kept->items() >= (s.rows * s.cols + 3) / 4 &&
+           (int64_t)steps->items() >= s.rows * ((s.cols + 127) / 128);
+}
+
+}  // namespace
+
+template <DataType DT>
+ComputingReturn CUDATensor<DT>::op_act8_pack(tensor_t self, tensor_t kept, tensor_t steps) {
+    ProfScope prof("act8_pack");
+    if (DT == DataType::Int) return OP_TODO_ERROR;
+    const KeptShape s = kept_shape(self);
+    if (!kept_fits(s, kept, steps)) return OP_OUTPUT_ERROR;
+    return ret(brk_act8_pack(mem_, (int8_t*)kept->data(), (float*)steps->data(), s.rows, s.cols, brk_dtype<DT>(), sptr()));
+}
+
+template <DataType DT>
+ComputingReturn CUDATensor<DT>::op_act8_unpack(tensor_t self, tensor_t kept, tensor_t steps) {
+    ProfScope prof("act8_unpack");
+    if (DT == DataType::Int) return OP_TODO_ERROR;
+    const KeptShape s = kept_shape(self);
+    if (!kept_fits(s, kept, steps)) return OP_INPUT_ERROR;
+    return ret(brk_act8_unpack((const int8_t*)kept->data(), (const float*)steps->data(), mem_, s.rows, s.cols, brk_dtype<DT>(), sptr()));
+}
+
+template <DataType DT>
+ComputingReturn CUDATensor<DT>::op_gelu_act8(tensor_t self, tensor_t dst, tensor_t kept, tensor_t steps) {
+    ProfScope prof("gelu_fwd");
+    if (DT == DataType::Int) return OP_TODO_ERROR;
+    const KeptShape s = kept_shape(self);
+    if (!dev_ok<DT>({dst}) || dst->items() != self->items() || !kept_fits(s, kept, steps)) return OP_OUTPUT_ERROR;
+    return ret(brk_gelu_fwd_act8(mem_, dst->data(), (int8_t*)kept->data(), (float*)steps->data(), s.rows, s.cols, brk_dtype<DT>(), sptr()));
+}
+
+template <DataType DT>
+ComputingReturn CUDATensor<DT>::op_gelu_act8_backward(tensor_t self, tensor_t kept, tensor_t steps, tensor_t x_g, tensor_t y) {
+    ProfScope prof("gelu_bwd");
+    if (DT == DataType::Int) return OP_TODO_ERROR;
+    const KeptShape s = kept_shape(self);
+    if (!kept_fits(s, kept, steps)) return OP_INPUT_ERROR;
+    if (!dev_ok<DT>({x_g}) || x_g->items() != self->items()) return OP_OUTPUT_ERROR;
+    if (y && (!dev_ok<DT>({y}) || y->items() != self->items())) return OP_OUTPUT_ERROR;
+    return ret(brk_gelu_bwd_act8(mem_, (const int8_t*)kept->data(), (const float*)steps->data(), x_g->data(), y ? y->data() : nullptr, s.rows,
+                                 s.cols, brk_dtype<DT>(), sptr()));
+}
+
+template <DataType DT>
+ComputingReturn CUDATensor<DT>::op_layernorm_act8(tensor_t self, tensor_t var, tensor_t scale, tensor_t bias, tensor_t y, tensor_t kept,
+                                                  tensor_t steps, float eps) {
+    ProfScope prof("layernorm_fwd");
+    if (DT == DataType::Int) return OP_TODO_ERROR;
+    const KeptShape s = kept_shape(self);
+    if (!dev_ok<DT>({scale, bias}) || (int64_t)scale->items() != s.cols || (int64_t)bias->items() != s.cols) return OP_INPUT_ERROR;
+    if (!dev_ok<DT>({y}) || y->items() != self->items() || !dev_ok<DataType::Float>({var}) || (int64_t)var->items() < s.rows) return OP_OUTPUT_ERROR;
+    if (!kept_fits(s, kept, steps)) return OP_OUTPUT_ERROR;
+    return ret(brk_layernorm_fwd_act8(mem_, scale->data(), bias->data(), y->data(), (int8_t*)kept->data(), (float*)steps->data(),
+                                      (float*)var->data(), s.rows, s.cols, eps, brk_dtype<DT>(), sptr()));
+}
+
+template <DataType DT>
+ComputingReturn CUDATensor<DT>::op_layernorm_act8_backward(tensor_t self, tensor_t scale, tensor_t bias, tensor_t var, tensor_t kept,
+                                                           tensor_t steps, tensor_t dscale, tensor_t dbias, tensor_t din, tensor_t y,
+                                                           tensor_t residual) {
+    ProfScope prof("layernorm_bwd");
+    if (DT == DataType::Int) return OP_TODO_ERROR;
+    const KeptShape s = kept_shape(self);
+    if (!dev_ok<DT>({scale, bias}) || !dev_ok<DataType::Float>({var}) || !kept_fits(s, kept, steps)) return OP_INPUT_ERROR;
+    if ((int64_t)scale->items() != s.cols || (int64_t)bias->items() != s.cols || (int64_t)var->items() < s.rows) return OP_INPUT_ERROR;
+    if (residual && (!dev_ok<DT>({residual}) || residual->items() != self->items())) return OP_INPUT_ERROR;
+    if (!dev_ok<DT>({dscale, dbias, din}) || din->items() != self->items()) return OP_OUTPUT_ERROR;
+    if ((int64_t)dscale->items() != s.cols || (int64_t)dbias->items() != s.cols) return OP_OUTPUT_ERROR;
+    if (y && (!dev_ok<DT>({y}) || y->items() != self->items())) return OP_OUTPUT_ERROR;
+    if (brk_layernorm_bwd_act8_workspace_bytes(s.rows, s.cols) > ComputingContext::workspace_size) return OP_ATTR_ERROR;
+    return ret(brk_layernorm_bwd_act8(mem_, scale->data(), bias->data(), (const float*)var->data(), (const int8_t*)kept->data(),
+                                      (const float*)steps->data(), residual ? residual->data() : nullptr, dscale->data(), dbias->data(),
+                                      din->data(), y ? y->data() : nullptr, s.rows, s.cols, ComputingContext::cuda_workspace,
+                                      ComputingContext::workspace_size, ComputingContext::grad_accumulate, brk_dtype<DT>(), sptr()));
+}
+
 template struct CUDATensor<DataType::Float>;
 template struct CUDATensor<DataType::F16>;
 template struct CUDATensor<DataType::Int>;

@@ -217,6 +217,65 @@ BR_WORD(FlashAttnBackward, {
     auto t = pop_tensors<6>(stack);
     t[0]->op_flash_attn_backward(t[0], t[1], t[2], t[3], t[4], t[5], heads);
 })
+// ( mask prompt ids spans target -- )  packed documents: mask numbers them (0 = padding), prompt is non-zero on the prompts' tokens
+BR_WORD(DocPlan, {
+    auto t = pop_tensors<5>(stack);
+    t[0]->op_doc_plan(t[0], t[1], t[2], t[3], t[4]);
+})
+// ( qkv spans out lse heads kv_heads distance cap -- )
+BR_WORD(DocAttn, {
+    float cap = (float)stack.pop_number();
+    int distance = (int)stack.pop_number();
+    int kv_heads = (int)stack.pop_number();
+    int heads = (int)stack.pop_number();
+    auto t = pop_tensors<4>(stack);
+    t[0]->op_doc_attn(t[0], t[1], t[2], t[3], heads, kv_heads, distance, cap);
+})
+// ( dout qkv out lse spans dqkv heads kv_heads distance cap -- )
+BR_WORD(DocAttnBackward, {
+    float cap = (float)stack.pop_number();
+    int distance = (int)stack.pop_number();
+    int kv_heads = (int)stack.pop_number();
+    int heads = (int)stack.pop_number();
+    auto t = pop_tensors<6>(stack);
+    t[0]->op_doc_attn_backward(t[0], t[1], t[2], t[3], t[4], t[5], heads, kv_heads, distance, cap);
+})
+// ( x kept steps -- )  x in 8 bits
+BR_WORD(Act8Pack, {
+    auto t = pop_tensors<3>(stack);
+    t[0]->op_act8_pack(t[0], t[1], t[2]);
+})
+// ( x kept steps -- )  x <- the kept values
+BR_WORD(Act8Unpack, {
+    auto t = pop_tensors<3>(stack);
+    t[0]->op_act8_unpack(t[0], t[1], t[2]);
+})
+// ( x y kept steps -- )
+BR_WORD(GeluAct8, {
+    auto t = pop_tensors<4>(stack);
+    t[0]->op_gelu_act8(t[0], t[1], t[2], t[3]);
+})
+// ( dy kept steps x_g y -- )  y = the forward's output again
+BR_WORD(GeluAct8Backward, {
+    auto t = pop_tensors<5>(stack);
+    t[0]->op_gelu_act8_backward(t[0], t[1], t[2], t[3], t[4]);
+})
+// ( x var scale bias y kept steps eps -- )
+BR_WORD(LayernormAct8, {
+    float eps = (float)stack.pop_number();
+    auto t = pop_tensors<7>(stack);
+    t[0]->op_layernorm_act8(t[0], t[1], t[2], t[3], t[4], t[5], t[6], eps);
+})
+// ( dy scale bias var kept steps dscale dbias din y -- )  y = the forward's output again
+BR_WORD(LayernormAct8Backward, {
+    auto t = pop_tensors<10>(stack);
+    t[0]->op_layernorm_act8_backward(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], nullptr);
+})
+// ( dy scale bias var kept steps dscale dbias din y residual -- )  and residual is added to din
+BR_WORD(LayernormAct8BackwardResidual, {
+    auto t = pop_tensors<11>(stack);
+    t[0]->op_layernorm_act8_backward(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], t[10]);
+})
 // ( x w b residual y -- )
 BR_WORD(LinearResidual, {
     auto t = pop_tensors<5>(stack);
@@ -303,12 +362,12 @@ BR_WORD(LossBackwardW, {
     t[0]->op_loss_backward_w(t[0], t[1], t[2]);
 })
 // ( -- code )  waits for the device; 0 when no tensor-core kernel gave up a bounded wait and no optimizer launch met a
-// non-finite gradient since the last query, else 256 * (Adam status) + 16 * (GEMM status) + (attention status)
+// non-finite gradient since the last query, else 256 * (Adam status) + 16 * (GEMM status) + (attention status, of either kind)
 BR_WORD(KernelStatus, {
     int code = 0;
     if (ComputingContext::booted) {
         BR_CUDA_CHECK(cudaStreamSynchronize(ComputingContext::cuda_stream));
-        code = 256 * brk_adam_status() + 16 * brk_gemm_f16_status() + brk_flash_attn_status();
+        code = 256 * brk_adam_status() + 16 * brk_gemm_f16_status() + (brk_flash_attn_status() | brk_doc_attn_status());
     }
     stack.push_number((double)code);
 })
@@ -485,6 +544,16 @@ void load_nn_words(Enviroment& env) {
     env.insert_native_word("io.replica", IoReplica::creator);
     env.insert_native_word("op.flash_attn", FlashAttn::creator);
     env.insert_native_word("op.flash_attn_backward", FlashAttnBackward::creator);
+    env.insert_native_word("op.doc_plan", DocPlan::creator);
+    env.insert_native_word("op.doc_attn", DocAttn::creator);
+    env.insert_native_word("op.doc_attn_backward", DocAttnBackward::creator);
+    env.insert_native_word("op.act8_pack", Act8Pack::creator);
+    env.insert_native_word("op.act8_unpack", Act8Unpack::creator);
+    env.insert_native_word("op.gelu_act8", GeluAct8::creator);
+    env.insert_native_word("op.gelu_act8_backward", GeluAct8Backward::creator);
+    env.insert_native_word("op.layernorm_act8", LayernormAct8::creator);
+    env.insert_native_word("op.layernorm_act8_backward", LayernormAct8Backward::creator);
+    env.insert_native_word("op.layernorm_act8_backward_residual", LayernormAct8BackwardResidual::creator);
     env.insert_native_word("op.linear_residual", LinearResidual::creator);
     env.insert_native_word("op.linear_gelu", LinearGelu::creator);
     env.insert_native_word("op.embed", Embed::creator);

@@ -128,6 +128,30 @@ struct TransformerComputing {
                                                    tensor_t x_g, tensor_t lm_head_g, tensor_t loss_out, int defer_weight) { return OP_TODO_ERROR; }
     // self = the band holding dlogits [rows, vocab] ; lm_head_g += dlogits^T x
     virtual ComputingReturn op_loss_backward_w(tensor_t self, tensor_t x, tensor_t lm_head_g) { return OP_TODO_ERROR; }
+    // Packed documents (brk_doc_plan).  self = Int [B,T], the number of each token's document (0 = padding); prompt Int [B,T], non-zero
+    // on the tokens of a prompt (may be null); spans Int [B,T,4] on the device.  With ids Int [B,T], target Int [B,T] on the
+    // device receives the next token's id where it counts and -100 elsewhere (both null otherwise).
+    virtual ComputingReturn op_doc_plan(tensor_t self, tensor_t prompt, tensor_t ids, tensor_t spans, tensor_t target) { return OP_TODO_ERROR; }
+    // Attention over packed documents.  self = qkv [B,T,(heads + 2 kv_heads) d] (q | k | v), out [B,T,heads d], lse [B,heads,T]
+    // fp32; distance != 0 subtracts the ALiBi slope times the distance, cap > 0 bounds the scores by cap tanh(x / cap).
+    virtual ComputingReturn op_doc_attn(tensor_t self, tensor_t spans, tensor_t out, tensor_t lse, int heads, int kv_heads,
+                                        int distance, float cap) { return OP_TODO_ERROR; }
+    // self = d_out [B,T,heads d]; writes dqkv in the layout of qkv.
+    virtual ComputingReturn op_doc_attn_backward(tensor_t self, tensor_t qkv, tensor_t out, tensor_t lse, tensor_t spans, tensor_t dqkv, int heads, int kv_heads,
+                                        int distance, float cap) { return OP_TODO_ERROR; }
+    // Activations kept in 8 bits, a scale per 128 columns of the last dimension: kept = Int tensor of at least items / 4 items (a
+    // byte per value), steps = Float [rows, ceil(cols / 128)], both on the device.
+    virtual ComputingReturn op_act8_pack(tensor_t self, tensor_t kept, tensor_t steps) { return OP_TODO_ERROR; }
+    // self <- the kept values
+    virtual ComputingReturn op_act8_unpack(tensor_t self, tensor_t kept, tensor_t steps) { return OP_TODO_ERROR; }
+    // op_gelu that keeps its input in 8 bits
+    virtual ComputingReturn op_gelu_act8(tensor_t self, tensor_t dst, tensor_t kept, tensor_t steps) { return OP_TODO_ERROR; }
+    // self = dy ; x_g = dy gelu'(kept input) ; y (may be null) = gelu(kept input) again
+    virtual ComputingReturn op_gelu_act8_backward(tensor_t self, tensor_t kept, tensor_t steps, tensor_t x_g, tensor_t y) { return OP_TODO_ERROR; }
+    // op_layernorm that keeps the normalised rows in 8 bits
+    virtual ComputingReturn op_layernorm_act8(tensor_t self, tensor_t var, tensor_t scale, tensor_t bias, tensor_t y, tensor_t kept, tensor_t steps, float eps) { return OP_TODO_ERROR; }
+    // op_layernorm_backward from them; y (may be null) = the forward's output again, residual (may be null) is added to din
+    virtual ComputingReturn op_layernorm_act8_backward(tensor_t self, tensor_t scale, tensor_t bias, tensor_t var, tensor_t kept, tensor_t steps, tensor_t dscale, tensor_t dbias, tensor_t din, tensor_t y, tensor_t residual) { return OP_TODO_ERROR; }
 };
 
 }  // namespace br

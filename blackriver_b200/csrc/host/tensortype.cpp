@@ -267,6 +267,52 @@ ComputingReturn TensorType::op_loss_backward_w(tensor_t self, tensor_t x, tensor
     auto r = impl_->op_loss_backward_w(self, x, lm_head_g);
     op_check(r, "loss_backward_w");
 }
+ComputingReturn TensorType::op_doc_plan(tensor_t self, tensor_t prompt, tensor_t ids, tensor_t spans, tensor_t target) {
+    SELF_CHECK();
+    if (!spans) op_check(OP_OUTPUT_ERROR, "doc_plan");
+    auto r = spans->impl_->op_doc_plan(self, prompt, ids, spans, target);
+    op_check(r, "doc_plan");
+}
+ComputingReturn TensorType::op_doc_attn(tensor_t self, tensor_t spans, tensor_t out, tensor_t lse, int heads, int kv_heads, int distance, float cap) {
+    SELF_CHECK();
+    auto r = impl_->op_doc_attn(self, spans, out, lse, heads, kv_heads, distance, cap);
+    op_check(r, "doc_attn");
+}
+ComputingReturn TensorType::op_doc_attn_backward(tensor_t self, tensor_t qkv, tensor_t out, tensor_t lse, tensor_t spans, tensor_t dqkv, int heads, int kv_heads, int distance, float cap) {
+    SELF_CHECK();
+    auto r = impl_->op_doc_attn_backward(self, qkv, out, lse, spans, dqkv, heads, kv_heads, distance, cap);
+    op_check(r, "doc_attn_backward");
+}
+ComputingReturn TensorType::op_act8_pack(tensor_t self, tensor_t kept, tensor_t steps) {
+    SELF_CHECK();
+    auto r = impl_->op_act8_pack(self, kept, steps);
+    op_check(r, "act8_pack");
+}
+ComputingReturn TensorType::op_act8_unpack(tensor_t self, tensor_t kept, tensor_t steps) {
+    SELF_CHECK();
+    auto r = impl_->op_act8_unpack(self, kept, steps);
+    op_check(r, "act8_unpack");
+}
+ComputingReturn TensorType::op_gelu_act8(tensor_t self, tensor_t dst, tensor_t kept, tensor_t steps) {
+    SELF_CHECK();
+    auto r = impl_->op_gelu_act8(self, dst, kept, steps);
+    op_check(r, "gelu_act8");
+}
+ComputingReturn TensorType::op_gelu_act8_backward(tensor_t self, tensor_t kept, tensor_t steps, tensor_t x_g, tensor_t y) {
+    SELF_CHECK();
+    auto r = impl_->op_gelu_act8_backward(self, kept, steps, x_g, y);
+    op_check(r, "gelu_act8_backward");
+}
+ComputingReturn TensorType::op_layernorm_act8(tensor_t self, tensor_t var, tensor_t scale, tensor_t bias, tensor_t y, tensor_t kept, tensor_t steps, float eps) {
+    SELF_CHECK();
+    auto r = impl_->op_layernorm_act8(self, var, scale, bias, y, kept, steps, eps);
+    op_check(r, "layernorm_act8");
+}
+ComputingReturn TensorType::op_layernorm_act8_backward(tensor_t self, tensor_t scale, tensor_t bias, tensor_t var, tensor_t kept, tensor_t steps, tensor_t dscale, tensor_t dbias, tensor_t din, tensor_t y, tensor_t residual) {
+    SELF_CHECK();
+    auto r = impl_->op_layernorm_act8_backward(self, scale, bias, var, kept, steps, dscale, dbias, din, y, residual);
+    op_check(r, "layernorm_act8_backward");
+}
 
 ComputingReturn TensorType::io_load(tensor_t self, const char* fileName) {
     SELF_CHECK();

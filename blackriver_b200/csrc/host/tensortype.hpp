@@ -160,6 +160,15 @@ struct TensorType : public TransformerComputing {
     ComputingReturn op_linear_backward_w(tensor_t self, tensor_t x, tensor_t weight_g, tensor_t bias_g) override;
     ComputingReturn op_loss_backward_async(tensor_t self, tensor_t ids, tensor_t mask, tensor_t lm_head, tensor_t all_logits, tensor_t x_g, tensor_t lm_head_g, tensor_t loss_out, int defer_weight) override;
     ComputingReturn op_loss_backward_w(tensor_t self, tensor_t x, tensor_t lm_head_g) override;
+    ComputingReturn op_doc_plan(tensor_t self, tensor_t prompt, tensor_t ids, tensor_t spans, tensor_t target) override;
+    ComputingReturn op_doc_attn(tensor_t self, tensor_t spans, tensor_t out, tensor_t lse, int heads, int kv_heads, int distance, float cap) override;
+    ComputingReturn op_doc_attn_backward(tensor_t self, tensor_t qkv, tensor_t out, tensor_t lse, tensor_t spans, tensor_t dqkv, int heads, int kv_heads, int distance, float cap) override;
+    ComputingReturn op_act8_pack(tensor_t self, tensor_t kept, tensor_t steps) override;
+    ComputingReturn op_act8_unpack(tensor_t self, tensor_t kept, tensor_t steps) override;
+    ComputingReturn op_gelu_act8(tensor_t self, tensor_t dst, tensor_t kept, tensor_t steps) override;
+    ComputingReturn op_gelu_act8_backward(tensor_t self, tensor_t kept, tensor_t steps, tensor_t x_g, tensor_t y) override;
+    ComputingReturn op_layernorm_act8(tensor_t self, tensor_t var, tensor_t scale, tensor_t bias, tensor_t y, tensor_t kept, tensor_t steps, float eps) override;
+    ComputingReturn op_layernorm_act8_backward(tensor_t self, tensor_t scale, tensor_t bias, tensor_t var, tensor_t kept, tensor_t steps, tensor_t dscale, tensor_t dbias, tensor_t din, tensor_t y, tensor_t residual) override;
 
     ComputingReturn io_load(tensor_t self, const char* fileName) override;
     ComputingReturn io_save(tensor_t self, const char* fileName) override;

@@ -197,6 +197,99 @@ def train_words():
     return "\n".join(L) + "\n"
 
 
+def packed_words(n_layers, batch, tokens, hidden, heads, cap=0.0):
+    """Decoder layers on packed documents, whose forward keeps its activations in 8 bits.  fp16, ALiBi, optionally capped
+    scores; follows init_words(..., dtype="half") in an environment of n_layers + 1 hash tables: table 0 holds what the layers
+    share, table i what layer i owns.
+
+    create_packed     everything; table 0 then has mask, prompt, ids, target [batch, tokens] and packed_in, packed_out,
+                      packed_out_g, packed_in_g [batch, tokens, hidden] (in and out may be one buffer, and so may the gradients)
+    packed_plan       spans and next-token targets from mask (document numbers, 0 = padding), prompt and ids
+    packed_forward    packed_in -> packed_out; a layer keeps 14 bytes per token and hidden column where fused_words keeps 28
+    packed_backward   packed_out_g -> packed_in_g and the layers' gradients
+
+    The reference has one sequence per row and keeps every activation in fp32 (bloomz-7b/train.words:10-227)."""
+    assert n_layers >= 1 and hidden % heads == 0
+    n = batch * tokens
+    L = []
+    w = L.append
+
+    def g(*names):
+        return " ".join(_get(x) for x in names)
+
+    def act(name, cols):
+        w(f'    {batch} {tokens} {cols * hidden} 3 "cuda" "half" op.create "{name}" !')
+
+    scratch = (("xattn_in", 1), ("xb", 1), ("xa", 1), ("x4a", 4), ("x4b", 4), ("dh1", 1), ("dh2", 1), ("dqkv", 3))
+    w("%def create_packed_layer")
+    w("    create_layer_weight create_layer_grad")
+    act("qkv", 3)
+    act("attn_out", 1)
+    w(f'    {batch} {heads} {tokens} 3 "cuda" "float" op.create "lse" !')
+    for name in ("input_ln_var", "post_ln_var"):
+        w(f'    {n} 1 "cuda" "float" op.create "{name}" !')
+    for name, cols in (("input_ln", hidden), ("post_ln", hidden), ("h_to_4h", 4 * hidden)):
+        w(f'    {(n * cols + 3) // 4} 1 "cuda" "int" op.create "{name}.kept" !')
+        w(f'    {n} {(cols + 127) // 128} 2 "cuda" "float" op.create "{name}.steps" !')
+    w("%end")
+    w("%def create_packed")
+    w('    0 # "cuda" $DEVICE !')
+    for name in ("mask", "prompt", "ids", "target"):
+        w(f'    {batch} {tokens} 2 "cuda" "int" op.create "{name}" !')
+    w(f'    {batch} {tokens} 4 3 "cuda" "int" op.create "spans" !')
+    for name, cols in scratch + (("hA", 1), ("hB", 1), ("gA", 1), ("gB", 1)):
+        act(name, cols)
+    shared = ["$DEVICE", "DTYPE", "LN_EPS", "HIDDEN_SIZE", "HIDDEN_SIZE_x3", "HIDDEN_SIZE_x4", "HIDDEN_SQUARE", "spans"] + [x for x, _ in scratch]
+    for i in range(1, n_layers + 1):
+        ends = ("A", "B") if i % 2 else ("B", "A")           # a layer reads one buffer of each pair and writes the other
+        for name, source in [(x, x) for x in shared] + [("xinput", "h" + ends[0]), ("xout", "h" + ends[1]), ("xin_g", "g" + ends[0]),
+                                                        ("yout_g", "g" + ends[1])]:
+            w(f'    0 # "{source}" @ {i} # "{name}" !')
+        w(f"    {i} # create_packed_layer")
+    for name, i, own in (("packed_in", 1, "xinput"), ("packed_in_g", 1, "xin_g"), ("packed_out", n_layers, "xout"), ("packed_out_g", n_layers, "yout_g")):
+        w(f'    {i} # "{own}" @ 0 # "{name}" !')
+    w("%end")
+    w("%def packed_plan")
+    w(f'    {g("mask", "prompt", "ids", "spans", "target")} op.doc_plan')
+    w("%end")
+
+    attn = f"{heads} {heads} 1 {float(cap)}"
+    w("%def packed_layer_forward")
+    w(f'    {g("xinput", "input_ln_var", "input_layernorm.weight", "input_layernorm.bias", "xattn_in", "input_ln.kept", "input_ln.steps", "LN_EPS")} op.layernorm_act8')
+    w(f'    {g("xattn_in", "query_key_value.weight", "query_key_value.bias", "qkv")} op.linear')
+    w(f'    {g("qkv", "spans", "attn_out", "lse")} {attn} op.doc_attn')
+    w(f'    {g("attn_out", "dense.weight", "dense.bias", "xinput", "xa")} op.linear_residual')
+    w(f'    {g("xa", "post_ln_var", "post_attention_layernorm.weight", "post_attention_layernorm.bias", "xb", "post_ln.kept", "post_ln.steps", "LN_EPS")} op.layernorm_act8')
+    w(f'    {g("xb", "dense_h_to_4h.weight", "dense_h_to_4h.bias", "x4a")} op.linear')
+    w(f'    {g("x4a", "x4b", "h_to_4h.kept", "h_to_4h.steps")} op.gelu_act8')
+    w(f'    {g("x4b", "dense_4h_to_h.weight", "dense_4h_to_h.bias", "xa", "xout")} op.linear_residual')
+    w("%end")
+    w("%def packed_layer_backward")
+    w(f'    {g("yout_g", "dense_4h_to_h.weight", "x4a")} op.linear_backward_x')
+    w(f'    {g("x4a", "h_to_4h.kept", "h_to_4h.steps", "x4a", "x4b")} op.gelu_act8_backward')
+    w(f'    {g("yout_g", "x4b", "dense_4h_to_h.weight_g", "dense_4h_to_h.bias_g")} op.linear_backward_w')
+    w(f'    {g("x4a", "dense_h_to_4h.weight", "dh1")} op.linear_backward_x')
+    w(f'    {g("dh1", "post_attention_layernorm.weight", "post_attention_layernorm.bias", "post_ln_var", "post_ln.kept", "post_ln.steps", "post_attention_layernorm.weight_g", "post_attention_layernorm.bias_g", "dh2", "xb", "yout_g")} op.layernorm_act8_backward_residual')
+    w(f'    {g("x4a", "xb", "dense_h_to_4h.weight_g", "dense_h_to_4h.bias_g")} op.linear_backward_w')
+    w(f'    {g("dh2", "attn_out", "dense.weight", "dense.bias", "dh1", "dense.weight_g", "dense.bias_g")} op.linear_backward')
+    w(f'    {g("dh1", "qkv", "attn_out", "lse", "spans", "dqkv")} {attn} op.doc_attn_backward')
+    w(f'    {g("dqkv", "query_key_value.weight", "dh1")} op.linear_backward_x')
+    w(f'    {g("dh1", "input_layernorm.weight", "input_layernorm.bias", "input_ln_var", "input_ln.kept", "input_ln.steps", "input_layernorm.weight_g", "input_layernorm.bias_g", "xin_g", "xattn_in", "dh2")} op.layernorm_act8_backward_residual')
+    w(f'    {g("dqkv", "xattn_in", "query_key_value.weight_g", "query_key_value.bias_g")} op.linear_backward_w')
+    w("%end")
+    w("%def packed_forward")
+    for i in range(1, n_layers + 1):
+        w(f"    {i} # packed_layer_forward")
+    w("    0 #")
+    w("%end")
+    w("%def packed_backward")
+    for i in range(n_layers, 0, -1):
+        w(f"    {i} # packed_layer_backward")
+    w("    0 #")
+    w("%end")
+    return "\n".join(L) + "\n"
+
+
 def var_elements(batch, tokens, hidden, heads, vocab, logits_rows):
     """Elements `create_var` must reserve for `create_dynamic(batch, tokens)` plus a logits band."""
     s = batch * tokens * hidden
