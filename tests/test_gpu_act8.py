@@ -223,3 +223,14 @@ def test_captured_and_on_another_stream():
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, again))
     assert not torch.equal(got[0], want[0])
+
+
+@pytest.mark.parametrize("cols", [256, 37])
+def test_gelu_of_values_whose_square_overflows(cols):
+    o = ops()
+    x = torch.full((3, cols), 1e25, device="cuda")
+    x[:, ::2] = -1e25
+    y, q, scale = o.gelu_act8(x)
+    assert torch.equal(y, torch.where(x > 0, x, torch.zeros_like(x)))
+    dx = o.gelu_backward_act8(torch.full_like(x, 3.0), q, scale)
+    assert torch.equal(dx, torch.where(x > 0, 3.0, 0.0))
