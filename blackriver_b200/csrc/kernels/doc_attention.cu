@@ -923,7 +923,7 @@ template <int D>
 struct DkvSmem {
     static constexpr uint32_t KV = 128 * D * 2, SUB = DA_SUB * D * 2;
     static constexpr int STAGES = 3;
-    static constexpr size_t BYTES = 1024 + 2 * KV + 2 * STAGES * SUB + 16 * DA_PATCH + 2 * 2 * DA_SUB * sizeof(float) + sizeof(DaTable) + 256;
+    static constexpr size_t BYTES = 1024 + 2 * KV + 2 * STAGES * SUB + 16 * DA_PATCH + 4 * 2 * DA_SUB * sizeof(float) + sizeof(DaTable) + 256;
 };
 
 // Transposed scores S^T = K Q^T and dP^T = V dO^T (a row owner is a key), so that P^T and dS^T are the A operands of
@@ -946,8 +946,8 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     unsigned char* sQ = sV + S::KV;
     unsigned char* sDO = sQ + S::STAGES * S::SUB;
     unsigned char* sOut = sDO + S::STAGES * S::SUB;     // a patch for each owner warp
-    float* stat = reinterpret_cast<float*>(sOut + 16 * DA_PATCH);       // [2][lse2 x 64 | delta x 64]
-    DaTable* table = reinterpret_cast<DaTable*>(stat + 2 * 2 * DA_SUB);
+    float* stat = reinterpret_cast<float*>(sOut + 16 * DA_PATCH);       // [team][2][lse2 x 64 | delta x 64]
+    DaTable* table = reinterpret_cast<DaTable*>(stat + 4 * 2 * DA_SUB);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + 1);
     uint64_t* kv_full = bars;
     uint64_t* kv_empty = bars + 1;
@@ -972,7 +972,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 16);
+            mbar_init(&p_full[i], 8);
         }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 16);
@@ -1102,9 +1102,12 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             if (!ok && issuer) atomicExch(&g_doc_error, 12);
         }
     } else {
-        // ---------------- row owners: four threads per key, 16 of the 64 query columns each ----------------
-        const int quarter = warp & 3, part = (warp - 2) >> 2;
-        const int r = quarter * 32 + lane, c0 = part * 16;
+        // ---------------- row owners ----------------
+        // Two groups of eight warps take the steps in turn, each with a score buffer of its own, so that one loads and stores
+        // while the other computes; in a group two threads share a key, 32 of the 64 query columns each.  The results are shared
+        // by all: a quarter of the columns each.
+        const int quarter = warp & 3, part = (warp - 2) >> 2, team = part >> 1, half = part & 1;
+        const int r = quarter * 32 + lane;
         const uint32_t tm = tmem_base + ((uint32_t)(quarter * 32) << 16);
         unsigned char* const patch = sOut + (warp - 2) * DA_PATCH;
         bool ok = true;
@@ -1112,14 +1115,20 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         Item m = {}, following = {};
         int4 next_span = make_int4(0, 0, 0, 0);
         float next = 0.0f, next_slope = 0.0f;
-        // A step's 64 log-sum-exps and 64 deltas, one for each of the first owners, fetched a step ahead as they are: arithmetic on
-        // them would wait for the load where it is issued.
+        // A step's 64 log-sum-exps and 64 deltas, one for each of the team's first owners, fetched a step ahead as they are:
+        // arithmetic on them would wait for the load where it is issued.  Step n of an item; the blocks repeat for every head.
         auto fetch = [&](const Item& of, int blk, int h) {
             const int i = blk * DA_SUB + (r & 63);
             next = 0.0f;
-            if (part == 0 && i < p.tokens) next = (r < 64 ? p.lse_in : p.delta)[((int64_t)of.b * p.heads + h) * p.tokens + i];
+            if (half == 0 && i < p.tokens) next = (r < 64 ? p.lse_in : p.delta)[((int64_t)of.b * p.heads + h) * p.tokens + i];
             if (BIAS) next_slope = p.slopes[h];
         };
+        // the team's first step of an item whose steps are counted from `from`
+        auto fetch_first = [&](const Item& of, uint32_t from) {
+            const int n = (from & 1) != (uint32_t)team, wide = of.r0.end - of.r0.begin;
+            if (n < of.n) fetch(of, of.r0.begin + (wide > 1 ? n : 0), of.head * group + (wide > 1 ? 0 : n));
+        };
+        auto team_meet = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + team) : "memory"); };
         auto fetch_span = [&]() {
             const int kj = following.t0 + r;
             // rows behind the sequence never force the masked path
@@ -1128,7 +1137,7 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         bool have = item_of(0, following);
         if (have) {
             fetch_span();
-            if (following.n > 0) fetch(following, following.r0.begin, following.head * group);
+            fetch_first(following, 0);
         }
         for (int round = 1; have; round++) {
             m = following;
@@ -1143,91 +1152,102 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     da_zero_row(p.dk + row * p.ld_dkv + m.head * D + part * (D / 4), D / 4);
                     da_zero_row(p.dv + row * p.ld_dkv + m.head * D + part * (D / 4), D / 4);
                 }
-                if (have && following.n > 0) fetch(following, following.r0.begin, following.head * group);
+                if (have) fetch_first(following, it0);
                 continue;
             }
             const int qlo = max(span.z, 0), qhi = live ? min(span.w, p.tokens) : span.w;
             int blk = m.r0.begin, h = m.head * group;
-            for (int n = 0; n < m.n; n++) {
-                const uint32_t i = it0 + n;
-                const int sb = i & 1, q0 = blk * DA_SUB;
-                const float slope2 = next_slope * LOG2E;
-                // negated, and the log-sum-exp in log2 units with the query's share of the bias
-                if (part == 0) stat[sb * 128 + r] = r < 64 ? fmaf(next, -LOG2E, -slope2 * (float)r) : -next;
+            auto advance = [&]() {
                 if (++blk == m.r0.end) {
                     blk = m.r0.begin;
                     h++;
                 }
-                if (n + 1 < m.n) fetch(m, blk, h);
-                else if (have && following.n > 0) fetch(following, following.r0.begin, following.head * group);
-                // orders this step's writes after every thread's reads two steps ago; every owner reaches it in every step,
-                // also one whose bounded wait gave up (it only skips the work)
-                asm volatile("bar.sync 1, 512;" ::: "memory");
+            };
+            const int first = (it0 & 1) != (uint32_t)team;
+            if (first) advance();
+            if (first >= m.n && have) fetch_first(following, it0 + m.n);
+            for (int n = first; n < m.n; n += 2) {
+                const uint32_t i = it0 + n;
+                const int sb = team, q0 = blk * DA_SUB;
+                float* const own = stat + (sb * 2 + ((i >> 1) & 1)) * 128;
+                const float slope2 = next_slope * LOG2E;
+                // negated, and the log-sum-exp in log2 units with the query's share of the bias
+                if (half == 0) own[r] = r < 64 ? fmaf(next, -LOG2E, -slope2 * (float)r) : -next;
+                advance();
+                advance();
+                if (n + 2 < m.n) fetch(m, blk, h);
+                else if (have) fetch_first(following, it0 + m.n);
+                // orders this step's writes after the team's reads two steps of its own ago; every owner of the team reaches it in
+                // every step, also one whose bounded wait gave up (it only skips the work)
+                team_meet();
                 if (ok) ok = mbar_wait(&s_full[sb], (i >> 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) continue;
                 tcgen05_fence_after();
-                const float4* nlse = reinterpret_cast<const float4*>(stat + sb * 128 + c0);
-                const float4* ndelta = nlse + 16;
-                float2 x[8], g[8];
-                tmem_ld_32x32b_x16(tm + sb * DA_SUB + c0, reinterpret_cast<float*>(x));
-                tmem_ld_32x32b_x16(tm + 128 + sb * DA_SUB + c0, reinterpret_cast<float*>(g));
-                tmem_ld_wait();
-                const float2 bias = both(slope2 * (float)(kj - q0));       // minus slope * (query - q0), which nlse holds
-                const bool inner = qlo <= q0 + c0 && qhi >= q0 + c0 + 16 && (!BIAS || kj <= q0 + c0);
-                const bool plain = __all_sync(0xffffffffu, inner);
-                bool near = true;
-                if (CAP) {
-                    float wide = 0.0f;
+#pragma unroll 1
+                for (int c0 = half * 32; c0 < half * 32 + 32; c0 += 16) {
+                    const float4* nlse = reinterpret_cast<const float4*>(own + c0);
+                    const float4* ndelta = nlse + 16;
+                    float2 x[8], g[8];
+                    tmem_ld_32x32b_x16(tm + sb * DA_SUB + c0, reinterpret_cast<float*>(x));
+                    tmem_ld_32x32b_x16(tm + 128 + sb * DA_SUB + c0, reinterpret_cast<float*>(g));
+                    tmem_ld_wait();
+                    const float2 bias = both(slope2 * (float)(kj - q0));       // minus slope * (query - q0), which nlse holds
+                    const bool inner = qlo <= q0 + c0 && qhi >= q0 + c0 + 16 && (!BIAS || kj <= q0 + c0);
+                    const bool plain = __all_sync(0xffffffffu, inner);
+                    bool near = true;
+                    if (CAP) {
+                        float wide = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) wide = max3(wide, fabsf(x[e].x), fabsf(x[e].y));
-                    near = __all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH);
-                }
-                auto step = [&](auto edge, auto reach) {
+                        for (int e = 0; e < 8; e++) wide = max3(wide, fabsf(x[e].x), fabsf(x[e].y));
+                        near = __all_sync(0xffffffffu, wide * p.cap_in <= TANH_REACH);
+                    }
+                    auto step = [&](auto edge, auto reach) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float4 l4 = nlse[e >> 1], d4 = ndelta[e >> 1];
+                            float2 off = e & 1 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+                            const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
+                            if (BIAS) off = __fadd2_rn(off, bias);
+                            const int far = q0 + c0 + 2 * e - kj;              // query - key
+                            if (BIAS && edge) {                                // a key ahead of the query: -slope (key - query)
+                                off.x += fminf(0.0f, 2.0f * slope2 * (float)far);
+                                off.y += fminf(0.0f, 2.0f * slope2 * (float)(far + 1));
+                            }
+                            float2 s, t;
+                            if (CAP) {
+                                t = reach ? da_capped_near(x[e], p, both(0.0f)) : da_capped_far(x[e], p);
+                                s = __fadd2_rn(t, off);
+                            } else {
+                                s = __ffma2_rn(x[e], both(p.scale_log2), off);
+                            }
+                            float2 pe = make_float2(fast_exp2(s.x), fast_exp2(s.y));
+                            float2 de = __fmul2_rn(pe, __fadd2_rn(g[e], nd));
+                            if (CAP) de = __fmul2_rn(de, __ffma2_rn(__fmul2_rn(t, both(p.cap_curve)), t, both(1.0f)));
+                            if (edge) {
+                                const int qi = q0 + c0 + 2 * e;
+                                if (!(qlo <= qi && qi < qhi)) pe.x = de.x = 0.0f;
+                                if (!(qlo <= qi + 1 && qi + 1 < qhi)) pe.y = de.y = 0.0f;
+                            }
+                            x[e].x = __uint_as_float(da_half2(pe.x, pe.y));
+                            g[e].x = __uint_as_float(da_half2(de.x, de.y));
+                        }
+                    };
+                    if (near) {
+                        if (plain) step(Flag<false>(), Flag<true>());
+                        else step(Flag<true>(), Flag<true>());
+                    } else {
+                        step(Flag<true>(), Flag<false>());
+                    }
+                    uint32_t wp[8], wd[8];
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float4 l4 = nlse[e >> 1], d4 = ndelta[e >> 1];
-                        float2 off = e & 1 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
-                        const float2 nd = e & 1 ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
-                        if (BIAS) off = __fadd2_rn(off, bias);
-                        const int far = q0 + c0 + 2 * e - kj;              // query - key
-                        if (BIAS && edge) {                                // a key ahead of the query: -slope (key - query)
-                            off.x += fminf(0.0f, 2.0f * slope2 * (float)far);
-                            off.y += fminf(0.0f, 2.0f * slope2 * (float)(far + 1));
-                        }
-                        float2 s, t;
-                        if (CAP) {
-                            t = reach ? da_capped_near(x[e], p, both(0.0f)) : da_capped_far(x[e], p);
-                            s = __fadd2_rn(t, off);
-                        } else {
-                            s = __ffma2_rn(x[e], both(p.scale_log2), off);
-                        }
-                        float2 pe = make_float2(fast_exp2(s.x), fast_exp2(s.y));
-                        float2 de = __fmul2_rn(pe, __fadd2_rn(g[e], nd));
-                        if (CAP) de = __fmul2_rn(de, __ffma2_rn(__fmul2_rn(t, both(p.cap_curve)), t, both(1.0f)));
-                        if (edge) {
-                            const int qi = q0 + c0 + 2 * e;
-                            if (!(qlo <= qi && qi < qhi)) pe.x = de.x = 0.0f;
-                            if (!(qlo <= qi + 1 && qi + 1 < qhi)) pe.y = de.y = 0.0f;
-                        }
-                        x[e].x = __uint_as_float(da_half2(pe.x, pe.y));
-                        g[e].x = __uint_as_float(da_half2(de.x, de.y));
+                        wp[e] = __float_as_uint(x[e].x);
+                        wd[e] = __float_as_uint(g[e].x);
                     }
-                };
-                if (near) {
-                    if (plain) step(Flag<false>(), Flag<true>());
-                    else step(Flag<true>(), Flag<true>());
-                } else {
-                    step(Flag<true>(), Flag<false>());
+                    tmem_st_32x32b_x8(tm + sb * DA_SUB + c0, wp);
+                    tmem_st_32x32b_x8(tm + 128 + sb * DA_SUB + c0, wd);
                 }
-                uint32_t wp[8], wd[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    wp[e] = __float_as_uint(x[e].x);
-                    wd[e] = __float_as_uint(g[e].x);
-                }
-                tmem_st_32x32b_x8(tm + sb * DA_SUB + c0, wp);
-                tmem_st_32x32b_x8(tm + 128 + sb * DA_SUB + c0, wd);
                 tmem_st_wait();
                 tcgen05_fence_before();
                 warp_arrive(&p_full[sb]);
@@ -1266,15 +1286,15 @@ doc_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             }
             // evaluated again by the warps of the rows' first owners, after all owners' stores
             const bool again = ok && live && !none && bad != 0.0f;
-            if (barrier_any(1, 512, again)) {
+            if (barrier_any(3, 512, again)) {
                 if (part == 0) stat[r] = 0.0f;
-                asm volatile("bar.sync 1, 512;" ::: "memory");
+                asm volatile("bar.sync 3, 512;" ::: "memory");
                 if (again) stat[r] = 1.0f;
                 da_patch_written();
-                asm volatile("bar.sync 1, 512;" ::: "memory");
+                asm volatile("bar.sync 3, 512;" ::: "memory");
                 const bool redo = stat[r] != 0.0f;
                 if (part == 0 && __any_sync(0xffffffffu, redo)) da_mend_dkv<D, CAP>(p, m.b, m.head, kj, qlo, qhi, redo);
-                asm volatile("bar.sync 1, 512;" ::: "memory");
+                asm volatile("bar.sync 3, 512;" ::: "memory");
             }
         }
         da_patch_free();                                // the patch is read before the CTA's shared memory goes
