@@ -1743,7 +1743,7 @@ static int da_check(const void* q, const void* k, const void* v, int64_t ld_q, i
     if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || (d != 64 && d != 128)) return BRK_ATTR_ERROR;
     if (heads > 4096 || tokens > (1 << 22) || (int64_t)batch * tokens > (1 << 30)) return BRK_ATTR_ERROR;
     if ((int64_t)batch * ((tokens + 127) / 128) * heads > 0x7fffffff) return BRK_ATTR_ERROR;
-    if (!(cap >= 0.0f) || cap > 1e4f) return BRK_ATTR_ERROR;
+    if (cap != 0.0f && !(cap >= 1e-6f && cap <= 1e4f)) return BRK_ATTR_ERROR;        // a NaN too; 1 / cap^2 stays finite
     if (ld_q % 8 != 0 || ld_kv % 8 != 0 || ld_out % 8 != 0 || ld_q < (int64_t)heads * d || ld_kv < (int64_t)kv_heads * d || ld_out < (int64_t)heads * d)
         return BRK_ATTR_ERROR;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(spans)) return BRK_ATTR_ERROR;

@@ -288,11 +288,13 @@ BRK_API int brk_doc_plan(const int32_t* mask, const int32_t* prompt, const int32
  * dk, dv: kv_heads heads, row strides ld_kv and ld_dkv (thirds of one fused buffer, or tensors of their own).  heads is a
  * multiple of kv_heads; query head h reads key head h / (heads / kv_heads), whose gradient is the sum over its query heads.
  * spans [batch, tokens, 4] as brk_doc_plan makes them: inside a row none of the four falls from a token to the next (other
- * values give wrong sums, never an access outside the tensors).  slopes [heads] fp32 or NULL; 0 <= cap <= 10000, 0 = none.
+ * values give wrong sums, never an access outside the tensors).  slopes [heads] fp32 or NULL; cap 0 (none) or 1e-6 to 10000.
  * A query that sees nothing (padding) has out = 0, lse = 0 and no gradient, a key that nobody sees has gradient 0; all rows of
- * the outputs are written.  What a query does not see does not reach it, NaN and infinity included.
+ * the outputs are written.  What a query does not see does not reach it, NaN and infinity included; a query that sees such a value
+ * may read NaN in all of its out, and so may the gradients that it takes part in.
  * lse [batch, heads, tokens] fp32, natural log (NULL when no backward follows).  The gradients are the same from run to run.
- * head_dim 64 or 128, tokens <= 2^22, batch * tokens <= 2^30, strides multiples of 8, pointers 16-byte aligned.
+ * head_dim 64 or 128, heads <= 4096, tokens <= 2^22, batch * tokens <= 2^30, batch * ceil(tokens / 128) * heads < 2^31, strides
+ * multiples of 8, pointers 16-byte aligned; no output overlaps another tensor of the call.
  * The backward's workspace is brk_doc_attn_bwd_workspace_bytes() of device scratch; calls that may run at the same time
  * need one each.  brk_doc_attn_status() (synchronous) returns non-zero if a kernel gave up on a bounded wait. */
 BRK_API int brk_doc_attn_fwd(const void* q, const void* k, const void* v, int64_t ld_q, int64_t ld_kv, void* out, int64_t ld_out,

@@ -91,3 +91,9 @@ def test_front_end_takes_cuda_tensors_only():
                  lambda: ops.doc_attn(*[torch.zeros(1, 4, 2, 64).half()] * 3, torch.zeros(1, 4, 4, dtype=torch.int32))):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_caps_outside_the_range_and_too_many_tiles():
+    for cap in (1e-7, 1e-30, 10001.0, -0.5, float("-inf")):
+        assert fwd(cap=cap) == brk.ATTR_ERROR and bwd(cap=cap) == brk.ATTR_ERROR
+    assert fwd(batch=1 << 21, tokens=256, heads=1024, kv=1024, ld_q=1 << 16, ld_kv=1 << 16, ld_out=1 << 16) == brk.ATTR_ERROR

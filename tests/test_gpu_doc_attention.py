@@ -332,3 +332,19 @@ def test_front_end_refuses_layouts_it_would_misread():
     from blackriver_b200 import brk
     with pytest.raises(brk.BrkError):
         o.doc_attn(x[:, :, :3], x[:, :, :2], x[:, :, 2:], spans)
+
+
+@pytest.mark.parametrize("cap", [1e-6, 1e4])
+def test_smallest_and_largest_cap(cap):
+    o = ops()
+    batch, tokens, heads, kv, d = 1, 200, 2, 1, 64
+    mask, prompt = rows(batch, tokens, [[120, 80]], 5)
+    spans = torch.tensor(ref.plan(mask, prompt)[0], dtype=torch.int32)
+    qkv, do = inputs(batch, tokens, heads, kv, d, 5)
+    want = ref.attention(*split(qkv, heads, kv), spans, None, cap, do)
+    out, lse = o.doc_attn(*split(qkv.cuda(), heads, kv), spans.cuda(), cap=cap)
+    got = dict(zip(("dq", "dk", "dv"), o.doc_attn_backward(do.cuda(), *split(qkv.cuda(), heads, kv), out, lse, spans.cuda(), cap=cap)))
+    assert status() == 0
+    for name, value in dict(got, out=out, lse=lse).items():
+        assert torch.isfinite(value.float()).all(), name
+        ref.assert_close(value, *want[name], name)
