@@ -13,8 +13,8 @@
 // rounding error by gamma.
 //
 // All of it is bound by HBM: one pass, 16-byte accesses, everything that a block shares travels by warp shuffles.  fp16:
-// GELU of [8192, 16384] 115 us forward and 163 us backward, 5.9 and 5.8 TB/s (gelu(x) written again with dx); LayerNorm of
-// [8192, 4096] 35 us and 62 us; [2048, 4096] packed in 6.0 us, unpacked in 5.4 us.
+// GELU of [8192, 16384] 119 us forward and 162 us backward, 5.7 and 5.8 TB/s (gelu(x) written again with dx); LayerNorm of
+// [8192, 4096] 35 us and 62 us; [2048, 4096] packed in 6.3 us, unpacked in 5.4 us.
 #include <mutex>
 
 #include "brk_common.cuh"
@@ -30,15 +30,18 @@ constexpr float A8_TINY = 1.5046328e-36f;     // 2^-119
 // largest magnitude as a bit pattern: NaN and infinity order above every number
 __device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// 127 / top, with EXACT in two parts, and the scale
 struct A8Scale {
-    float inv, scale;
+    float inv, rest, scale;
 };
-// EXACT: the quotient correctly rounded, for inputs whose ratios to the block's largest are simple fractions (halves of it
-// lie between two steps); normalised rows have none, and a rounding of 2^-22 there saves 20 instructions a block.
+// EXACT: x * 127 / top correctly rounded, so that a value in the middle between two steps (half of the block's largest, say:
+// a few fp16 values in ten thousand) stays there and goes to even as it does in exact arithmetic.  Normalised rows, in fp32, hold no such
+// values, and a rounding of 2^-22 there saves 20 instructions a block.
 template <bool EXACT = true>
 __device__ __forceinline__ A8Scale a8_scale(uint32_t top_bits) {
     A8Scale s;
     const float top = __uint_as_float(top_bits);
+    s.rest = 0.0f;
     if (top_bits >= 0x7f800000u) {
         s.inv = 0.0f;
         s.scale = __uint_as_float(0x7fffffffu);
@@ -47,6 +50,7 @@ __device__ __forceinline__ A8Scale a8_scale(uint32_t top_bits) {
         s.scale = 0.0f;
     } else {
         s.inv = EXACT ? __fdiv_rn(127.0f, top) : __fdividef(127.0f, top);
+        if (EXACT) s.rest = fmaf(-s.inv, top, 127.0f) * (s.inv * (1.0f / 127.0f));
         s.scale = top * (1.0f / 127.0f);
     }
     return s;
@@ -54,17 +58,22 @@ __device__ __forceinline__ A8Scale a8_scale(uint32_t top_bits) {
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 // Four values to four bytes.  Adding 1.5 * 2^23 leaves the nearest integer (ties to even) in the low mantissa bits, and
-// a byte permute gathers them: no conversion instruction, which would run at an eighth of the rate.  The product is rounded
-// before the sum, not fused with it: a value in the middle between two steps (half of the block's largest, say) then stays
-// there, and ties go to even as they do in exact arithmetic.  With inv == 0 the product is 0, or NaN for a value that is
-// not finite; its low byte is whatever it is, the block's scale is NaN then.
-__device__ __forceinline__ uint32_t a8_pack4(float2 a, float2 b, float inv) {
-    const float2 x = __fadd2_rn(__fmul2_rn(a, both(inv)), both(12582912.0f)), y = __fadd2_rn(__fmul2_rn(b, both(inv)), both(12582912.0f));
+// a byte permute gathers them: no conversion instruction, which would run at an eighth of the rate.  With inv == 0 the product is
+// 0, or NaN for a value that is not finite; its low byte is whatever it is, the block's scale is NaN then.
+template <bool EXACT = true>
+__device__ __forceinline__ float2 a8_step(float2 x, const A8Scale& s) {
+    return EXACT ? __ffma2_rn(x, both(s.inv), __fmul2_rn(x, both(s.rest))) : __fmul2_rn(x, both(s.inv));
+}
+template <bool EXACT = true>
+__device__ __forceinline__ uint32_t a8_pack4(float2 a, float2 b, const A8Scale& s) {
+    const float2 x = __fadd2_rn(a8_step<EXACT>(a, s), both(12582912.0f)), y = __fadd2_rn(a8_step<EXACT>(b, s), both(12582912.0f));
     return __byte_perm(__byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040), __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040), 0x5410);
 }
-__device__ __forceinline__ int8_t a8_pack1(float x, float inv) { return (int8_t)(__float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f)) & 0xff); }
-__device__ __forceinline__ uint4 a8_pack16(const float2 (&v)[8], float inv) {
-    return make_uint4(a8_pack4(v[0], v[1], inv), a8_pack4(v[2], v[3], inv), a8_pack4(v[4], v[5], inv), a8_pack4(v[6], v[7], inv));
+__device__ __forceinline__ int8_t a8_pack1(float x, const A8Scale& s) {
+    return (int8_t)(__float_as_uint(__fadd_rn(fmaf(x, s.inv, __fmul_rn(x, s.rest)), 12582912.0f)) & 0xff);
+}
+__device__ __forceinline__ uint4 a8_pack16(const float2 (&v)[8], const A8Scale& s) {
+    return make_uint4(a8_pack4(v[0], v[1], s), a8_pack4(v[2], v[3], s), a8_pack4(v[4], v[5], s), a8_pack4(v[6], v[7], s));
 }
 // Two bytes of a word as the numbers they stand for: 2^23 + (b + 128) assembled from its bits, exactly.
 template <int B>
@@ -178,7 +187,7 @@ a8_pack_kernel(const T* x, T* y, int8_t* __restrict__ q, float* __restrict__ sca
             for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
             if (unit[i].live) {
                 const A8Scale s = a8_scale(top);
-                __stcs(reinterpret_cast<uint4*>(q + unit[i].at), a8_pack16(v, s.inv));
+                __stcs(reinterpret_cast<uint4*>(q + unit[i].at), a8_pack16(v, s));
                 if ((threadIdx.x & 7) == 0) scale[(u0 + i * stride) >> 3] = s.scale;
                 if (GELU) {
 #pragma unroll
@@ -214,7 +223,7 @@ a8_pack_generic_kernel(const T* x, T* y, int8_t* q, float* scale, int64_t rows, 
         for (int i = 0; i < 4; i++) {
             const int c = i * 32 + lane;
             if (c0 + c < cols) {
-                q[at + c] = a8_pack1(v[i], s.inv);
+                q[at + c] = a8_pack1(v[i], s);
                 if (GELU) y[at + c] = from_f32<T>(gelu_terms<T>(v[i]).y);
             }
         }
@@ -527,7 +536,7 @@ a8_ln_fwd_kernel(const T* x, const T* __restrict__ gamma, const T* __restrict__ 
             const int c = c0 + k * cstep;
             if (c >= cols) continue;
             const A8Scale sc = a8_scale<false>(finite ? __float_as_uint(top[k]) : 0x7fffffffu);
-            __stcs(reinterpret_cast<uint2*>(qr + c), make_uint2(a8_pack4(v[4 * k], v[4 * k + 1], sc.inv), a8_pack4(v[4 * k + 2], v[4 * k + 3], sc.inv)));
+            __stcs(reinterpret_cast<uint2*>(qr + c), make_uint2(a8_pack4<false>(v[4 * k], v[4 * k + 1], sc), a8_pack4<false>(v[4 * k + 2], v[4 * k + 3], sc)));
             if ((threadIdx.x & 15) == 0) sr[c >> 7] = sc.scale;
             float2 o[4];
 #pragma unroll
@@ -575,7 +584,7 @@ a8_ln_fwd_generic_kernel(const T* x, const T* gamma, const T* beta, T* y, int8_t
         for (int i = 0; i < 4; i++) {
             const int c = b * A8_BLOCK + i * 32 + lane;
             if (c < cols) {
-                q[row * cols + c] = a8_pack1(v[i], sc.inv);
+                q[row * cols + c] = a8_pack1(v[i], sc);
                 y[row * cols + c] = from_f32<T>(fmaf(v[i], to_f32(gamma[c]), to_f32(beta[c])));
             }
         }

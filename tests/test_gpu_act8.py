@@ -234,3 +234,15 @@ def test_gelu_of_values_whose_square_overflows(cols):
     assert torch.equal(y, torch.where(x > 0, x, torch.zeros_like(x)))
     dx = o.gelu_backward_act8(torch.full_like(x, 3.0), q, scale)
     assert torch.equal(dx, torch.where(x > 0, 3.0, 0.0))
+
+
+@pytest.mark.parametrize("cols", [512, 131])
+def test_values_between_two_steps_go_to_even(cols):
+    o = ops()
+    x = torch.randn(700, cols, generator=torch.Generator().manual_seed(cols)).half()
+    x[:, 1] = (x[:, :128].abs().amax(1).float() / 2).half()
+    blocks = [x[:, at:at + 128] for at in range(0, cols, 128)]
+    # x * 127 is exact in 64 bits and a quotient that is a half stays one
+    want = torch.cat([torch.round(b.double() * 127 / b.double().abs().amax(1, keepdim=True)) for b in blocks], 1)
+    assert torch.equal(o.act8_pack(x.cuda())[0].double().cpu(), want)
+    assert torch.equal(o.gelu_act8(x.cuda())[1].double().cpu(), want)
