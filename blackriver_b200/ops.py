@@ -244,6 +244,22 @@ def _take(name, t, dtype, shape, device):
     return t.data_ptr()
 
 
+def _workspace(like, given, need, device):
+    """(address, bytes, tensor) of the workspace given, or of a new one."""
+    if given is None:
+        given = like.new_empty((max(need, 16),), dtype=torch.uint8)
+        return given.data_ptr(), max(need, 16), given
+    return _take("workspace", given, given.dtype, given.shape, device), given.numel() * given.element_size(), given
+
+
+def _result(name, t, like, device):
+    """(tensor, address) of an output of the type and shape of `like`: the one given, or a new one."""
+    if t is None:
+        t = torch.empty_like(like)
+        return t, t.data_ptr()
+    return t, _take(name, t, like.dtype, like.shape, device)
+
+
 def doc_plan(mask, prompt=None, ids=None):
     """Spans of packed documents: mask [batch, tokens] int32 numbers the documents (0 or less = padding), prompt marks
     the tokens of prompts.  Returns int32 spans [batch, tokens, 4] for doc_attn; with ids also the loss targets and their
@@ -300,11 +316,15 @@ def doc_attn(q, k, v, spans, slopes=None, cap=0.0, out=None, lse=None):
     device, b, n, h, hk, d, a_q, a_k, a_v, ld_q, ld_kv, a_spans, a_slopes = _doc_args(q, k, v, spans, slopes)
     if out is None:
         out = q.new_empty((b, n, h, d))
+        a_out, ld_out = out.data_ptr(), h * d
+    else:
+        a_out, ld_out = _heads("out", out, b, n, h, d, device)
     if lse is None:
         lse = q.new_empty((b, h, n), dtype=torch.float32)
-    a_out, ld_out = _heads("out", out, b, n, h, d, device)
-    brk.call("brk_doc_attn_fwd", a_q, a_k, a_v, ld_q, ld_kv, a_out, ld_out, _take("lse", lse, torch.float32, (b, h, n), device), a_spans, a_slopes, cap, b, n, h,
-             hk, d, stream())
+        a_lse = lse.data_ptr()
+    else:
+        a_lse = _take("lse", lse, torch.float32, (b, h, n), device)
+    brk.call("brk_doc_attn_fwd", a_q, a_k, a_v, ld_q, ld_kv, a_out, ld_out, a_lse, a_spans, a_slopes, cap, b, n, h, hk, d, stream())
     return out, lse
 
 
@@ -318,19 +338,21 @@ def doc_attn_backward(d_out, q, k, v, out, lse, spans, slopes=None, cap=0.0, dq=
         raise ValueError("out and d_out must have the same row stride")
     a_lse = _take("lse", lse, torch.float32, (b, h, n), device)
     if dq is None and dk is None and dv is None:
-        dq, dk, dv = q.new_empty((b, n, h + 2 * hk, d)).split((h, hk, hk), 2)
+        fused = q.new_empty((b, n, h + 2 * hk, d))
+        dq, dk, dv = fused.split_with_sizes((h, hk, hk), 2)
+        a_dq, ld_dq = fused.data_ptr(), (h + 2 * hk) * d
+        a_dk, a_dv, ld_dkv = a_dq + 2 * h * d, a_dq + 2 * (h + hk) * d, ld_dq
     elif dq is None or dk is None or dv is None:
         raise ValueError("give all of dq, dk and dv, or none")
-    a_dq, ld_dq = _heads("dq", dq, b, n, h, d, device)
-    a_dk, ld_dkv = _heads("dk", dk, b, n, hk, d, device)
-    a_dv, ld_dv = _heads("dv", dv, b, n, hk, d, device)
-    if ld_dv != ld_dkv:
-        raise ValueError("dk and dv must have the same row stride")
-    if workspace is None:
-        workspace = q.new_empty((max(brk.lib().brk_doc_attn_bwd_workspace_bytes(b, n, h), 16),), dtype=torch.uint8)
-    a_ws = _take("workspace", workspace, workspace.dtype, workspace.shape, device)
+    else:
+        a_dq, ld_dq = _heads("dq", dq, b, n, h, d, device)
+        a_dk, ld_dkv = _heads("dk", dk, b, n, hk, d, device)
+        a_dv, ld_dv = _heads("dv", dv, b, n, hk, d, device)
+        if ld_dv != ld_dkv:
+            raise ValueError("dk and dv must have the same row stride")
+    a_ws, ws_bytes, workspace = _workspace(q, workspace, brk.lib().brk_doc_attn_bwd_workspace_bytes(b, n, h), device)
     brk.call("brk_doc_attn_bwd", a_q, a_k, a_v, ld_q, ld_kv, a_out, a_do, ld_out, a_lse, a_dq, ld_dq, a_dk, a_dv, ld_dkv, a_spans, a_slopes, cap, b, n, h, hk, d,
-             a_ws, workspace.numel() * workspace.element_size(), stream())
+             a_ws, ws_bytes, stream())
     return dq, dk, dv
 
 
@@ -372,16 +394,19 @@ def act8_unpack(q, scale, dtype=torch.float16, out=None):
     a_q, a_scale = _act8_take(q, scale, rows, cols, device)
     if out is None:
         out = torch.empty_like(q, dtype=dtype)
-    brk.call("brk_act8_unpack", a_q, a_scale, _take("out", out, out.dtype, q.shape, device), rows, cols, _dt(out), stream())
+        a_out = out.data_ptr()
+    else:
+        a_out = _take("out", out, out.dtype, q.shape, device)
+    brk.call("brk_act8_unpack", a_q, a_scale, a_out, rows, cols, _dt(out), stream())
     return out
 
 
 def gelu_act8(x, out=None):
     """gelu(x) and x kept in 8 bits: (y, q, scale)."""
     device, rows, cols, a_x = _act8_like(x)
-    y = torch.empty_like(x) if out is None else out
+    y, a_y = _result("out", out, x, device)
     q, scale = _act8_new(x, rows, cols)
-    brk.call("brk_gelu_fwd_act8", a_x, _take("out", y, x.dtype, x.shape, device), q.data_ptr(), scale.data_ptr(), rows, cols, _dt(x), stream())
+    brk.call("brk_gelu_fwd_act8", a_x, a_y, q.data_ptr(), scale.data_ptr(), rows, cols, _dt(x), stream())
     return y, q, scale
 
 
@@ -389,9 +414,9 @@ def gelu_backward_act8(dy, q, scale, out=None, recompute=False):
     """dy * gelu'(kept x); with recompute also gelu(kept x) again: dx, or (dx, y)."""
     device, rows, cols, a_dy = _act8_like(dy)
     a_q, a_scale = _act8_take(q, scale, rows, cols, device)
-    dx = torch.empty_like(dy) if out is None else out
-    y = torch.empty_like(dy) if recompute else None
-    brk.call("brk_gelu_bwd_act8", a_dy, a_q, a_scale, _take("out", dx, dy.dtype, dy.shape, device), _ptr(y), rows, cols, _dt(dy), stream())
+    dx, a_dx = _result("out", out, dy, device)
+    y, a_y = _result("y", None, dy, device) if recompute else (None, 0)
+    brk.call("brk_gelu_bwd_act8", a_dy, a_q, a_scale, a_dx, a_y, rows, cols, _dt(dy), stream())
     return (dx, y) if recompute else dx
 
 
@@ -399,11 +424,10 @@ def layernorm_act8(x, gamma, beta, eps=1e-5, out=None):
     """LayerNorm that keeps the normalised rows in 8 bits: (y, q, scale, var)."""
     device, rows, cols, a_x = _act8_like(x)
     a_gamma, a_beta = _take("gamma", gamma, x.dtype, (cols,), device), _take("beta", beta, x.dtype, (cols,), device)
-    y = torch.empty_like(x) if out is None else out
+    y, a_y = _result("out", out, x, device)
     q, scale = _act8_new(x, rows, cols)
     var = x.new_empty((rows,), dtype=torch.float32)
-    brk.call("brk_layernorm_fwd_act8", a_x, a_gamma, a_beta, _take("out", y, x.dtype, x.shape, device), q.data_ptr(), scale.data_ptr(), var.data_ptr(), rows, cols,
-             eps, _dt(x), stream())
+    brk.call("brk_layernorm_fwd_act8", a_x, a_gamma, a_beta, a_y, q.data_ptr(), scale.data_ptr(), var.data_ptr(), rows, cols, eps, _dt(x), stream())
     return y, q, scale, var
 
 
@@ -412,22 +436,17 @@ def layernorm_backward_act8(dy, gamma, var, q, scale, beta=None, residual=None, 
     device, rows, cols, a_dy = _act8_like(dy)
     if accumulate and (dgamma is None or dbeta is None):
         raise ValueError("accumulate needs dgamma and dbeta")
-    dtype, vec, full = dy.dtype, (cols,), dy.shape
+    dtype, vec = dy.dtype, (cols,)
     a_q, a_scale = _act8_take(q, scale, rows, cols, device)
     a_gamma, a_beta = _take("gamma", gamma, dtype, vec, device), _take("beta", beta, dtype, vec, device)
-    if dgamma is None:
-        dgamma = torch.empty_like(gamma)
-    if dbeta is None:
-        dbeta = torch.empty_like(gamma)
-    if dx is None:
-        dx = torch.empty_like(dy)
-    y = torch.empty_like(dy) if beta is not None else None
-    if workspace is None:
-        workspace = dy.new_empty((max(brk.lib().brk_layernorm_bwd_act8_workspace_bytes(rows, cols), 16),), dtype=torch.uint8)
-    a_ws = _take("workspace", workspace, workspace.dtype, workspace.shape, device)
-    brk.call("brk_layernorm_bwd_act8", a_dy, a_gamma, a_beta, _take("var", var, torch.float32, (rows,), device), a_q, a_scale,
-             _take("residual", residual, dtype, full, device), _take("dgamma", dgamma, dtype, vec, device), _take("dbeta", dbeta, dtype, vec, device),
-             _take("dx", dx, dtype, full, device), _ptr(y), rows, cols, a_ws, workspace.numel() * workspace.element_size(), int(accumulate), _dt(dy), stream())
+    a_var, a_residual = _take("var", var, torch.float32, (rows,), device), _take("residual", residual, dtype, dy.shape, device)
+    dgamma, a_dgamma = _result("dgamma", dgamma, gamma, device)
+    dbeta, a_dbeta = _result("dbeta", dbeta, gamma, device)
+    dx, a_dx = _result("dx", dx, dy, device)
+    y, a_y = _result("y", None, dy, device) if beta is not None else (None, 0)
+    a_ws, ws_bytes, workspace = _workspace(dy, workspace, brk.lib().brk_layernorm_bwd_act8_workspace_bytes(rows, cols), device)
+    brk.call("brk_layernorm_bwd_act8", a_dy, a_gamma, a_beta, a_var, a_q, a_scale, a_residual, a_dgamma, a_dbeta, a_dx, a_y, rows, cols, a_ws, ws_bytes,
+             int(accumulate), _dt(dy), stream())
     return (dgamma, dbeta, dx) if y is None else (dgamma, dbeta, dx, y)
 
 
