@@ -348,3 +348,33 @@ def test_smallest_and_largest_cap(cap):
     for name, value in dict(got, out=out, lse=lse).items():
         assert torch.isfinite(value.float()).all(), name
         ref.assert_close(value, *want[name], name)
+
+
+def test_two_streams_at_once_and_inputs_overwritten_right_behind_the_call():
+    o = ops()
+    batch, tokens, heads, kv, d = 2, 900, 8, 2, 128
+    mask, prompt = rows(batch, tokens, [[500, 400], [30, -20, 850]], 9)
+    spans = torch.tensor(ref.plan(mask, prompt)[0], dtype=torch.int32).cuda()
+    sets = [tuple(x.cuda() for x in inputs(batch, tokens, heads, kv, d, seed)) for seed in (1, 2)]
+
+    def run(qkv, do):
+        out, lse = o.doc_attn(*split(qkv, heads, kv), spans, cap=20.0)
+        return (out, lse) + tuple(o.doc_attn_backward(do, *split(qkv, heads, kv), out, lse, spans, cap=20.0))
+
+    want = [run(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        got = []
+        for st, (qkv, do) in zip(streams, sets):
+            with torch.cuda.stream(st):
+                a, b = qkv.clone(), do.clone()
+                r = run(a, b)
+                a.fill_(float("nan"))          # the backward's last kernel starts before the one in front of it ends
+                b.fill_(float("nan"))
+                got.append((r, a, b))
+        torch.cuda.synchronize()
+        for (r, _, _), w in zip(got, want):
+            for x, y in zip(r, w):
+                assert torch.equal(x, y)
+    assert status() == 0
