@@ -219,7 +219,7 @@ def _device(t):
     """The current device, which `t` has to be on: the kernels are queued on its current stream."""
     if not t.is_cuda:
         raise RuntimeError("blackriver_b200 operators run on CUDA tensors only (no CPU path)")
-    device = torch.cuda.current_device()
+    device = torch._C._cuda_getDevice()
     if t.get_device() != device:
         raise RuntimeError("tensors must live on the current device, whose stream the kernels are queued on")
     return device
@@ -244,10 +244,13 @@ def _take(name, t, dtype, shape, device):
     return t.data_ptr()
 
 
+_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _workspace(like, given, need, device):
     """(address, bytes, tensor) of the workspace given, or of a new one."""
     if given is None:
-        given = like.new_empty((max(need, 16),), dtype=torch.uint8)
+        given = torch.empty(max(need, 16), dtype=torch.uint8, device=like.device)
         return given.data_ptr(), max(need, 16), given
     return _take("workspace", given, given.dtype, given.shape, device), given.numel() * given.element_size(), given
 
@@ -272,11 +275,11 @@ def doc_plan(mask, prompt=None, ids=None):
     a_mask, a_prompt, a_ids = (_take(n, x, torch.int32, shape, device) for n, x in (("mask", mask), ("prompt", prompt), ("ids", ids)))
     spans = mask.new_empty((b, t, 4))
     if ids is None:
-        brk.call("brk_doc_plan", a_mask, a_prompt, 0, b, t, spans.data_ptr(), 0, 0, stream())
+        brk.call("brk_doc_plan", a_mask, a_prompt, 0, b, t, spans.data_ptr(), 0, 0, _stream(device))
         return spans
     target = torch.empty_like(ids)
     count = ids.new_empty((1,))
-    brk.call("brk_doc_plan", a_mask, a_prompt, a_ids, b, t, spans.data_ptr(), target.data_ptr(), count.data_ptr(), stream())
+    brk.call("brk_doc_plan", a_mask, a_prompt, a_ids, b, t, spans.data_ptr(), target.data_ptr(), count.data_ptr(), _stream(device))
     return spans, target, count
 
 
@@ -320,11 +323,11 @@ def doc_attn(q, k, v, spans, slopes=None, cap=0.0, out=None, lse=None):
     else:
         a_out, ld_out = _heads("out", out, b, n, h, d, device)
     if lse is None:
-        lse = q.new_empty((b, h, n), dtype=torch.float32)
+        lse = torch.empty(b, h, n, dtype=torch.float32, device=q.device)
         a_lse = lse.data_ptr()
     else:
         a_lse = _take("lse", lse, torch.float32, (b, h, n), device)
-    brk.call("brk_doc_attn_fwd", a_q, a_k, a_v, ld_q, ld_kv, a_out, ld_out, a_lse, a_spans, a_slopes, cap, b, n, h, hk, d, stream())
+    brk.call("brk_doc_attn_fwd", a_q, a_k, a_v, ld_q, ld_kv, a_out, ld_out, a_lse, a_spans, a_slopes, cap, b, n, h, hk, d, _stream(device))
     return out, lse
 
 
@@ -352,7 +355,7 @@ def doc_attn_backward(d_out, q, k, v, out, lse, spans, slopes=None, cap=0.0, dq=
             raise ValueError("dk and dv must have the same row stride")
     a_ws, ws_bytes, workspace = _workspace(q, workspace, brk.lib().brk_doc_attn_bwd_workspace_bytes(b, n, h), device)
     brk.call("brk_doc_attn_bwd", a_q, a_k, a_v, ld_q, ld_kv, a_out, a_do, ld_out, a_lse, a_dq, ld_dq, a_dk, a_dv, ld_dkv, a_spans, a_slopes, cap, b, n, h, hk, d,
-             a_ws, ws_bytes, stream())
+             a_ws, ws_bytes, _stream(device))
     return dq, dk, dv
 
 
@@ -373,7 +376,7 @@ def _act8_like(t):
 
 def _act8_new(t, rows, cols):
     q = torch.empty_like(t, dtype=torch.int8) if t.dim() == 2 else t.new_empty((rows, cols), dtype=torch.int8)
-    return q, t.new_empty((rows, -(-cols // ACT8_BLOCK)), dtype=torch.float32)
+    return q, torch.empty(rows, -(-cols // ACT8_BLOCK), dtype=torch.float32, device=t.device)
 
 
 def _act8_take(q, scale, rows, cols, device):
@@ -384,7 +387,7 @@ def act8_pack(x):
     """x [..., cols] -> (q int8 [rows, cols], scale fp32 [rows, ceil(cols / 128)])."""
     device, rows, cols, a_x = _act8_like(x)
     q, scale = _act8_new(x, rows, cols)
-    brk.call("brk_act8_pack", a_x, q.data_ptr(), scale.data_ptr(), rows, cols, _dt(x), stream())
+    brk.call("brk_act8_pack", a_x, q.data_ptr(), scale.data_ptr(), rows, cols, _dt(x), _stream(device))
     return q, scale
 
 
@@ -397,7 +400,7 @@ def act8_unpack(q, scale, dtype=torch.float16, out=None):
         a_out = out.data_ptr()
     else:
         a_out = _take("out", out, out.dtype, q.shape, device)
-    brk.call("brk_act8_unpack", a_q, a_scale, a_out, rows, cols, _dt(out), stream())
+    brk.call("brk_act8_unpack", a_q, a_scale, a_out, rows, cols, _dt(out), _stream(device))
     return out
 
 
@@ -406,7 +409,7 @@ def gelu_act8(x, out=None):
     device, rows, cols, a_x = _act8_like(x)
     y, a_y = _result("out", out, x, device)
     q, scale = _act8_new(x, rows, cols)
-    brk.call("brk_gelu_fwd_act8", a_x, a_y, q.data_ptr(), scale.data_ptr(), rows, cols, _dt(x), stream())
+    brk.call("brk_gelu_fwd_act8", a_x, a_y, q.data_ptr(), scale.data_ptr(), rows, cols, _dt(x), _stream(device))
     return y, q, scale
 
 
@@ -416,7 +419,7 @@ def gelu_backward_act8(dy, q, scale, out=None, recompute=False):
     a_q, a_scale = _act8_take(q, scale, rows, cols, device)
     dx, a_dx = _result("out", out, dy, device)
     y, a_y = _result("y", None, dy, device) if recompute else (None, 0)
-    brk.call("brk_gelu_bwd_act8", a_dy, a_q, a_scale, a_dx, a_y, rows, cols, _dt(dy), stream())
+    brk.call("brk_gelu_bwd_act8", a_dy, a_q, a_scale, a_dx, a_y, rows, cols, _dt(dy), _stream(device))
     return (dx, y) if recompute else dx
 
 
@@ -426,8 +429,8 @@ def layernorm_act8(x, gamma, beta, eps=1e-5, out=None):
     a_gamma, a_beta = _take("gamma", gamma, x.dtype, (cols,), device), _take("beta", beta, x.dtype, (cols,), device)
     y, a_y = _result("out", out, x, device)
     q, scale = _act8_new(x, rows, cols)
-    var = x.new_empty((rows,), dtype=torch.float32)
-    brk.call("brk_layernorm_fwd_act8", a_x, a_gamma, a_beta, a_y, q.data_ptr(), scale.data_ptr(), var.data_ptr(), rows, cols, eps, _dt(x), stream())
+    var = torch.empty(rows, dtype=torch.float32, device=x.device)
+    brk.call("brk_layernorm_fwd_act8", a_x, a_gamma, a_beta, a_y, q.data_ptr(), scale.data_ptr(), var.data_ptr(), rows, cols, eps, _dt(x), _stream(device))
     return y, q, scale, var
 
 
@@ -446,7 +449,7 @@ def layernorm_backward_act8(dy, gamma, var, q, scale, beta=None, residual=None, 
     y, a_y = _result("y", None, dy, device) if beta is not None else (None, 0)
     a_ws, ws_bytes, workspace = _workspace(dy, workspace, brk.lib().brk_layernorm_bwd_act8_workspace_bytes(rows, cols), device)
     brk.call("brk_layernorm_bwd_act8", a_dy, a_gamma, a_beta, a_var, a_q, a_scale, a_residual, a_dgamma, a_dbeta, a_dx, a_y, rows, cols, a_ws, ws_bytes,
-             int(accumulate), _dt(dy), stream())
+             int(accumulate), _dt(dy), _stream(device))
     return (dgamma, dbeta, dx) if y is None else (dgamma, dbeta, dx, y)
 
 
