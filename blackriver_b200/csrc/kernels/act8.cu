@@ -34,9 +34,9 @@ __device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x
 struct A8Scale {
     float inv, rest, scale;
 };
-// EXACT: x * 127 / top correctly rounded, so that a value in the middle between two steps (half of the block's largest, say:
-// a few fp16 values in ten thousand) stays there and goes to even as it does in exact arithmetic.  Normalised rows, in fp32, hold no such
-// values, and a rounding of 2^-22 there saves 20 instructions a block.
+// EXACT: x * 127 / top correctly rounded, so that a value in the middle between two steps (half of the block's largest, say; a
+// few fp16 values in ten thousand) stays there and goes to even as it does in exact arithmetic.  Normalised rows, in fp32,
+// hold no such values, and a rounding of 2^-22 there saves 20 instructions a block.
 template <bool EXACT = true>
 __device__ __forceinline__ A8Scale a8_scale(uint32_t top_bits) {
     A8Scale s;
