@@ -362,12 +362,13 @@ BR_WORD(LossBackwardW, {
     t[0]->op_loss_backward_w(t[0], t[1], t[2]);
 })
 // ( -- code )  waits for the device; 0 when no tensor-core kernel gave up a bounded wait and no optimizer launch met a
-// non-finite gradient since the last query, else 256 * (Adam status) + 16 * (GEMM status) + (attention status, of either kind)
+// non-finite gradient since the last query, else 256 * (Adam status) + 16 * (GEMM status) + (attention status, of either kind: that of
+// packed documents counts as 1)
 BR_WORD(KernelStatus, {
     int code = 0;
     if (ComputingContext::booted) {
         BR_CUDA_CHECK(cudaStreamSynchronize(ComputingContext::cuda_stream));
-        code = 256 * brk_adam_status() + 16 * brk_gemm_f16_status() + (brk_flash_attn_status() | brk_doc_attn_status());
+        code = 256 * brk_adam_status() + 16 * brk_gemm_f16_status() + (brk_flash_attn_status() | (brk_doc_attn_status() != 0 ? 1 : 0));
     }
     stack.push_number((double)code);
 })
