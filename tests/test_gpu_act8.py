@@ -246,3 +246,17 @@ def test_values_between_two_steps_go_to_even(cols):
     want = torch.cat([torch.round(b.double() * 127 / b.double().abs().amax(1, keepdim=True)) for b in blocks], 1)
     assert torch.equal(o.act8_pack(x.cuda())[0].double().cpu(), want)
     assert torch.equal(o.gelu_act8(x.cuda())[1].double().cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_layernorm_of_rows_of_one_value(dtype):
+    o = ops()
+    x, gamma, beta = data(5, 1, dtype, 3).cuda(), torch.full((1,), 2.0, dtype=dtype, device="cuda"), torch.full((1,), 0.5, dtype=dtype, device="cuda")
+    y, q, scale, var = o.layernorm_act8(x, gamma, beta, 1e-3)
+    assert torch.equal(y, beta.expand(5, 1)) and not q.any() and not scale.any()
+    assert ((var - 1e-3).abs() <= 1e-3 * 2.0 ** -23).all()
+    dy = data(5, 1, dtype, 4).cuda()
+    dgamma, dbeta, dx, again = o.layernorm_backward_act8(dy, gamma, var, q, scale, beta=beta)
+    assert not dgamma.any() and not dx.any() and torch.equal(again, y)
+    total = dy.double().sum()
+    assert (dbeta.double() - total).abs() <= total.abs() * torch.finfo(dtype).eps / 2 + dy.double().abs().sum() * 2.0 ** -21
